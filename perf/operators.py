@@ -183,8 +183,7 @@ def prepare(case: dict, seed: int) -> dict:
         state.update(plain_plan(state))
         state["pool"] = filled_pool(case, pages, gen)
     if case["kind"] == "append":
-        width = (heads + 2 * kv_heads) * dim
-        state["qkv"] = torch.randn(rows, width, device=DEV, generator=gen).bfloat16()
+        state["qkv"] = torch.randn(rows, (heads + 2 * kv_heads) * dim, device=DEV, generator=gen).bfloat16()
         state["gain"] = [1 + 0.1 * torch.randn(dim, device=DEV, generator=gen) for _ in "qk"]
         angles = torch.arange(max(a + b for a, b in zip(*lengths(case))), dtype=F64, device=DEV)[:, None] * THETA ** -(torch.arange(0, dim, 2, dtype=F64, device=DEV) / dim)
         state["cos"], state["sin"] = angles.cos().float(), angles.sin().float()
