@@ -52,7 +52,9 @@ enum {
 enum {
     NCB_DEV_BAD_POSITION = 1, /* kv_append_fp8: a row's position or slot is outside the cache; the row was skipped */
     NCB_DEV_WAIT_TIMEOUT = 2, /* decode_attn_fp8: a bounded wait on a copy barrier ran out; outputs are invalid */
-    NCB_DEV_BAD_LENGTH = 4    /* decode_attn_fp8: a length or slot is outside the cache; the sequence was skipped */
+    NCB_DEV_BAD_LENGTH = 4,   /* decode_attn_fp8: a length or slot is outside the cache; the sequence was skipped */
+    NCB_DEV_NO_PAGES = 8,     /* page_plan: the free pages do not last for every request; those behind were not served */
+    NCB_DEV_BAD_PAGE = 16     /* page_plan, paged_*: a page outside the pool in a block table, a free list or a place; it was left out */
 };
 
 const char *ncb_status_string(int status);
@@ -623,6 +625,66 @@ int delta_tokens(const ncb_delta *args, int f32, void *stream);
 int delta_chunk_tokens(int dim, int vdim, int taps, int rank_a, int rank_g);
 int delta_chunked(const ncb_delta *args, void *stream);
 int delta_step(const ncb_delta *args, int f32, void *stream);
+
+/* ---- library page_plan -------------------------------------------------------------------------------------------------
+ * A pool of pages shared by requests of any length, in place of slots of one size. Page: 64 positions of one request, in one layer's
+ * pool [n_pages][kv_heads] of NCB_PAGE_BYTES records (e4m3, the layout above) or of bf16 [2][64][128] (keys, then values). One block table
+ * int32 [requests][width] (request, position / 64) -> page serves the pools of every layer; a page belongs to one request.
+ *   page_plan     one step's bookkeeping in one launch. Request b holds `cached` positions and adds `fresh` ones, whose rows lie one after
+ *                 the other in the step's row buffers: row_start [requests + 1] = sums of max(fresh, 0). Pages come from the end of the
+ *                 list `free_pages` [n_pages], of which *free_count are in use; *free_left (may be free_count) is what stays; lens may be cached. Requests
+ *                 are served in order; one that needs pages and cannot have all of them is not served (NCB_DEV_NO_PAGES), nor is one
+ *                 with a negative length, more positions than the table has room for, more fresh rows than max_fresh, or rows past
+ *                 `rows` (NCB_DEV_BAD_LENGTH). out: table's new entries; served [requests] = fresh where served, else 0; lens
+ *                 [requests] = positions held after the step; per row position, place (page * 64 + position % 64) and request;
+ *                 -1, -1 for rows of requests not served and -1 in all three behind the last request.
+ *                 work: for each of n_windows windows the schedule of that layer kind's paged_attn calls, page_plan_words() words,
+ *                 in units that fill `blocks` blocks; a schedule holds for `group` query heads per key/value head.
+ *                 ticket: one word, zero before the first call and after each. At most NCB_PLAN_REQUESTS requests, 64 heads a group.
+ *   page_release  requests with release[b] != 0 give back the pages of their lens[b] positions: their entries become -1, lens 0, the
+ *                 pages go to the end of the free list. A request whose entries are not in the pool gives back none of those.
+ */
+#define NCB_PLAN_REQUESTS 8192
+#define NCB_PLAN_WINDOWS 8
+typedef struct {
+    int *table;
+    const int *cached, *fresh, *free_pages, *free_count;
+    int *free_left, *row_start, *served, *lens, *pos, *place, *request, *work, *ticket, *status;
+    long long rows;
+    int requests, width, n_pages, max_fresh, group, kv_heads, blocks, n_windows;
+    int windows[NCB_PLAN_WINDOWS]; /* 0: none */
+} ncb_page_plan;
+long long page_plan_words(int requests, long long rows, int max_fresh, int group, int kv_heads, int blocks); /* of one window; -1: refused */
+int page_plan(const ncb_page_plan *args, void *stream);
+int page_release(int *table, int *lens, const int *release, int *free_pages, int *free_count, int requests, int width, int n_pages, int *status,
+                 void *stream);
+
+/* ---- library paged_append ----------------------------------------------------------------------------------------------
+ * kv_append_fp8 (same arithmetic, same bits) with a row's k and v stored at place[row] = page * 64 + position % 64 of the pool; bf16 pools
+ * take the rotated keys and the values as they are. A row with a negative position or place is idle: nothing is written for it, q_out
+ * included. A position outside the tables or a place outside the pool is flagged and skipped the same way. */
+int paged_append(const void *qkv, const void *q_gain, const void *k_gain, const void *cos, const void *sin, const void *pos, const void *place,
+                 void *q_out, void *pool, long long rows, int Hq, int Hkv, long long qkv_row_stride, int table_len, int n_pages, int e4m3,
+                 void *status, void *stream);
+
+/* ---- library paged_attn ------------------------------------------------------------------------------------------------
+ * Causal attention of every request's new rows over its pages, after page_plan and paged_append: row i of request b, at position
+ * p = lens[b] - served[b] + i, attends positions (p - window, p]. q bf16 [rows][ldq], out bf16 [rows][ldo]: Hq heads of 128. `work` is
+ * page_plan's schedule for this window, made with the same requests, rows, max_fresh, group and kv_heads; `blocks` of page_plan is
+ * paged_attn_blocks(). Rows of requests that were not served become zeros; rows behind the last request are left as they were.
+ * workspace: paged_attn_workspace_bytes(), 16-byte aligned, for calls on one stream at a time. */
+typedef struct {
+    const void *q, *pool;
+    void *out, *workspace;
+    const int *table, *row_start, *served, *lens, *work;
+    int *status;
+    long long rows, ldq, ldo, workspace_bytes;
+    int requests, width, n_pages, max_fresh, Hq, Hkv, e4m3, window, blocks;
+    float scale;
+} ncb_paged;
+int paged_attn_blocks(void);
+long long paged_attn_workspace_bytes(int requests, long long rows, int max_fresh, int Hq, int Hkv, int blocks);
+int paged_attn(const ncb_paged *args, void *stream);
 
 /* ---- GEMMs around an fp32 residual stream (ncb_gemm_rs above) ------------------------------------------------
  * Shapes as for the plain entry points: skinny_gemm_rs at most 16 rows, K as skinny_gemm without norm, N a multiple of 8,

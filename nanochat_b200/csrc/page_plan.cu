@@ -1,0 +1,378 @@
+/*
+ * page_plan: block tables, positions and places of one step from the requests' lengths, on the GPU, so that a captured step serves
+ * lengths that change; page_release: finished requests give their pages back. No counterpart in the reference, whose slots are of
+ * one size (inference/decoder.py:112-121).
+ *
+ * Every block repeats the same two prefix sums over the requests (rows, then new pages) in shared memory, 16 KB for a thousand requests,
+ * instead of waiting for a launch that makes them once; then the row blocks write rows and table entries, each finding its
+ * request by a binary search in the sums, and one block per window cuts the attention's work into entries (paged.cuh). A step's bytes
+ * are a few per row, so the launch is bound by latency: the chain of sums and searches.
+ */
+#include "paged.cuh"
+
+namespace {
+
+using namespace paged;
+
+constexpr int THREADS = 1024, WARPS = THREADS / 32;
+constexpr int LISTED = 16384; /* owners whose pages are kept in shared memory; where there are more, none is cut */
+constexpr int MIN_CHUNK = 2;  /* pages of a chunk */
+constexpr int OVERHEAD = 3;   /* what starting and ending a chunk costs, in pages */
+constexpr int WHOLE = 1 << 28; /* a chunk size that cuts nothing: a table is at most 2^24 wide */
+
+/* Exclusive prefix sum of v over the block's threads; *total gets the sum. */
+__device__ __forceinline__ long long block_sum_before(long long v, long long *sums, long long *total) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    long long upto = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long x = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += x;
+    }
+    __syncthreads(); /* the sums of the call before have been read */
+    if (lane == 31) sums[warp] = upto;
+    __syncthreads();
+    long long w = sums[lane]; /* every warp sums the warps' sums for itself: no third barrier */
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long x = __shfl_up_sync(0xffffffffu, w, o);
+        if (lane >= o) w += x;
+    }
+    *total = __shfl_sync(0xffffffffu, w, 31);
+    const long long before = __shfl_sync(0xffffffffu, w, warp > 0 ? warp - 1 : 0);
+    return (warp > 0 ? before : 0) + upto - v;
+}
+
+/* The first index whose value is greater than x in an ascending array. */
+__device__ __forceinline__ int first_above(const int *a, int n, int x) {
+    int low = 0, high = n;
+    while (low < high) {
+        const int mid = (low + high) >> 1;
+        if (a[mid] > x) high = mid;
+        else low = mid + 1;
+    }
+    return low;
+}
+
+__device__ __forceinline__ int pages_for(long long positions) { return (int)((positions + PAGE_TOKENS - 1) / PAGE_TOKENS); }
+__device__ __forceinline__ int clamp_int(long long v) { return v > 0x7fffffffll ? 0x7fffffff : (int)v; }
+
+struct Requests { /* shared memory, one value a request each */
+    int *row_end, *page_end; /* inclusive sums of rows and of new pages */
+    int *cached, *served;    /* served: rows, 0 for a request that is not */
+    int *owner_end;          /* schedule blocks: inclusive sum of owners */
+    uint32_t *owner_pages;
+};
+
+struct Cut {
+    int pages, chunks, len; /* of one owner */
+    __device__ Cut(int pages, int chunk) : pages(pages) {
+        chunks = pages > 0 ? (pages + chunk - 1) / chunk : 1;
+        len = (pages + chunks - 1) / chunks; /* evened out: no stub at the end */
+    }
+};
+
+/* The schedule of one window's attention. */
+__device__ void schedule(const ncb_page_plan &a, const Requests &r, int window, int *work, long long *sums) {
+    __shared__ unsigned long long best;
+    const Caps caps = caps_of(a.requests, a.rows, a.max_fresh, a.group, a.kv_heads, a.blocks);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, per = (a.requests + THREADS - 1) / THREADS, b0 = tid * per;
+    const int rows_per = SPLIT_SLOTS / a.group, rows = (int)a.rows, units = units_of(a.blocks, a.kv_heads);
+    auto rows_of = [&](int b) { return min(r.row_end[b], rows) - min(b ? r.row_end[b - 1] : 0, rows); }; /* not served ones among them: zeros to write */
+    long long total, mine = 0;
+    for (int b = b0; b < min(b0 + per, a.requests); b++) mine += (rows_of(b) + rows_per - 1) / rows_per;
+    long long at = block_sum_before(mine, sums, &total);
+    for (int b = b0; b < min(b0 + per, a.requests); b++) r.owner_end[b] = (int)(at += (rows_of(b) + rows_per - 1) / rows_per);
+    __syncthreads();
+    const int owners = (int)total;
+    struct Owner { int request, row0, rows, page0, page1; };
+    auto owner = [&](int o) {
+        Owner w;
+        w.request = first_above(r.owner_end, a.requests, o);
+        const int n = rows_of(w.request);
+        w.row0 = (o - (w.request ? r.owner_end[w.request - 1] : 0)) * rows_per;
+        w.rows = min(rows_per, n - w.row0);
+        w.page0 = w.page1 = 0;
+        if (r.served[w.request] > 0) {
+            const int first = r.cached[w.request] + w.row0;
+            w.page0 = window > 0 && first + 1 > window ? (first + 1 - window) / PAGE_TOKENS : 0;
+            w.page1 = (first + w.rows - 1) / PAGE_TOKENS + 1;
+        }
+        return w;
+    };
+    const bool listed = owners <= LISTED;
+    long long sum = 0;
+    for (int o = tid; o < owners; o += THREADS) {
+        const Owner w = owner(o);
+        sum += w.page1 - w.page0;
+        if (listed) r.owner_pages[o] = w.page1 - w.page0;
+    }
+    if (tid == 0) best = ~0ull;
+    long long pages;
+    block_sum_before(sum, sums, &pages); /* its barriers also publish owner_pages and best */
+    int chunk = WHOLE;
+    if (listed && pages > 0) {
+        /* Each warp estimates the time of one chunk size: the longest entry where all run at once, else the mean load and half an entry of
+         * tail. Warp 0: nothing is cut. */
+        const long long waves = 1 + warp; /* in eighths: chunks of four times an even share of the units' work down to a quarter of one */
+        const int c = warp == 0 ? WHOLE : (int)max((long long)MIN_CHUNK, (8 * pages + units * waves - 1) / (units * waves));
+        long long n = 0;
+        int longest = 0;
+        for (int o = lane; o < owners; o += 32) {
+            const Cut cut(r.owner_pages[o], c);
+            n += cut.chunks;
+            longest = max(longest, cut.len);
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            n += __shfl_xor_sync(0xffffffffu, n, o);
+            longest = max(longest, __shfl_xor_sync(0xffffffffu, longest, o));
+        }
+        const long long even = 16 * (pages + n * OVERHEAD) / units; /* in sixteenths of a page */
+        const long long cost = n <= units ? 16ll * (longest + OVERHEAD) : max(even + 8ll * longest, 16ll * (longest + OVERHEAD));
+        const long long merge = n > owners ? 16ll * OVERHEAD : 0; /* and their states are read again */
+        if (lane == 0) atomicMin(&best, (unsigned long long)(cost + merge) << 32 | (unsigned)warp);
+        __syncthreads();
+        const int chosen = (int)(best & 0xffffffffu);
+        const long long w = 1 + chosen;
+        if (chosen > 0) chunk = (int)max((long long)MIN_CHUNK, (8 * pages + units * w - 1) / (units * w));
+    }
+    Entry *entries = reinterpret_cast<Entry *>(work + HEADER_WORDS);
+    Merge *merges = reinterpret_cast<Merge *>(work + HEADER_WORDS + caps.entries * ENTRY_WORDS);
+    long long n_entries = 0, n_parts = 0, n_merges = 0;
+    for (int from = 0; from < owners; from += THREADS) { /* the last rows of a request reach furthest: they start first */
+        const int o = owners - 1 - from - tid;
+        Owner w = {};
+        int chunks = 0, len = 0;
+        if (o >= 0) {
+            w = owner(o);
+            const Cut cut(w.page1 - w.page0, chunk);
+            chunks = cut.chunks, len = cut.len;
+        }
+        const int parts = chunks > 1 ? chunks : 0;
+        long long t, t2; /* entries; parts, and merges above them */
+        const long long e = n_entries + block_sum_before(chunks, sums, &t), pm = block_sum_before(parts | (long long)(parts > 0) << 32, sums, &t2);
+        const long long p = n_parts + (pm & 0xffffffffll), m = n_merges + (pm >> 32);
+        for (int c = 0; c < chunks; c++) {
+            if (e + c >= caps.entries || (parts && p + c >= caps.parts)) break; /* cannot be: see Caps */
+            Entry x = {w.request, w.row0, w.rows, w.page0 + c * len, min(w.page0 + (c + 1) * len, w.page1), parts ? (int)p + c : -1, {0, 0}};
+            entries[e + c] = x;
+        }
+        if (parts && m < caps.merges) merges[m] = Merge{(w.request ? r.row_end[w.request - 1] : 0) + w.row0, w.rows, (int)p, parts};
+        n_entries += t, n_parts += t2 & 0xffffffffll, n_merges += t2 >> 32;
+    }
+    if (tid == 0) work[0] = (int)min(n_entries, caps.entries), work[1] = (int)min(n_merges, caps.merges);
+}
+
+struct PlanArgs {
+    ncb_page_plan p;
+    int row_blocks;
+    long long words;
+};
+
+__global__ void __launch_bounds__(THREADS) k_page_plan(const PlanArgs args) {
+    extern __shared__ __align__(16) int smem[];
+    __shared__ long long sums[WARPS];
+    __shared__ int last;
+    const ncb_page_plan &a = args.p;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const int tid = threadIdx.x, n = a.requests, per = (n + THREADS - 1) / THREADS, b0 = tid * per, end = min(b0 + per, n);
+    const Requests r = {smem, smem + n, smem + 2 * n, smem + 3 * n, smem + 4 * n, reinterpret_cast<uint32_t *>(smem + 5 * n)};
+    const int free_count = max(0, min(*reinterpret_cast<const volatile int *>(a.free_count), a.n_pages));
+    for (int b = tid; b < n; b += THREADS) r.cached[b] = a.cached[b], r.served[b] = a.fresh[b];
+    __syncthreads();
+    long long total, mine = 0;
+    for (int b = b0; b < end; b++) mine += max(r.served[b], 0);
+    long long at = block_sum_before(mine, sums, &total);
+    const int rows_used = clamp_int(min(total, a.rows));
+    bool bad = false;
+    mine = 0;
+    for (int b = b0; b < end; b++) {
+        const int cached = r.cached[b], fresh = r.served[b];
+        at += max(fresh, 0);
+        r.row_end[b] = clamp_int(at);
+        const bool ok = cached >= 0 && fresh >= 0 && fresh <= a.max_fresh && (long long)cached + fresh <= (long long)a.width * PAGE_TOKENS && (fresh == 0 || at <= a.rows);
+        bad |= !ok;
+        if (!ok || fresh == 0) r.served[b] = 0;
+        else mine += pages_for((long long)cached + fresh) - pages_for(cached);
+    }
+    long long new_pages;
+    at = block_sum_before(mine, sums, &new_pages);
+    bool none = false;
+    mine = 0; /* pages that are taken */
+    for (int b = b0; b < end; b++) {
+        const int fresh = r.served[b], need = fresh > 0 ? pages_for((long long)r.cached[b] + fresh) - pages_for(r.cached[b]) : 0;
+        at += need;
+        r.page_end[b] = clamp_int(at);
+        if (need > 0 && at > free_count) r.served[b] = 0, none = true;
+        else mine += need;
+    }
+    long long taken;
+    block_sum_before(mine, sums, &taken); /* its barriers publish the arrays */
+    if (blockIdx.x >= args.row_blocks) {
+        const int w = blockIdx.x - args.row_blocks;
+        schedule(a, r, a.windows[w], a.work + w * args.words, sums);
+    } else {
+        if (blockIdx.x == 0) {
+            if (bad) flag(a.status, NCB_DEV_BAD_LENGTH);
+            if (none) flag(a.status, NCB_DEV_NO_PAGES);
+            for (int b = tid; b < n; b += THREADS) {
+                a.row_start[b + 1] = r.row_end[b];
+                a.served[b] = r.served[b];
+            }
+            if (tid == 0) a.row_start[0] = 0;
+        }
+        /* page i of request b's new ones; i and b must be in range */
+        auto new_page = [&](int b, int i) {
+            const int before = b ? r.page_end[b - 1] : 0, from = free_count - 1 - before - i;
+            const int page = from >= 0 ? a.free_pages[from] : -1;
+            if ((unsigned)page < (unsigned)a.n_pages) return page;
+            flag(a.status, NCB_DEV_BAD_PAGE);
+            return -1;
+        };
+        const int step = args.row_blocks * THREADS, first = blockIdx.x * THREADS + tid;
+        for (long long i = first; i < min(new_pages, (long long)free_count); i += step) {
+            const int b = first_above(r.page_end, n, (int)i);
+            if (r.served[b] == 0) continue;
+            const int before = b ? r.page_end[b - 1] : 0, j = (int)i - before;
+            a.table[(size_t)b * a.width + pages_for(r.cached[b]) + j] = new_page(b, j);
+        }
+        for (long long row = first; row < a.rows; row += step) {
+            int pos = -1, place = -1, request = -1;
+            if (row < rows_used) {
+                request = first_above(r.row_end, n, (int)row);
+                if (r.served[request] > 0) {
+                    const int cached = r.cached[request], have = pages_for(cached);
+                    pos = cached + (int)row - (request ? r.row_end[request - 1] : 0);
+                    const int p = pos / PAGE_TOKENS;
+                    int page;
+                    if (p < have) {
+                        page = a.table[(size_t)request * a.width + p];
+                        if ((unsigned)page >= (unsigned)a.n_pages) flag(a.status, NCB_DEV_BAD_PAGE), page = -1;
+                    } else {
+                        page = new_page(request, p - have);
+                    }
+                    if (page >= 0) place = page * PAGE_TOKENS + pos % PAGE_TOKENS;
+                }
+            }
+            a.pos[row] = pos, a.place[row] = place, a.request[row] = request;
+        }
+    }
+    /* what may be written over its input (lens over cached, free_left over free_count) is left to the last block: all have read by then */
+    __syncthreads();
+    if (tid == 0) {
+        __threadfence();
+        last = atomicAdd(a.ticket, 1) == (int)gridDim.x - 1;
+        if (last) {
+            *a.free_left = free_count - (int)taken;
+            *a.ticket = 0;
+        }
+    }
+    __syncthreads();
+    if (last)
+        for (int b = tid; b < n; b += THREADS) a.lens[b] = max(r.cached[b], 0) + r.served[b];
+}
+
+struct ReleaseArgs {
+    int *table, *lens;
+    const int *release;
+    int *free_pages, *free_count;
+    int requests, width, n_pages;
+    int *status;
+};
+
+/* One block: requests in order, a request's pages from its last to its first, so that the next request gets them in order again. */
+__global__ void __launch_bounds__(THREADS) k_page_release(const ReleaseArgs a) {
+    __shared__ long long sums[WARPS];
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    long long count = max(0, min(*a.free_count, a.n_pages));
+    auto valid = [&](int page) { return (unsigned)page < (unsigned)a.n_pages; };
+    for (int from = 0; from < a.requests; from += WARPS) { /* a warp per request: its entries are counted, then moved */
+        const int b = from + warp;
+        const bool on = b < a.requests && a.release[b] != 0;
+        const int held = on ? min(pages_for(max(a.lens[b], 0)), a.width) : 0;
+        int *entries = a.table + (size_t)(on ? b : 0) * a.width;
+        int good = 0;
+        for (int i = 0; i < held; i += 32) {
+            const bool in = i + lane < held, ok = in && valid(entries[i + lane]);
+            good += __popc(__ballot_sync(0xffffffffu, ok));
+            if (in && !ok) flag(a.status, NCB_DEV_BAD_PAGE);
+        }
+        long long total;
+        long long at = count + block_sum_before(lane == 0 ? good : 0, sums, &total);
+        at = __shfl_sync(0xffffffffu, at, 0) + good; /* the end of this request's pages in the list */
+        for (int i = 0; i < held; i += 32) {
+            const int page = i + lane < held ? entries[i + lane] : -1;
+            const uint32_t ok = __ballot_sync(0xffffffffu, valid(page));
+            if (valid(page)) {
+                const long long to = at - 1 - __popc(ok & ((1u << lane) - 1u));
+                if (to < a.n_pages) a.free_pages[to] = page;
+                else flag(a.status, NCB_DEV_BAD_PAGE); /* more pages than the pool has: some came back twice */
+            }
+            at -= __popc(ok);
+            if (i + lane < held) entries[i + lane] = -1;
+        }
+        if (on && lane == 0) a.lens[b] = 0;
+        count += total;
+    }
+    __syncthreads();
+    if (tid == 0) *a.free_count = (int)min(count, (long long)a.n_pages);
+}
+
+cudaError_t launch(void (*kernel)(const PlanArgs), int grid, int smem, cudaStream_t stream, const PlanArgs &args) {
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(grid);
+    config.blockDim = dim3(THREADS);
+    config.dynamicSmemBytes = smem;
+    config.stream = stream;
+    cudaLaunchAttribute attribute[1];
+    attribute[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attribute[0].val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = attribute;
+    config.numAttrs = 1;
+    return cudaLaunchKernelEx(&config, kernel, args);
+}
+
+} /* namespace */
+
+extern "C" {
+
+long long page_plan_words(int requests, long long rows, int max_fresh, int group, int kv_heads, int blocks) {
+    if (!sizes_ok(requests, rows, max_fresh, group, kv_heads, blocks)) return -1;
+    return schedule_words(caps_of(requests, rows, max_fresh, group, kv_heads, blocks));
+}
+
+int page_plan(const ncb_page_plan *args, void *stream) {
+    if (!args) return NCB_ERR_ARG;
+    const ncb_page_plan &a = *args;
+    if (!sizes_ok(a.requests, a.rows, a.max_fresh, a.group, a.kv_heads, a.blocks)) return NCB_ERR_ARG;
+    if (a.width <= 0 || a.width > (1 << 24) || a.n_pages <= 0 || a.n_pages > 0x7fffffff / PAGE_TOKENS || a.n_windows < 0 || a.n_windows > NCB_PLAN_WINDOWS) return NCB_ERR_ARG;
+    for (int w = 0; w < a.n_windows; w++)
+        if (a.windows[w] < 0) return NCB_ERR_ARG;
+    if (!a.table || !a.cached || !a.fresh || !a.free_pages || !a.free_count || !a.free_left || !a.row_start || !a.served || !a.lens || !a.ticket ||
+        (a.rows > 0 && (!a.pos || !a.place || !a.request)) || (a.n_windows > 0 && !a.work))
+        return NCB_ERR_ARG;
+    if ((uintptr_t)a.work % 16) return NCB_ERR_ALIGN;
+    PlanArgs p = {a, 1, schedule_words(caps_of(a.requests, a.rows, a.max_fresh, a.group, a.kv_heads, a.blocks))};
+    /* a block writes 2,048 rows in about the time that its sums take; more blocks than SMs would repeat them */
+    p.row_blocks = (int)((a.rows + 2047) / 2048);
+    p.row_blocks = p.row_blocks < 1 ? 1 : p.row_blocks > 64 ? 64 : p.row_blocks;
+    const long long listed = caps_of(a.requests, a.rows, a.max_fresh, a.group, a.kv_heads, a.blocks).owners;
+    const int smem = 4 * (5 * a.requests + (int)(listed < LISTED ? listed : LISTED));
+    if (smem > 48 * 1024 && cudaFuncSetAttribute(k_page_plan, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return NCB_ERR_LAUNCH;
+    return launch(k_page_plan, p.row_blocks + a.n_windows, smem, (cudaStream_t)stream, p) == cudaSuccess ? NCB_OK : NCB_ERR_LAUNCH;
+}
+
+int page_release(int *table, int *lens, const int *release, int *free_pages, int *free_count, int requests, int width, int n_pages, int *status,
+                 void *stream) {
+    if (requests <= 0 || requests > NCB_PLAN_REQUESTS || width <= 0 || n_pages <= 0) return NCB_ERR_ARG;
+    if (!table || !lens || !release || !free_pages || !free_count) return NCB_ERR_ARG;
+    const ReleaseArgs a = {table, lens, release, free_pages, free_count, requests, width, n_pages, status};
+    k_page_release<<<1, THREADS, 0, (cudaStream_t)stream>>>(a);
+    return cudaGetLastError() == cudaSuccess ? NCB_OK : NCB_ERR_LAUNCH;
+}
+
+} /* extern "C" */

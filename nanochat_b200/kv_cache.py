@@ -101,6 +101,68 @@ class Fp8KVCache:
         return k, floats[:, fbase + PAGE_KS // 4], v, floats[:, fbase + PAGE_VS // 4]
 
 
+class PagedKVCache:
+    """One layer's pool of pages for requests of any length (paged.py): `pages` uint8 [n_pages, kv_heads, PAGE_BYTES] for
+    float8_e4m3fn (Fp8KVCache's page), bf16 [n_pages, kv_heads, 2, 64, 128] (keys, then values) for bfloat16. Which pages are a
+    request's, and in what order, is the block table's to say."""
+
+    def __init__(self, n_pages: int, kv_heads: int, dtype: torch.dtype = torch.float8_e4m3fn, device: "torch.device | str" = "cuda",
+                 pages: torch.Tensor | None = None):
+        if dtype not in (torch.float8_e4m3fn, torch.bfloat16):
+            raise ValueError(f"pages of {dtype}: they are float8_e4m3fn or bfloat16")
+        self.n_pages, self.kv_heads, self.dtype, self.e4m3 = n_pages, kv_heads, dtype, dtype == torch.float8_e4m3fn
+        shape = (n_pages, kv_heads, PAGE_BYTES) if self.e4m3 else (n_pages, kv_heads, 2, PAGE_TOKENS, HEAD_DIM)
+        if pages is None:
+            pages = torch.zeros(shape, dtype=torch.uint8 if self.e4m3 else dtype, device=device)
+        assert pages.shape == shape and pages.dtype == (torch.uint8 if self.e4m3 else dtype) and pages.is_contiguous()
+        self.pages = pages
+
+    @property
+    def device(self) -> torch.device:
+        return self.pages.device
+
+    def nbytes(self) -> int:
+        return self.pages.numel() * self.pages.element_size()
+
+    @staticmethod
+    def pages_for(positions: int) -> int:
+        return cache_pages(positions)
+
+    def _places(self, table_row: torch.Tensor, start: int, n: int) -> tuple[torch.Tensor, torch.Tensor]:
+        """(page, position in it) of positions start .. start + n of the request with this row of the block table."""
+        pos = torch.arange(start, start + n, device=self.device)
+        page = table_row.to(self.device).long()[pos // PAGE_TOKENS]
+        assert bool(((page >= 0) & (page < self.n_pages)).all()), "positions without a page"
+        return page, pos % PAGE_TOKENS
+
+    def write(self, table_row: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor | None = None,
+              v_scale: torch.Tensor | None = None, start: int = 0) -> None:
+        """Store rows k, v [kv_heads, n, 128] at positions start .. of a request: bf16, or e4m3 bytes (uint8) with fp32 scales
+        [kv_heads, n]."""
+        page, j = self._places(table_row, start, k.shape[1])
+        if not self.e4m3:
+            self.pages[page, :, 0, j], self.pages[page, :, 1, j] = (x.to(self.device).transpose(0, 1) for x in (k, v))
+            return
+        head = torch.arange(self.kv_heads, device=self.device)[None]
+        floats = self.pages.view(torch.float32)
+        for x, scale, offsets, at in ((k, k_scale, page_offsets(str(self.device))[0], PAGE_KS), (v, v_scale, page_offsets(str(self.device))[1], PAGE_VS)):
+            self.pages[page[:, None, None], head[..., None], offsets[j][:, None]] = x.to(self.device).transpose(0, 1)
+            floats[page[:, None], head, at // 4 + j[:, None]] = scale.to(self.device).T
+
+    def read(self, table_row: torch.Tensor, n: int, start: int = 0) -> tuple[torch.Tensor, torch.Tensor]:
+        """(k, v) fp32 [kv_heads, n, 128] of positions start .. start + n of a request: the values that the pages stand for."""
+        page, j = self._places(table_row, start, n)
+        if not self.e4m3:
+            return tuple(self.pages[page, :, i, j].transpose(0, 1).float() for i in range(2))
+        head = torch.arange(self.kv_heads, device=self.device)[None]
+        found = []
+        for offsets, at in zip(page_offsets(str(self.device)), (PAGE_KS, PAGE_VS)):
+            codes = self.pages[page[:, None, None], head[..., None], offsets[j][:, None]].view(torch.float8_e4m3fn).float()
+            scale = self.pages.view(torch.float32)[page[:, None], head, at // 4 + j[:, None]]
+            found.append((codes * scale[..., None]).transpose(0, 1))
+        return tuple(found)
+
+
 class SingleCache:
     """A layer's cache that is one buffer."""
 

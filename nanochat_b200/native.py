@@ -23,9 +23,10 @@ INCLUDE = PACKAGE.parent / "include"
 NATIVE = PACKAGE / "_native"
 HEAD_DIM = 128
 LIBRARIES = ("kv_append", "decode_attn", "decode_step", "stream_gemm", "tile_gemm", "gemm_f32", "latent_attn", "gla",
-             "short_conv", "gqa_attn", "delta_rule", "prefill_attn")
+             "short_conv", "gqa_attn", "delta_rule", "prefill_attn", "page_plan", "paged_append", "paged_attn")
 
 MAX_STREAMS = 8  # NCB_MAX_STREAMS
+PLAN_WINDOWS = 8  # NCB_PLAN_WINDOWS
 c_ptr, c_int, c_ll, c_float = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_float
 
 
@@ -93,7 +94,35 @@ class Delta(ctypes.Structure):
                                      "tok_qk", "tok_g", "tok_v", "tok_s")]
 
 
+class Plan(ctypes.Structure):
+    """ncb_page_plan of include/nanochat_b200.h, field for field."""
+    _fields_ = [(n, c_ptr) for n in ("table", "cached", "fresh", "free_pages", "free_count", "free_left", "row_start", "served", "lens", "pos",
+                                     "place", "request", "work", "ticket", "status")] + \
+               [("rows", c_ll)] + \
+               [(n, c_int) for n in ("requests", "width", "n_pages", "max_fresh", "group", "kv_heads", "blocks", "n_windows")] + \
+               [("windows", c_int * PLAN_WINDOWS)]
+
+
+class Paged(ctypes.Structure):
+    """ncb_paged of include/nanochat_b200.h, field for field."""
+    _fields_ = [(n, c_ptr) for n in ("q", "pool", "out", "workspace", "table", "row_start", "served", "lens", "work", "status")] + \
+               [(n, c_ll) for n in ("rows", "ldq", "ldo", "workspace_bytes")] + \
+               [(n, c_int) for n in ("requests", "width", "n_pages", "max_fresh", "Hq", "Hkv", "e4m3", "window", "blocks")] + \
+               [("scale", c_float)]
+
+
 SIGNATURES = {
+    "page_plan": {
+        "page_plan_words": ([c_int, c_ll] + [c_int] * 4, c_ll),
+        "page_plan": ([c_ptr, c_ptr], c_int),
+        "page_release": ([c_ptr] * 5 + [c_int] * 3 + [c_ptr, c_ptr], c_int),
+    },
+    "paged_append": {"paged_append": ([c_ptr] * 9 + [c_ll, c_int, c_int, c_ll, c_int, c_int, c_int, c_ptr, c_ptr], c_int)},
+    "paged_attn": {
+        "paged_attn_blocks": ([], c_int),
+        "paged_attn_workspace_bytes": ([c_int, c_ll] + [c_int] * 4, c_ll),
+        "paged_attn": ([c_ptr, c_ptr], c_int),
+    },
     "kv_append": {
         "ncb_status_string": ([c_int], ctypes.c_char_p),
         "kv_cache_bytes": ([c_int, c_int, c_int], c_ll),

@@ -1,0 +1,184 @@
+"""A paged KV cache: pages of 64 positions taken from one pool by requests of any length, where Fp8KVCache cuts the memory into
+slots of one size (as the reference does, inference/decoder.py:112-121). One step of a server runs
+
+    plan = page_plan(pages, pages.lens, fresh, rows, ..., lens=pages.lens)     once: pages, positions, places, schedules
+    for every layer:
+        q = paged_append(qkv, ..., plan.pos, plan.place, cache, Hq)
+        out = paged_attention(q, cache, plan, window=...)
+
+with any mixture of decoding requests (one fresh token), drafted tokens (a few) and chunks of prompts (hundreds); a finished request's
+pages go back with pages.release(). Lengths stay on the device, so a captured step serves lengths that change. Like attention.py's
+operators, each launches on the current stream and returns without synchronising; a non-zero native status raises
+NativeError, what only the device can see is ORed into `status` (NCB_DEV_* bits)."""
+
+import contextlib
+import ctypes
+
+import torch
+from torch import Tensor
+
+from .kv_cache import HEAD_DIM, PAGE_TOKENS, PagedKVCache, cache_pages
+from .native import PLAN_WINDOWS, Paged, Plan, check, cuda_library, pointer, stream
+
+_READY = contextlib.nullcontext()
+
+
+def on_device_of(t: Tensor):
+    """The launches below go to the current stream of the current device: make it the tensors' one."""
+    assert t.is_cuda, "the operands live on a CUDA device"
+    return _READY if t.device.index == torch._C._cuda_getDevice() else torch.cuda.device(t.device)
+
+
+def _words(t: Tensor, *shape: int) -> bool:
+    return t.dtype == torch.int32 and t.shape == shape and t.is_contiguous()
+
+
+def address(t: "Tensor | None") -> "int | None":
+    return None if t is None else t.data_ptr()
+
+
+class PageTable:
+    """Which pages the requests hold, for the pools of every layer, on the device: `table` int32 (requests, width), -1 where there is
+    none; `lens` int32 (requests,), positions held; `free` int32 (n_pages,) and `free_count` int32 (1,), the pages nobody holds.
+    A page belongs to one request. At most 8,192 requests."""
+
+    def __init__(self, n_pages: int, requests: int, max_len: int, device: "torch.device | str" = "cuda", table: Tensor | None = None,
+                 lens: Tensor | None = None, free: Tensor | None = None, free_count: Tensor | None = None):
+        self.n_pages, self.requests, self.width = n_pages, requests, cache_pages(max_len)
+        new = dict(dtype=torch.int32, device=device)
+        self.table = torch.full((requests, self.width), -1, **new) if table is None else table
+        self.lens = torch.zeros(requests, **new) if lens is None else lens
+        # taken from the end: the first request gets pages 0, 1, ..
+        self.free = torch.arange(n_pages - 1, -1, -1, **new) if free is None else free
+        self.free_count = torch.full((1,), n_pages, **new) if free_count is None else free_count
+        assert _words(self.table, requests, self.width) and _words(self.lens, requests)
+        assert _words(self.free, n_pages) and _words(self.free_count, 1)
+        self.ticket = torch.zeros(1, **new)
+
+    @property
+    def device(self) -> torch.device:
+        return self.table.device
+
+    @property
+    def capacity(self) -> int:
+        """Positions a request can hold."""
+        return self.width * PAGE_TOKENS
+
+    def release(self, which: Tensor, status: Tensor | None = None) -> None:
+        """Requests with which[b] != 0 (int32 (requests,)) give back the pages of their lens[b] positions and hold none."""
+        assert _words(which, self.requests)
+        with on_device_of(self.table):
+            check(cuda_library("page_plan").page_release(
+                pointer(self.table), pointer(self.lens), pointer(which), pointer(self.free), pointer(self.free_count), self.requests, self.width,
+                self.n_pages, pointer(status), stream()), "page_release")
+
+
+class PagePlan:
+    """One step of a PageTable's requests, in device memory that page_plan fills (and may fill again):
+    row_start (requests + 1,) first rows; fresh (requests,) rows that are served, 0 for a request that is not; lens (requests,)
+    positions after the step; pos, place, request (rows,) of every row: its position, page * 64 + position % 64, its request; -1 in pos
+    and place of a row that is not served, in all three behind the last request. All int32. Schedules of paged_attention for
+    each of `windows`, for Hq query heads over Hkv."""
+
+    def __init__(self, pages: PageTable, rows: int, max_new: int, Hq: int, Hkv: int, windows: "tuple[int, ...]" = (0,)):
+        assert Hkv > 0 and Hq > 0 and Hq % Hkv == 0 and 0 < len(windows) <= PLAN_WINDOWS and len(set(windows)) == len(windows)
+        self.pages, self.rows, self.max_new, self.Hq, self.Hkv, self.windows = pages, rows, max_new, Hq, Hkv, tuple(windows)
+        n, group = pages.requests, Hq // Hkv
+        self.blocks = cuda_library("paged_attn").paged_attn_blocks()
+        words = cuda_library("page_plan").page_plan_words(n, rows, max_new, group, Hkv, self.blocks)
+        if words < 0:
+            raise ValueError(f"no plan for {n} requests, {rows} rows, at most {max_new} a request, {Hq} heads over {Hkv}")
+        at = (3 * n + 1 + 3 * rows + 3) // 4 * 4
+        flat = self._flat = torch.empty(at + words * len(windows), dtype=torch.int32, device=pages.device)
+        self.row_start, self.fresh, self.lens, self.pos, self.place, self.request, _, self.work = flat.split(
+            [n + 1, n, n, rows, rows, rows, at - (3 * n + 1 + 3 * rows), words * len(windows)])
+        self._at = {w: self.work.data_ptr() + 4 * words * i for i, w in enumerate(self.windows)}
+        base = flat.data_ptr()
+        places = [base + 4 * i for i in (0, n + 1, 2 * n + 1, 3 * n + 1, 3 * n + 1 + rows, 3 * n + 1 + 2 * rows)]
+        self._args = Plan(pages.table.data_ptr(), None, None, pages.free.data_ptr(), pages.free_count.data_ptr(), None, *places, self.work.data_ptr(),
+                          pages.ticket.data_ptr(), None, rows, n, pages.width, pages.n_pages, max_new, group, Hkv, self.blocks, len(windows),
+                          (ctypes.c_int * PLAN_WINDOWS)(*windows))
+        self._own_lens = places[2]
+
+
+def page_plan(pages: PageTable, cached: Tensor, new: Tensor, rows: int, *, max_new: int, Hq: int, Hkv: int, windows: "tuple[int, ...]" = (0,),
+              lens: Tensor | None = None, free_left: Tensor | None = None, plan: PagePlan | None = None, status: Tensor | None = None) -> PagePlan:
+    """One step's bookkeeping in one launch: request b holds cached[b] positions and adds new[b] (int32 (requests,) on the device, 0 for
+    a request that idles), whose rows follow the rows of request b - 1 in the step's `rows` rows. Takes the new pages off pages.free
+    into pages.table, and returns the step's PagePlan (`plan`: one of the same sizes to fill again, as a captured step does).
+    max_new: an upper bound of new known to the host. lens: where the new lengths go (default: the plan's own; pages.lens, or
+    `cached` itself, to advance them in place); free_left: where the count of free pages goes (default: pages.free_count).
+    Requests are served in order. One that would need more pages than are left (NCB_DEV_NO_PAGES), or that passes the table's
+    width, max_new or `rows` or has a negative length (NCB_DEV_BAD_LENGTH), is not served: it keeps its length, and its rows are idle in the operators below."""
+    n = pages.requests
+    assert _words(cached, n) and _words(new, n)
+    assert lens is None or _words(lens, n)
+    assert free_left is None or _words(free_left, 1)
+    with on_device_of(pages.table):
+        if plan is None:
+            plan = PagePlan(pages, rows, max_new, Hq, Hkv, windows)
+        elif plan.pages is not pages or (plan.rows, plan.max_new, plan.Hq, plan.Hkv, plan.windows) != (rows, max_new, Hq, Hkv, tuple(windows)):
+            raise ValueError("the plan was made for other sizes or another table")
+        plan.lens = plan.lens if lens is None else lens
+        args = plan._args
+        args.cached, args.fresh, args.status = cached.data_ptr(), new.data_ptr(), address(status)
+        args.lens = plan.lens.data_ptr()
+        args.free_left = (pages.free_count if free_left is None else free_left).data_ptr()
+        check(cuda_library("page_plan").page_plan(ctypes.byref(args), stream()), "page_plan")
+    return plan
+
+
+def paged_append(qkv: Tensor, q_gain: Tensor, k_gain: Tensor, cos: Tensor, sin: Tensor, pos: Tensor, place: Tensor, cache: PagedKVCache,
+                 Hq: int, q_out: Tensor | None = None, status: Tensor | None = None) -> Tensor:
+    """kv_append into a pool of pages: norm + rotate q and k, and store k and v at place[row] = page * 64 + position % 64 (a plan's
+    pos and place; int32 (rows,), no place twice), quantised to e4m3 with a scale per row and head, or in bf16, as the pool is.
+    Same bits as kv_append. Rows with a negative position or place are idle: nothing is written for them. Returns q_out (rows, Hq, 128) bf16."""
+    rows, Hkv = qkv.shape[0], cache.kv_heads
+    assert qkv.dtype == torch.bfloat16 and qkv.stride(-1) == 1 and qkv.shape[1] == (Hq + 2 * Hkv) * HEAD_DIM
+    assert _words(pos, rows) and _words(place, rows)
+    assert cos.shape == sin.shape and cos.shape[1] == HEAD_DIM // 2 and cos.is_contiguous() and sin.is_contiguous()
+    assert q_gain.dtype == k_gain.dtype == cos.dtype == sin.dtype == torch.float32
+    assert q_gain.shape == k_gain.shape == (HEAD_DIM,) and q_gain.is_contiguous() and k_gain.is_contiguous()
+    if q_out is None:
+        q_out = torch.empty((rows, Hq, HEAD_DIM), dtype=torch.bfloat16, device=qkv.device)
+    assert q_out.dtype == torch.bfloat16 and q_out.shape == (rows, Hq, HEAD_DIM) and q_out.is_contiguous()
+    with on_device_of(qkv):
+        check(cuda_library("paged_append").paged_append(
+            qkv.data_ptr(), q_gain.data_ptr(), k_gain.data_ptr(), cos.data_ptr(), sin.data_ptr(), pos.data_ptr(), place.data_ptr(),
+            q_out.data_ptr(), cache.pages.data_ptr(), rows, Hq, Hkv, qkv.stride(0), cos.shape[0], cache.n_pages, cache.e4m3, address(status),
+            stream()), "paged_append")
+    return q_out
+
+
+def paged_attention(q: Tensor, cache: PagedKVCache, plan: PagePlan, window: int = 0, softmax_scale: float | None = None,
+                    out: Tensor | None = None, workspace: Tensor | None = None, status: Tensor | None = None) -> Tensor:
+    """Causal attention of a step's rows over their requests' pages, whose positions already hold the step's own (paged_append): the
+    row at position p attends (p - window, p], or [0, p] with window 0. q (rows, Hq, 128) bf16, heads contiguous, row stride free;
+    `window` is one that the plan was made with. Rows of requests that the plan did not serve become zeros; rows behind the last
+    request are left as they were in `out`. workspace: uint8, workspace_bytes_for(plan) bytes, for calls that no other stream overlaps
+    (default: a new one). Returns out (rows, Hq, 128) bf16."""
+    rows, Hq = plan.rows, plan.Hq
+    assert q.dtype == torch.bfloat16 and q.shape == (rows, Hq, HEAD_DIM) and q.stride(2) == 1 and q.stride(1) == HEAD_DIM
+    assert cache.kv_heads == plan.Hkv
+    work = plan._at.get(window)
+    if work is None:
+        raise ValueError(f"the plan has schedules for windows {plan.windows}, not {window}")
+    pages = plan.pages
+    if cache.n_pages != pages.n_pages:
+        raise ValueError(f"a pool of {cache.n_pages} pages, a table over {pages.n_pages}")
+    if out is None:
+        out = torch.empty((rows, Hq, HEAD_DIM), dtype=torch.bfloat16, device=q.device)
+    assert out.dtype == torch.bfloat16 and out.shape == (rows, Hq, HEAD_DIM) and out.stride(2) == 1 and out.stride(1) == HEAD_DIM
+    if workspace is None:
+        workspace = torch.empty(workspace_bytes_for(plan), dtype=torch.uint8, device=q.device)
+    args = Paged(q.data_ptr(), cache.pages.data_ptr(), out.data_ptr(), workspace.data_ptr(), pages.table.data_ptr(), plan.row_start.data_ptr(),
+                 plan.fresh.data_ptr(), plan.lens.data_ptr(), work, address(status), rows, q.stride(0), out.stride(0), workspace.numel(),
+                 pages.requests, pages.width, pages.n_pages, plan.max_new, Hq, plan.Hkv, cache.e4m3, window, plan.blocks,
+                 HEAD_DIM ** -0.5 if softmax_scale is None else softmax_scale)
+    with on_device_of(q):
+        check(cuda_library("paged_attn").paged_attn(ctypes.byref(args), stream()), "paged_attn")
+    return out
+
+
+def workspace_bytes_for(plan: PagePlan) -> int:
+    return cuda_library("paged_attn").paged_attn_workspace_bytes(plan.pages.requests, plan.rows, plan.max_new, plan.Hq, plan.Hkv, plan.blocks)
