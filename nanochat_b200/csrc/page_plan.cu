@@ -72,13 +72,17 @@ struct Cut {
     }
 };
 
-/* The schedule of one window's attention. */
-__device__ void schedule(const ncb_page_plan &a, const Requests &r, int window, int *work, long long *sums) {
+/* The schedule of one window's attention, of one class of requests. */
+__device__ void schedule(const ncb_page_plan &a, const Requests &r, int window, int tile, int *work, long long *sums) {
     __shared__ unsigned long long best;
     const Caps caps = caps_of(a.requests, a.rows, a.max_fresh, a.group, a.kv_heads, a.blocks);
+    const Class &c = tile ? caps.tile : caps.split;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, per = (a.requests + THREADS - 1) / THREADS, b0 = tid * per;
-    const int rows_per = SPLIT_SLOTS / a.group, rows = (int)a.rows, units = units_of(a.blocks, a.kv_heads);
-    auto rows_of = [&](int b) { return min(r.row_end[b], rows) - min(b ? r.row_end[b - 1] : 0, rows); }; /* not served ones among them: zeros to write */
+    const int rows_per = c.rows_per, rows = (int)a.rows, units = units_of(a.blocks, a.kv_heads);
+    auto rows_of = [&](int b) { /* not served ones among them: zeros to write */
+        const int n = min(r.row_end[b], rows) - min(b ? r.row_end[b - 1] : 0, rows);
+        return caps.tiles && (n > caps.split.rows_per) != (tile != 0) ? 0 : n;
+    };
     long long total, mine = 0;
     for (int b = b0; b < min(b0 + per, a.requests); b++) mine += (rows_of(b) + rows_per - 1) / rows_per;
     long long at = block_sum_before(mine, sums, &total);
@@ -112,14 +116,17 @@ __device__ void schedule(const ncb_page_plan &a, const Requests &r, int window, 
     block_sum_before(sum, sums, &pages); /* its barriers also publish owner_pages and best */
     int chunk = WHOLE;
     if (listed && pages > 0) {
-        /* Each warp estimates the time of one chunk size: the longest entry where all run at once, else the mean load and half an entry of
-         * tail. Warp 0: nothing is cut. */
-        const long long waves = 1 + warp; /* in eighths: chunks of four times an even share of the units' work down to a quarter of one */
-        const int c = warp == 0 ? WHOLE : (int)max((long long)MIN_CHUNK, (8 * pages + units * waves - 1) / (units * waves));
+        /* Each warp estimates the time of one chunk size, in sixteenths of a page: every unit's share of entries of the mean length, and half of what the
+         * longest is longer. Warp 0: nothing is cut; warp w: chunks of total / (units * waves * w / 32) pages. */
+        auto chunk_of = [&](int w) {
+            const long long shares = (long long)units * c.waves * w; /* in 32nds */
+            return w == 0 ? WHOLE : (int)max((long long)MIN_CHUNK, (32 * pages + shares - 1) / shares);
+        };
+        const int size = chunk_of(warp);
         long long n = 0;
         int longest = 0;
         for (int o = lane; o < owners; o += 32) {
-            const Cut cut(r.owner_pages[o], c);
+            const Cut cut(r.owner_pages[o], size);
             n += cut.chunks;
             longest = max(longest, cut.len);
         }
@@ -128,17 +135,15 @@ __device__ void schedule(const ncb_page_plan &a, const Requests &r, int window, 
             n += __shfl_xor_sync(0xffffffffu, n, o);
             longest = max(longest, __shfl_xor_sync(0xffffffffu, longest, o));
         }
-        const long long even = 16 * (pages + n * OVERHEAD) / units; /* in sixteenths of a page */
-        const long long cost = n <= units ? 16ll * (longest + OVERHEAD) : max(even + 8ll * longest, 16ll * (longest + OVERHEAD));
-        const long long merge = n > owners ? 16ll * OVERHEAD : 0; /* and their states are read again */
-        if (lane == 0) atomicMin(&best, (unsigned long long)(cost + merge) << 32 | (unsigned)warp);
+        const long long mean = 16 * pages / n, each = mean + 16 * OVERHEAD, most = 16ll * longest;
+        long long cost = max((n + units - 1) / units * each + (most - mean) / 2, most + 16 * OVERHEAD);
+        if (n > owners) cost += 16 * OVERHEAD; /* states are written and read again */
+        if (lane == 0 && (!tile || n == owners || n <= c.parts)) atomicMin(&best, (unsigned long long)cost << 32 | (unsigned)warp);
         __syncthreads();
-        const int chosen = (int)(best & 0xffffffffu);
-        const long long w = 1 + chosen;
-        if (chosen > 0) chunk = (int)max((long long)MIN_CHUNK, (8 * pages + units * w - 1) / (units * w));
+        chunk = chunk_of((int)(best & 0xffffffffu));
     }
-    Entry *entries = reinterpret_cast<Entry *>(work + HEADER_WORDS);
-    Merge *merges = reinterpret_cast<Merge *>(work + HEADER_WORDS + caps.entries * ENTRY_WORDS);
+    Entry *entries = reinterpret_cast<Entry *>(work + entries_at(caps, tile));
+    Merge *merges = reinterpret_cast<Merge *>(work + merges_at(caps, tile));
     long long n_entries = 0, n_parts = 0, n_merges = 0;
     for (int from = 0; from < owners; from += THREADS) { /* the last rows of a request reach furthest: they start first */
         const int o = owners - 1 - from - tid;
@@ -153,15 +158,18 @@ __device__ void schedule(const ncb_page_plan &a, const Requests &r, int window, 
         long long t, t2; /* entries; parts, and merges above them */
         const long long e = n_entries + block_sum_before(chunks, sums, &t), pm = block_sum_before(parts | (long long)(parts > 0) << 32, sums, &t2);
         const long long p = n_parts + (pm & 0xffffffffll), m = n_merges + (pm >> 32);
-        for (int c = 0; c < chunks; c++) {
-            if (e + c >= caps.entries || (parts && p + c >= caps.parts)) break; /* cannot be: see Caps */
-            Entry x = {w.request, w.row0, w.rows, w.page0 + c * len, min(w.page0 + (c + 1) * len, w.page1), parts ? (int)p + c : -1, {0, 0}};
-            entries[e + c] = x;
+        for (int i = 0; i < chunks; i++) {
+            if (e + i >= c.entries || (parts && p + i >= c.parts)) break; /* cannot be: see Caps */
+            Entry x = {w.request, w.row0, w.rows, w.page0 + i * len, min(w.page0 + (i + 1) * len, w.page1), parts ? (int)p + i : -1, {0, 0}};
+            entries[e + i] = x;
         }
-        if (parts && m < caps.merges) merges[m] = Merge{(w.request ? r.row_end[w.request - 1] : 0) + w.row0, w.rows, (int)p, parts};
+        if (parts && m < c.merges) merges[m] = Merge{(w.request ? r.row_end[w.request - 1] : 0) + w.row0, w.rows, (int)p, parts};
         n_entries += t, n_parts += t2 & 0xffffffffll, n_merges += t2 >> 32;
     }
-    if (tid == 0) work[0] = (int)min(n_entries, caps.entries), work[1] = (int)min(n_merges, caps.merges);
+    if (tid == 0) {
+        work[2 * tile] = (int)min(n_entries, c.entries), work[2 * tile + 1] = (int)min(n_merges, c.merges);
+        if (!caps.tiles) work[2] = work[3] = 0;
+    }
 }
 
 struct PlanArgs {
@@ -211,8 +219,8 @@ __global__ void __launch_bounds__(THREADS) k_page_plan(const PlanArgs args) {
     long long taken;
     block_sum_before(mine, sums, &taken); /* its barriers publish the arrays */
     if (blockIdx.x >= args.row_blocks) {
-        const int w = blockIdx.x - args.row_blocks;
-        schedule(a, r, a.windows[w], a.work + w * args.words, sums);
+        const int w = (blockIdx.x - args.row_blocks) % a.n_windows, tile = (blockIdx.x - args.row_blocks) / a.n_windows;
+        schedule(a, r, a.windows[w], tile, a.work + w * args.words, sums);
     } else {
         if (blockIdx.x == 0) {
             if (bad) flag(a.status, NCB_DEV_BAD_LENGTH);
@@ -342,7 +350,8 @@ extern "C" {
 
 long long page_plan_words(int requests, long long rows, int max_fresh, int group, int kv_heads, int blocks) {
     if (!sizes_ok(requests, rows, max_fresh, group, kv_heads, blocks)) return -1;
-    return schedule_words(caps_of(requests, rows, max_fresh, group, kv_heads, blocks));
+    const long long words = schedule_words(caps_of(requests, rows, max_fresh, group, kv_heads, blocks));
+    return (words + 3) / 4 * 4; /* schedules one after the other stay 16-byte aligned */
 }
 
 int page_plan(const ncb_page_plan *args, void *stream) {
@@ -356,14 +365,15 @@ int page_plan(const ncb_page_plan *args, void *stream) {
         (a.rows > 0 && (!a.pos || !a.place || !a.request)) || (a.n_windows > 0 && !a.work))
         return NCB_ERR_ARG;
     if ((uintptr_t)a.work % 16) return NCB_ERR_ALIGN;
-    PlanArgs p = {a, 1, schedule_words(caps_of(a.requests, a.rows, a.max_fresh, a.group, a.kv_heads, a.blocks))};
+    const Caps caps = caps_of(a.requests, a.rows, a.max_fresh, a.group, a.kv_heads, a.blocks);
+    PlanArgs p = {a, 1, page_plan_words(a.requests, a.rows, a.max_fresh, a.group, a.kv_heads, a.blocks)};
     /* a block writes 2,048 rows in about the time that its sums take; more blocks than SMs would repeat them */
     p.row_blocks = (int)((a.rows + 2047) / 2048);
     p.row_blocks = p.row_blocks < 1 ? 1 : p.row_blocks > 64 ? 64 : p.row_blocks;
-    const long long listed = caps_of(a.requests, a.rows, a.max_fresh, a.group, a.kv_heads, a.blocks).owners;
+    const long long listed = caps.split.owners > caps.tile.owners ? caps.split.owners : caps.tile.owners;
     const int smem = 4 * (5 * a.requests + (int)(listed < LISTED ? listed : LISTED));
     if (smem > 48 * 1024 && cudaFuncSetAttribute(k_page_plan, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return NCB_ERR_LAUNCH;
-    return launch(k_page_plan, p.row_blocks + a.n_windows, smem, (cudaStream_t)stream, p) == cudaSuccess ? NCB_OK : NCB_ERR_LAUNCH;
+    return launch(k_page_plan, p.row_blocks + a.n_windows * (caps.tiles ? 2 : 1), smem, (cudaStream_t)stream, p) == cudaSuccess ? NCB_OK : NCB_ERR_LAUNCH;
 }
 
 int page_release(int *table, int *lens, const int *release, int *free_pages, int *free_count, int requests, int width, int n_pages, int *status,

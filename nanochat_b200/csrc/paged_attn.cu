@@ -19,8 +19,7 @@
  * k_paged_merge: the states of owners that were cut, one warp per query slot.
  * Waits are bounded: when one expires NCB_DEV_WAIT_TIMEOUT is flagged and the block leaves after its copies in flight.
  */
-#include "paged.cuh"
-#include "umma.cuh"
+#include "paged_tiles.cuh"
 
 namespace {
 
@@ -38,12 +37,6 @@ template <bool E4M3> struct Ring {
     static constexpr int SMEM = 1024 + STAGE * STAGES; /* 1024: swizzled boxes are aligned by hand */
     static_assert(BLOCKS_PER_SM * (SMEM + 2048) <= 228 * 1024, "blocks per SM");
     static_assert(SPLIT_WARPS * 16 * PART * 4 <= STAGE * STAGES, "the warps' states reuse the ring");
-};
-
-struct PagedArgs {
-    ncb_paged p;
-    Caps caps;
-    float scale_log2;
 };
 
 __device__ __forceinline__ float lg2(float x) {
@@ -147,9 +140,11 @@ template <bool E4M3> __global__ void __launch_bounds__(SPLIT_THREADS, BLOCKS_PER
     __syncthreads();
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const int entry = blockIdx.x / a.Hkv, kvh = blockIdx.x % a.Hkv, G = a.Hq / a.Hkv;
-    if (entry >= a.work[0]) return;
-    const Entry e = reinterpret_cast<const Entry *>(a.work + HEADER_WORDS)[entry];
+    const int G = a.Hq / a.Hkv, jobs = a.work[0] * a.Hkv;
+    int base = 0; /* pages that have been through the ring */
+    for (int job = blockIdx.x; job < jobs; job += gridDim.x) {
+    const int kvh = job % a.Hkv;
+    const Entry e = reinterpret_cast<const Entry *>(a.work + entries_at(args.caps, 0))[job / a.Hkv];
     const int served = a.served[e.request], slots = e.rows * G, n = e.page1 - e.page0;
     const int first_pos = a.lens[e.request] - served + e.row0, last_pos = first_pos + e.rows - 1;
     const long long first_row = a.row_start[e.request] + e.row0;
@@ -161,8 +156,8 @@ template <bool E4M3> __global__ void __launch_bounds__(SPLIT_THREADS, BLOCKS_PER
             uint64_t once = policy_evict_first();
             int sent = 0, page = n > 0 ? table[0] : 0;
             for (int i = 0; i < n; i++) {
-                const int st = i % R::STAGES, next = i + 1 < n ? table[i + 1] : 0;
-                if (i >= R::STAGES && !mbar_wait(empty(st), (i / R::STAGES - 1) & 1)) {
+                const int at = base + i, st = at % R::STAGES, next = i + 1 < n ? table[i + 1] : 0;
+                if (at >= R::STAGES && !mbar_wait(empty(st), (at / R::STAGES - 1) & 1)) {
                     flag(a.status, NCB_DEV_WAIT_TIMEOUT);
                     failed = 1;
                     break;
@@ -184,7 +179,8 @@ template <bool E4M3> __global__ void __launch_bounds__(SPLIT_THREADS, BLOCKS_PER
                 sent++;
                 page = next;
             }
-            for (int i = sent > R::STAGES ? sent - R::STAGES : 0; i < sent; i++) mbar_wait(full(i % R::STAGES), (i / R::STAGES) & 1); /* nobody leaves under a copy */
+            if (failed) /* nobody leaves under a copy */
+                for (int at = base + max(0, sent - R::STAGES); at < base + sent; at++) mbar_wait(full(at % R::STAGES), (at / R::STAGES) & 1);
         }
         __syncwarp();
     } else {
@@ -240,9 +236,9 @@ template <bool E4M3> __global__ void __launch_bounds__(SPLIT_THREADS, BLOCKS_PER
             for (int x = 0; x < 4; x++) o[d][x] = 0.f;
 
         for (int i = 0; i < n; i++) {
-            const int st = i % R::STAGES;
-            if (!__all_sync(0xffffffffu, mbar_wait(full(st), (i / R::STAGES) & 1))) {
-                if (lane == 0) flag(a.status, NCB_DEV_WAIT_TIMEOUT);
+            const int at = base + i, st = at % R::STAGES;
+            if (!__all_sync(0xffffffffu, mbar_wait(full(st), (at / R::STAGES) & 1))) {
+                if (lane == 0) flag(a.status, NCB_DEV_WAIT_TIMEOUT), failed = 1;
                 break;
             }
             const uint8_t *page = smem + st * R::STAGE;
@@ -417,11 +413,16 @@ template <bool E4M3> __global__ void __launch_bounds__(SPLIT_THREADS, BLOCKS_PER
                 const float inv = sum > 0.f || sum != sum ? __fdiv_rn(1.f, E4M3 ? sum * P_SCALE : sum) : 0.f;
                 ((bf16 *)a.out)[row * a.ldo + (size_t)head * HEAD_DIM + tid] = __float2bfloat16_rn(x * inv);
             } else {
-                float *part = (float *)a.workspace + ((size_t)((long long)e.part * a.Hkv + kvh) * args.caps.slots + slot) * PART;
+                float *part = (float *)a.workspace + ((size_t)((long long)e.part * a.Hkv + kvh) * args.caps.split.slots + slot) * PART;
                 if (tid == 0) part[0] = top, part[1] = sum;
                 part[4 + tid] = x;
             }
         }
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); /* the states were written where the next pages will be copied */
+    __syncthreads();
+    if (failed) break;
+    base += n;
     }
 }
 
@@ -432,31 +433,37 @@ __global__ void __launch_bounds__(32 * MERGE_WARPS) k_paged_merge(const PagedArg
     const ncb_paged &a = args.p;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const int lane = threadIdx.x & 31, G = a.Hq / a.Hkv, slots = args.caps.slots;
-    const Merge *merges = reinterpret_cast<const Merge *>(a.work + HEADER_WORDS + args.caps.entries * ENTRY_WORDS);
-    const long long jobs = (long long)a.work[1] * a.Hkv * slots;
-    for (long long job = (long long)blockIdx.x * MERGE_WARPS + threadIdx.x / 32; job < jobs; job += (long long)gridDim.x * MERGE_WARPS) {
-        const int slot = (int)(job % slots), kvh = (int)(job / slots % a.Hkv);
-        const Merge e = merges[job / slots / a.Hkv];
-        if (slot >= e.rows * G) continue;
-        const float *part = (const float *)a.workspace + ((size_t)((long long)e.part * a.Hkv + kvh) * slots + slot) * PART;
-        const size_t step = (size_t)a.Hkv * slots * PART;
-        float top = -INFINITY, sum = 0.f;
-        for (int c = lane; c < e.parts; c += 32) top = fmaxf(top, part[c * step]);
+    const int lane = threadIdx.x & 31, G = a.Hq / a.Hkv, warps = gridDim.x * MERGE_WARPS;
+    long long job = (long long)blockIdx.x * MERGE_WARPS + threadIdx.x / 32;
+    for (int tile = 0; tile <= args.caps.tiles; tile++) {
+        const Class &cls = tile ? args.caps.tile : args.caps.split;
+        const Merge *merges = reinterpret_cast<const Merge *>(a.work + merges_at(args.caps, tile));
+        const float *parts = (const float *)a.workspace + parts_at(args.caps, a.Hkv, tile);
+        const long long jobs = (long long)a.work[2 * tile + 1] * a.Hkv * cls.slots;
+        for (; job < jobs; job += warps) {
+            const int slot = (int)(job % cls.slots), kvh = (int)(job / cls.slots % a.Hkv);
+            const Merge e = merges[job / cls.slots / a.Hkv];
+            if (slot >= e.rows * G) continue;
+            const float *part = parts + ((size_t)((long long)e.part * a.Hkv + kvh) * cls.slots + slot) * PART;
+            const size_t step = (size_t)a.Hkv * cls.slots * PART;
+            float top = -INFINITY, sum = 0.f;
+            for (int c = lane; c < e.parts; c += 32) top = fmaxf(top, part[c * step]);
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-        for (int c = 0; c < e.parts; c++) {
-            const float2 ml = *reinterpret_cast<const float2 *>(part + c * step);
-            const float4 v = *reinterpret_cast<const float4 *>(part + c * step + 4 + 4 * lane);
-            const float f = scale_of(ml.x, ml.y, top);
-            sum = fmaf(ml.y, f, sum);
-            if (f != 0.f) x.x = fmaf(v.x, f, x.x), x.y = fmaf(v.y, f, x.y), x.z = fmaf(v.z, f, x.z), x.w = fmaf(v.w, f, x.w);
+            for (int c = 0; c < e.parts; c++) {
+                const float2 ml = *reinterpret_cast<const float2 *>(part + c * step);
+                const float4 v = *reinterpret_cast<const float4 *>(part + c * step + 4 + 4 * lane);
+                const float f = scale_of(ml.x, ml.y, top);
+                sum = fmaf(ml.y, f, sum);
+                if (f != 0.f) x.x = fmaf(v.x, f, x.x), x.y = fmaf(v.y, f, x.y), x.z = fmaf(v.z, f, x.z), x.w = fmaf(v.w, f, x.w);
+            }
+            const float inv = sum > 0.f || sum != sum ? __fdiv_rn(1.f, a.e4m3 ? sum * P_SCALE : sum) : 0.f;
+            const uint2 y = make_uint2(pack_bf16(x.x * inv, x.y * inv), pack_bf16(x.z * inv, x.w * inv));
+            *reinterpret_cast<uint2 *>((bf16 *)a.out + (e.row + slot / G) * a.ldo + (size_t)(kvh * G + slot % G) * HEAD_DIM + 4 * lane) = y;
         }
-        const float inv = sum > 0.f || sum != sum ? __fdiv_rn(1.f, a.e4m3 ? sum * P_SCALE : sum) : 0.f;
-        const uint2 y = make_uint2(pack_bf16(x.x * inv, x.y * inv), pack_bf16(x.z * inv, x.w * inv));
-        *reinterpret_cast<uint2 *>((bf16 *)a.out + (e.row + slot / G) * a.ldo + (size_t)(kvh * G + slot % G) * HEAD_DIM + 4 * lane) = y;
+        job -= jobs;
     }
 }
 
@@ -478,7 +485,24 @@ template <bool E4M3> cudaError_t split(const CUtensorMap &map, const PagedArgs &
     constexpr int smem = Ring<E4M3>::SMEM;
     const cudaError_t rc = cudaFuncSetAttribute(k_paged_split<E4M3>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (rc != cudaSuccess) return rc;
-    return launch(k_paged_split<E4M3>, (unsigned)(args.caps.entries * args.p.Hkv), SPLIT_THREADS, smem, stream, map, args);
+    const long long jobs = args.caps.split.entries * args.p.Hkv;
+    return launch(k_paged_split<E4M3>, (unsigned)(jobs < args.p.blocks ? jobs : args.p.blocks), SPLIT_THREADS, smem, stream, map, args);
+}
+template <bool E4M3> cudaError_t tile(const CUtensorMap &map_q, const CUtensorMap &map_kv, const PagedArgs &args, cudaStream_t stream) {
+    constexpr int smem = tiles::Shape<E4M3>::SMEM;
+    const cudaError_t rc = cudaFuncSetAttribute(tiles::k_paged_tiles<E4M3>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (rc != cudaSuccess) return rc;
+    return launch(tiles::k_paged_tiles<E4M3>, (unsigned)(args.caps.tile.entries * args.p.Hkv), E4M3 ? tiles::THREADS : 32 * tiles::WIDEN_WARP, smem, stream, map_q, map_kv, args);
+}
+
+/* The queries as [rows][heads][128] in boxes of 64 columns, the heads of a group and the rows of a tile. */
+bool query_map(const ncb_paged &a, int rows_per, CUtensorMap *out) {
+    EncodeTiled encode = encoder();
+    if (!encode) return false;
+    const cuuint64_t dims[3] = {(cuuint64_t)HEAD_DIM, (cuuint64_t)a.Hq, (cuuint64_t)a.rows}, strides[2] = {HEAD_DIM * 2, (cuuint64_t)a.ldq * 2};
+    const cuuint32_t box[3] = {64, (cuuint32_t)(a.Hq / a.Hkv), (cuuint32_t)rows_per}, elem[3] = {1, 1, 1};
+    return encode(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void *>(a.q), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 } /* namespace */
@@ -490,7 +514,7 @@ int paged_attn_blocks(void) { return BLOCKS_PER_SM * 148; }
 long long paged_attn_workspace_bytes(int requests, long long rows, int max_fresh, int Hq, int Hkv, int blocks) {
     if (Hq <= 0 || Hkv <= 0 || Hq % Hkv || !sizes_ok(requests, rows, max_fresh, Hq / Hkv, Hkv, blocks)) return -1;
     const Caps c = caps_of(requests, rows, max_fresh, Hq / Hkv, Hkv, blocks);
-    return c.parts * Hkv * c.slots * PART * 4;
+    return 4 * workspace_floats(c, Hkv);
 }
 
 int paged_attn(const ncb_paged *args, void *stream) {
@@ -505,10 +529,15 @@ int paged_attn(const ncb_paged *args, void *stream) {
     PagedArgs p = {a, caps_of(a.requests, a.rows, a.max_fresh, a.Hq / a.Hkv, a.Hkv, a.blocks), a.scale * LOG2_E};
     if (a.workspace_bytes < paged_attn_workspace_bytes(a.requests, a.rows, a.max_fresh, a.Hq, a.Hkv, a.blocks)) return NCB_ERR_WORKSPACE;
     const long long key_rows = (long long)a.n_pages * a.Hkv * 2 * PAGE_TOKENS;
-    if (key_rows > 0x7fffffffll || p.caps.entries * a.Hkv > 0x7fffffffll) return NCB_ERR_UNSUPPORTED;
-    CUtensorMap map = {};
+    if (key_rows > 0x7fffffffll || p.caps.split.entries * a.Hkv > 0x7fffffffll || p.caps.tile.entries * a.Hkv > 0x7fffffffll) return NCB_ERR_UNSUPPORTED;
+    CUtensorMap map = {}, map_q = {}, map_tile = {};
     if (!a.e4m3 && !tensor_map(a.pool, (int)key_rows, HEAD_DIM, 2 * PAGE_TOKENS, &map)) return NCB_ERR_LAUNCH;
     const cudaStream_t s = (cudaStream_t)stream;
+    if (p.caps.tiles) {
+        if (!query_map(a, p.caps.tile.rows_per, &map_q)) return NCB_ERR_LAUNCH;
+        if (!a.e4m3 && !tensor_map(a.pool, (int)key_rows, HEAD_DIM, PAGE_TOKENS, &map_tile)) return NCB_ERR_LAUNCH;
+        if ((a.e4m3 ? tile<true>(map_q, map_tile, p, s) : tile<false>(map_q, map_tile, p, s)) != cudaSuccess) return NCB_ERR_LAUNCH;
+    }
     if ((a.e4m3 ? split<true>(map, p, s) : split<false>(map, p, s)) != cudaSuccess) return NCB_ERR_LAUNCH;
     return launch(k_paged_merge, 4 * 148, 32 * MERGE_WARPS, 0, s, p) == cudaSuccess ? NCB_OK : NCB_ERR_LAUNCH;
 }

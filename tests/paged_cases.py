@@ -54,9 +54,20 @@ def attention(q, k, v, first_pos, window):
     return out, size
 
 
-def schedule(words, caps_entries):
-    """The entries and merges of a schedule as arrays."""
+def schedule(words, requests, rows, max_new, group, units):
+    """[(rows an owner has at most, entries, merges, most parts)] of a schedule: the split kernel's, the tile kernel's."""
     w = np.asarray(words)
-    entries = w[16:16 + 8 * w[0]].reshape(-1, 8)
-    at = 16 + 8 * caps_entries
-    return entries, w[at:at + 4 * w[1]].reshape(-1, 4)
+    per = [64 // group, 128 // group]
+    tiles = max_new > per[0]
+    each = min(requests, rows)
+    slots = min(max_new, per[0]) * group
+    merges = [units * (8 if slots <= 16 else 4), units]
+    parts = [2 * m for m in merges]
+    entries = [each + (0 if tiles else rows // per[0]) + parts[0], max(rows // per[1] + min(rows // (per[0] + 1), each), parts[1])]
+    found, at = [], 16
+    for i in range(1 + tiles):
+        m = at + 8 * entries[i]
+        found.append((per[i], w[at:at + 8 * w[2 * i]].reshape(-1, 8), w[m:m + 4 * w[2 * i + 1]].reshape(-1, 4), parts[i]))
+        at = m + 4 * merges[i]
+    assert len(w) == -(-at // 4) * 4
+    return found
