@@ -76,12 +76,12 @@ struct Cut {
 __device__ void schedule(const ncb_page_plan &a, const Requests &r, int window, int tile, int *work, long long *sums) {
     __shared__ unsigned long long best;
     const Caps caps = caps_of(a.requests, a.rows, a.max_fresh, a.group, a.kv_heads, a.blocks);
-    const Class &c = tile ? caps.tile : caps.split;
+    const Class &c = tile ? caps.tile : caps.small;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, per = (a.requests + THREADS - 1) / THREADS, b0 = tid * per;
-    const int rows_per = c.rows_per, rows = (int)a.rows, units = units_of(a.blocks, a.kv_heads);
+    const int rows_per = c.rows_per, rows = (int)a.rows, units = c.units;
     auto rows_of = [&](int b) { /* not served ones among them: zeros to write */
         const int n = min(r.row_end[b], rows) - min(b ? r.row_end[b - 1] : 0, rows);
-        return caps.tiles && (n > caps.split.rows_per) != (tile != 0) ? 0 : n;
+        return caps.tiles && (n > SMALL_SLOTS / a.group) != (tile != 0) ? 0 : n;
     };
     long long total, mine = 0;
     for (int b = b0; b < min(b0 + per, a.requests); b++) mine += (rows_of(b) + rows_per - 1) / rows_per;
@@ -169,12 +169,13 @@ __device__ void schedule(const ncb_page_plan &a, const Requests &r, int window, 
     if (tid == 0) {
         work[2 * tile] = (int)min(n_entries, c.entries), work[2 * tile + 1] = (int)min(n_merges, c.merges);
         if (!caps.tiles) work[2] = work[3] = 0;
+        if (!caps.smalls) work[0] = work[1] = 0;
     }
 }
 
 struct PlanArgs {
     ncb_page_plan p;
-    int row_blocks;
+    int row_blocks, first_class; /* 1: only tiles */
     long long words;
 };
 
@@ -219,7 +220,7 @@ __global__ void __launch_bounds__(THREADS) k_page_plan(const PlanArgs args) {
     long long taken;
     block_sum_before(mine, sums, &taken); /* its barriers publish the arrays */
     if (blockIdx.x >= args.row_blocks) {
-        const int w = (blockIdx.x - args.row_blocks) % a.n_windows, tile = (blockIdx.x - args.row_blocks) / a.n_windows;
+        const int w = (blockIdx.x - args.row_blocks) % a.n_windows, tile = (blockIdx.x - args.row_blocks) / a.n_windows + args.first_class;
         schedule(a, r, a.windows[w], tile, a.work + w * args.words, sums);
     } else {
         if (blockIdx.x == 0) {
@@ -366,14 +367,14 @@ int page_plan(const ncb_page_plan *args, void *stream) {
         return NCB_ERR_ARG;
     if ((uintptr_t)a.work % 16) return NCB_ERR_ALIGN;
     const Caps caps = caps_of(a.requests, a.rows, a.max_fresh, a.group, a.kv_heads, a.blocks);
-    PlanArgs p = {a, 1, page_plan_words(a.requests, a.rows, a.max_fresh, a.group, a.kv_heads, a.blocks)};
+    PlanArgs p = {a, 1, !caps.smalls, page_plan_words(a.requests, a.rows, a.max_fresh, a.group, a.kv_heads, a.blocks)};
     /* a block writes 2,048 rows in about the time that its sums take; more blocks than SMs would repeat them */
     p.row_blocks = (int)((a.rows + 2047) / 2048);
     p.row_blocks = p.row_blocks < 1 ? 1 : p.row_blocks > 64 ? 64 : p.row_blocks;
-    const long long listed = caps.split.owners > caps.tile.owners ? caps.split.owners : caps.tile.owners;
+    const long long listed = caps.small.owners > caps.tile.owners ? caps.small.owners : caps.tile.owners;
     const int smem = 4 * (5 * a.requests + (int)(listed < LISTED ? listed : LISTED));
     if (smem > 48 * 1024 && cudaFuncSetAttribute(k_page_plan, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return NCB_ERR_LAUNCH;
-    return launch(k_page_plan, p.row_blocks + a.n_windows * (caps.tiles ? 2 : 1), smem, (cudaStream_t)stream, p) == cudaSuccess ? NCB_OK : NCB_ERR_LAUNCH;
+    return launch(k_page_plan, p.row_blocks + a.n_windows * (caps.smalls + caps.tiles), smem, (cudaStream_t)stream, p) == cudaSuccess ? NCB_OK : NCB_ERR_LAUNCH;
 }
 
 int page_release(int *table, int *lens, const int *release, int *free_pages, int *free_count, int requests, int width, int n_pages, int *status,

@@ -55,19 +55,23 @@ def attention(q, k, v, first_pos, window):
 
 
 def schedule(words, requests, rows, max_new, group, units):
-    """[(rows an owner has at most, entries, merges, most parts)] of a schedule: the split kernel's, the tile kernel's."""
+    """[(rows an owner has at most, entries, merges, most parts)] of a schedule: the small kernel's, the tile kernel's, where they run."""
     w = np.asarray(words)
-    per = [64 // group, 128 // group]
-    tiles = max_new > per[0]
+    few, per = 16 // group, 128 // group
     each = min(requests, rows)
-    slots = min(max_new, per[0]) * group
-    merges = [units * (8 if slots <= 16 else 4), units]
-    parts = [2 * m for m in merges]
-    entries = [each + (0 if tiles else rows // per[0]) + parts[0], max(rows // per[1] + min(rows // (per[0] + 1), each), parts[1])]
     found, at = [], 16
-    for i in range(1 + tiles):
-        m = at + 8 * entries[i]
-        found.append((per[i], w[at:at + 8 * w[2 * i]].reshape(-1, 8), w[m:m + 4 * w[2 * i + 1]].reshape(-1, 4), parts[i]))
-        at = m + 4 * merges[i]
+    small, tile = few > 0, max_new > few
+    if small:
+        merges = 8 * units[0]
+        found.append((0, few, each + (0 if tile else rows // few) + 2 * merges, merges))
+    if tile:
+        found.append((2, per, max(rows // per + min(rows // (few + 1), each), 2 * units[1]), units[1]))
+    out = []
+    for head, limit, entries, merges in found:
+        m = at + 8 * entries
+        out.append((limit, w[at:at + 8 * w[head]].reshape(-1, 8), w[m:m + 4 * w[head + 1]].reshape(-1, 4), 2 * merges))
+        at = m + 4 * merges
     assert len(w) == -(-at // 4) * 4
-    return found
+    assert small or not w[:2].any()
+    assert tile or not w[2:4].any()
+    return out

@@ -53,7 +53,7 @@ def check_plan(cached, new, rows, max_new, n_pages, width, free=None, in_place=F
 
 def check_schedule(plan, want, cached, new, rows, group, Hkv, max_new):
     """Every row in reach once, every page of its owner once and in order, states without gaps, merges for exactly the cut owners."""
-    units = max(1, plan.blocks // Hkv)
+    units = [max(1, n // Hkv) for n in (plan.blocks // 2 * 3, plan.blocks)]
     each = len(plan.work) // len(plan.windows)
     for w, window in enumerate(plan.windows):
         cover = {}
