@@ -15,10 +15,6 @@ namespace {
 using namespace paged;
 
 constexpr int THREADS = 1024, WARPS = THREADS / 32;
-constexpr int LISTED = 16384; /* owners whose pages are kept in shared memory; where there are more, none is cut */
-constexpr int MIN_CHUNK = 2;  /* pages of a chunk */
-constexpr int OVERHEAD = 3;   /* what starting and ending a chunk costs, in pages */
-constexpr int WHOLE = 1 << 28; /* a chunk size that cuts nothing: a table is at most 2^24 wide */
 
 /* Exclusive prefix sum of v over the block's threads; *total gets the sum. */
 __device__ __forceinline__ long long block_sum_before(long long v, long long *sums, long long *total) {
@@ -61,115 +57,90 @@ struct Requests { /* shared memory, one value a request each */
     int *row_end, *page_end; /* inclusive sums of rows and of new pages */
     int *cached, *served;    /* served: rows, 0 for a request that is not */
     int *owner_end;          /* schedule blocks: inclusive sum of owners */
-    uint32_t *owner_pages;
 };
 
-struct Cut {
-    int pages, chunks, len; /* of one owner */
-    __device__ Cut(int pages, int chunk) : pages(pages) {
-        chunks = pages > 0 ? (pages + chunk - 1) / chunk : 1;
-        len = (pages + chunks - 1) / chunks; /* evened out: no stub at the end */
-    }
-};
-
-/* The schedule of one window's attention, of one class of requests. */
+/* The schedule of one window's attention, of one class of requests (paged.cuh). */
 __device__ void schedule(const ncb_page_plan &a, const Requests &r, int window, int tile, int *work, long long *sums) {
-    __shared__ unsigned long long best;
-    const Caps caps = caps_of(a.requests, a.rows, a.max_fresh, a.group, a.kv_heads, a.blocks);
+    const Caps caps = caps_of(a.requests, a.rows, a.max_fresh, a.group, a.blocks);
     const Class &c = tile ? caps.tile : caps.small;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, per = (a.requests + THREADS - 1) / THREADS, b0 = tid * per;
-    const int rows_per = c.rows_per, rows = (int)a.rows, units = c.units;
+    const int tid = threadIdx.x, per = (a.requests + THREADS - 1) / THREADS, b0 = tid * per, b1 = min(b0 + per, a.requests);
+    const int rows_per = c.rows_per, rows = (int)a.rows, few = SMALL_SLOTS / a.group;
     auto rows_of = [&](int b) { /* not served ones among them: zeros to write */
         const int n = min(r.row_end[b], rows) - min(b ? r.row_end[b - 1] : 0, rows);
-        return caps.tiles && (n > SMALL_SLOTS / a.group) != (tile != 0) ? 0 : n;
+        return caps.tiles && (n > few) != (tile != 0) ? 0 : n;
     };
     long long total, mine = 0;
-    for (int b = b0; b < min(b0 + per, a.requests); b++) mine += (rows_of(b) + rows_per - 1) / rows_per;
+    for (int b = b0; b < b1; b++) mine += (rows_of(b) + rows_per - 1) / rows_per;
     long long at = block_sum_before(mine, sums, &total);
-    for (int b = b0; b < min(b0 + per, a.requests); b++) r.owner_end[b] = (int)(at += (rows_of(b) + rows_per - 1) / rows_per);
+    for (int b = b0; b < b1; b++) r.owner_end[b] = (int)(at += (rows_of(b) + rows_per - 1) / rows_per);
     __syncthreads();
-    const int owners = (int)total;
-    struct Owner { int request, row0, rows, page0, page1; };
-    auto owner = [&](int o) {
-        Owner w;
-        w.request = first_above(r.owner_end, a.requests, o);
-        const int n = rows_of(w.request);
-        w.row0 = (o - (w.request ? r.owner_end[w.request - 1] : 0)) * rows_per;
-        w.rows = min(rows_per, n - w.row0);
-        w.page0 = w.page1 = 0;
-        if (r.served[w.request] > 0) {
-            const int first = r.cached[w.request] + w.row0;
-            w.page0 = window > 0 && first + 1 > window ? (first + 1 - window) / PAGE_TOKENS : 0;
-            w.page1 = (first + w.rows - 1) / PAGE_TOKENS + 1;
-        }
-        return w;
-    };
-    const bool listed = owners <= LISTED;
-    long long sum = 0;
-    for (int o = tid; o < owners; o += THREADS) {
-        const Owner w = owner(o);
-        sum += w.page1 - w.page0;
-        if (listed) r.owner_pages[o] = w.page1 - w.page0;
-    }
-    if (tid == 0) best = ~0ull;
-    long long pages;
-    block_sum_before(sum, sums, &pages); /* its barriers also publish owner_pages and best */
-    int chunk = WHOLE;
-    if (listed && pages > 0) {
-        /* Each warp estimates the time of one chunk size, in sixteenths of a page: every unit's share of entries of the mean length, and half of what the
-         * longest is longer. Warp 0: nothing is cut; warp w: chunks of total / (units * waves * w / 32) pages. */
-        auto chunk_of = [&](int w) {
-            const long long shares = (long long)units * c.waves * w; /* in 32nds */
-            return w == 0 ? WHOLE : (int)max((long long)MIN_CHUNK, (32 * pages + shares - 1) / shares);
-        };
-        const int size = chunk_of(warp);
-        long long n = 0;
-        int longest = 0;
-        for (int o = lane; o < owners; o += 32) {
-            const Cut cut(r.owner_pages[o], size);
-            n += cut.chunks;
-            longest = max(longest, cut.len);
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            n += __shfl_xor_sync(0xffffffffu, n, o);
-            longest = max(longest, __shfl_xor_sync(0xffffffffu, longest, o));
-        }
-        const long long mean = 16 * pages / n, each = mean + 16 * OVERHEAD, most = 16ll * longest;
-        long long cost = max((n + units - 1) / units * each + (most - mean) / 2, most + 16 * OVERHEAD);
-        if (n > owners) cost += 16 * OVERHEAD; /* states are written and read again */
-        if (lane == 0 && (!tile || n == owners || n <= c.parts)) atomicMin(&best, (unsigned long long)cost << 32 | (unsigned)warp);
-        __syncthreads();
-        chunk = chunk_of((int)(best & 0xffffffffu));
-    }
-    Entry *entries = reinterpret_cast<Entry *>(work + entries_at(caps, tile));
-    Merge *merges = reinterpret_cast<Merge *>(work + merges_at(caps, tile));
-    long long n_entries = 0, n_parts = 0, n_merges = 0;
-    for (int from = 0; from < owners; from += THREADS) { /* the last rows of a request reach furthest: they start first */
-        const int o = owners - 1 - from - tid;
+    const int owners = (int)min(total, c.owners);
+    work += class_at(caps, tile);
+    Owner *records = reinterpret_cast<Owner *>(work + HEADER_WORDS);
+    int *before = r.page_end; /* the sums once more, for the searches below (nobody reads the pages' in this block) */
+    long long weight = 0;
+    for (int from = 0; from < owners; from += THREADS) {
+        const int o = from + tid;
         Owner w = {};
-        int chunks = 0, len = 0;
-        if (o >= 0) {
-            w = owner(o);
-            const Cut cut(w.page1 - w.page0, chunk);
-            chunks = cut.chunks, len = cut.len;
+        if (o < owners) {
+            w.request = first_above(r.owner_end, a.requests, o);
+            const int row0 = (o - (w.request ? r.owner_end[w.request - 1] : 0)) * rows_per;
+            w.row = (w.request ? r.row_end[w.request - 1] : 0) + row0;
+            w.rows = min(rows_per, rows_of(w.request) - row0);
+            if (r.served[w.request] > 0) {
+                w.pos = r.cached[w.request] + row0;
+                w.page0 = window > 0 && w.pos + 1 > window ? (w.pos + 1 - window) / PAGE_TOKENS : 0;
+                w.pages = (w.pos + w.rows - 1) / PAGE_TOKENS + 1 - w.page0;
+            }
         }
-        const int parts = chunks > 1 ? chunks : 0;
-        long long t, t2; /* entries; parts, and merges above them */
-        const long long e = n_entries + block_sum_before(chunks, sums, &t), pm = block_sum_before(parts | (long long)(parts > 0) << 32, sums, &t2);
-        const long long p = n_parts + (pm & 0xffffffffll), m = n_merges + (pm >> 32);
-        for (int i = 0; i < chunks; i++) {
-            if (e + i >= c.entries || (parts && p + i >= c.parts)) break; /* cannot be: see Caps */
-            Entry x = {w.request, w.row0, w.rows, w.page0 + i * len, min(w.page0 + (i + 1) * len, w.page1), parts ? (int)p + i : -1, {0, 0}};
-            entries[e + i] = x;
+        const long long sum = weight + block_sum_before(o < owners ? max(w.pages, 1) + c.overhead : 0, sums, &total);
+        if (o < owners) {
+            w.before = (int)sum;
+            records[o] = w;
+            if (o < a.requests) before[o] = w.before;
         }
-        if (parts && m < c.merges) merges[m] = Merge{(w.request ? r.row_end[w.request - 1] : 0) + w.row0, w.rows, (int)p, parts};
-        n_entries += t, n_parts += t2 & 0xffffffffll, n_merges += t2 >> 32;
+        weight += total;
     }
-    if (tid == 0) {
-        work[2 * tile] = (int)min(n_entries, c.entries), work[2 * tile + 1] = (int)min(n_merges, c.merges);
-        if (!caps.tiles) work[2] = work[3] = 0;
-        if (!caps.smalls) work[0] = work[1] = 0;
+    const long long all = weight * a.kv_heads, share = min(max((all + c.blocks - 1) / c.blocks, (long long)c.least), 0x7fffffffll);
+    /* Enough tiles for every block: the GPU's own order balances them, and states of cut ones (128 slots each) would cost more than that leaves. */
+    const bool whole = tile && (long long)owners * a.kv_heads >= (long long)WHOLE_ROUNDS * c.blocks;
+    if (tid == 0) *reinterpret_cast<int4 *>(work) = make_int4(owners, (int)weight, (int)share, whole);
+    if (whole || owners == 0) return;
+    __syncthreads();
+    Start *starts = reinterpret_cast<Start *>(work + starts_at(c));
+    Piece *pieces = reinterpret_cast<Piece *>(work + pieces_at(c));
+    const bool listed = owners <= a.requests;
+    long long count = 0; /* of pieces */
+    for (int from = 0; from <= c.blocks; from += THREADS) {
+        const int b = from + tid;
+        const long long x = b * share;
+        const bool on = b <= c.blocks && x < all;
+        Start start = {0, 0, 0, 0};
+        if (on) {
+            start.head = (int)(x / weight);
+            const int place = (int)(x - start.head * weight);
+            int low = 0, high = owners; /* the last owner whose `before` is at most `place` */
+            while (high - low > 1) {
+                const int mid = (low + high) >> 1;
+                if ((listed ? before[mid] : records[mid].before) <= place) low = mid;
+                else high = mid;
+            }
+            start.owner = low, start.local = place - (listed ? before[low] : records[low].before);
+        }
+        if (tile) { /* the block's pieces: counted, then written */
+            int mine = 0;
+            if (on)
+                for (Walk walk(records, owners, c.overhead, (int)share, start, all - x, b); walk.next();) mine++;
+            const long long to = count + block_sum_before(mine, sums, &total);
+            start.piece = (int)to;
+            if (on) {
+                int i = 0;
+                for (Walk walk(records, owners, c.overhead, (int)share, start, all - x, b); walk.next() && to + i < (WHOLE_ROUNDS + 1ll) * c.blocks; i++)
+                    pieces[to + i] = Piece{walk.o.request, walk.o.row, walk.o.rows, walk.o.pos, walk.o.page0 + walk.page0, walk.page1 - walk.page0, walk.head, walk.part};
+            }
+            count += total;
+        }
+        if (b <= c.blocks) starts[b] = start;
     }
 }
 
@@ -187,7 +158,7 @@ __global__ void __launch_bounds__(THREADS) k_page_plan(const PlanArgs args) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int tid = threadIdx.x, n = a.requests, per = (n + THREADS - 1) / THREADS, b0 = tid * per, end = min(b0 + per, n);
-    const Requests r = {smem, smem + n, smem + 2 * n, smem + 3 * n, smem + 4 * n, reinterpret_cast<uint32_t *>(smem + 5 * n)};
+    const Requests r = {smem, smem + n, smem + 2 * n, smem + 3 * n, smem + 4 * n};
     const int free_count = max(0, min(*reinterpret_cast<const volatile int *>(a.free_count), a.n_pages));
     for (int b = tid; b < n; b += THREADS) r.cached[b] = a.cached[b], r.served[b] = a.fresh[b];
     __syncthreads();
@@ -351,28 +322,26 @@ extern "C" {
 
 long long page_plan_words(int requests, long long rows, int max_fresh, int group, int kv_heads, int blocks) {
     if (!sizes_ok(requests, rows, max_fresh, group, kv_heads, blocks)) return -1;
-    const long long words = schedule_words(caps_of(requests, rows, max_fresh, group, kv_heads, blocks));
-    return (words + 3) / 4 * 4; /* schedules one after the other stay 16-byte aligned */
+    return schedule_words(caps_of(requests, rows, max_fresh, group, blocks));
 }
 
 int page_plan(const ncb_page_plan *args, void *stream) {
     if (!args) return NCB_ERR_ARG;
     const ncb_page_plan &a = *args;
     if (!sizes_ok(a.requests, a.rows, a.max_fresh, a.group, a.kv_heads, a.blocks)) return NCB_ERR_ARG;
-    if (a.width <= 0 || a.width > (1 << 24) || a.n_pages <= 0 || a.n_pages > 0x7fffffff / PAGE_TOKENS || a.n_windows < 0 || a.n_windows > NCB_PLAN_WINDOWS) return NCB_ERR_ARG;
+    if (a.width <= 0 || a.width > (1 << 16) || a.n_pages <= 0 || a.n_pages > 0x7fffffff / PAGE_TOKENS || a.n_windows < 0 || a.n_windows > NCB_PLAN_WINDOWS) return NCB_ERR_ARG;
     for (int w = 0; w < a.n_windows; w++)
         if (a.windows[w] < 0) return NCB_ERR_ARG;
     if (!a.table || !a.cached || !a.fresh || !a.free_pages || !a.free_count || !a.free_left || !a.row_start || !a.served || !a.lens || !a.ticket ||
         (a.rows > 0 && (!a.pos || !a.place || !a.request)) || (a.n_windows > 0 && !a.work))
         return NCB_ERR_ARG;
     if ((uintptr_t)a.work % 16) return NCB_ERR_ALIGN;
-    const Caps caps = caps_of(a.requests, a.rows, a.max_fresh, a.group, a.kv_heads, a.blocks);
-    PlanArgs p = {a, 1, !caps.smalls, page_plan_words(a.requests, a.rows, a.max_fresh, a.group, a.kv_heads, a.blocks)};
+    const Caps caps = caps_of(a.requests, a.rows, a.max_fresh, a.group, a.blocks);
+    PlanArgs p = {a, 1, !caps.smalls, schedule_words(caps)};
     /* a block writes 2,048 rows in about the time that its sums take; more blocks than SMs would repeat them */
     p.row_blocks = (int)((a.rows + 2047) / 2048);
     p.row_blocks = p.row_blocks < 1 ? 1 : p.row_blocks > 64 ? 64 : p.row_blocks;
-    const long long listed = caps.small.owners > caps.tile.owners ? caps.small.owners : caps.tile.owners;
-    const int smem = 4 * (5 * a.requests + (int)(listed < LISTED ? listed : LISTED));
+    const int smem = 4 * 5 * a.requests;
     if (smem > 48 * 1024 && cudaFuncSetAttribute(k_page_plan, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return NCB_ERR_LAUNCH;
     return launch(k_page_plan, p.row_blocks + a.n_windows * (caps.smalls + caps.tiles), smem, (cudaStream_t)stream, p) == cudaSuccess ? NCB_OK : NCB_ERR_LAUNCH;
 }

@@ -1,8 +1,14 @@
 /*
- * Shared by page_plan.cu and paged_attn.cu: what the schedule of a paged attention call looks like in memory, and how much of it
- * there can be. Work is cut into owners: the `rows_per` consecutive new rows of one request (with all query heads of a key/value head:
- * query slots) that one block takes; an owner's pages are cut into chunks of at most a chosen number of pages. An owner of several chunks leaves
- * a state per chunk in the workspace and is listed for the merge.
+ * Shared by page_plan.cu and paged_attn.cu: the schedule of a paged attention call. Work is cut into owners: consecutive new rows of one request
+ * which, with all query heads of a key/value head (query slots), one block can take. Requests of at most SMALL_SLOTS query slots belong to the small kernel,
+ * the others to the tile kernel; each class has a schedule of its own.
+ *
+ * An owner weighs its pages and OVERHEAD (what a block spends on it besides); `before` are the exclusive sums of the weights, `total` their sum. The work of all
+ * key/value heads, one after the other, is a line of length total * heads, and block b has the piece [b * share, (b + 1) * share) of it, wherever owners
+ * begin and end: every block has the same to do, whatever the lengths are. A block leaves at most two owners unfinished, the one that it goes on with
+ * from the block before it and the one that the next block goes on with: their states go to parts 2 b and 2 b + 1, and whoever joins them finds
+ * them from the sums alone. Where tiles are so many that they fill the GPU several times over, none is cut (WHOLE): each is a block's, the
+ * longest first, and no state is written or read.
  */
 #pragma once
 
@@ -13,88 +19,136 @@ namespace paged {
 
 constexpr int SMALL_SLOTS = 16, TILE_SLOTS = 128; /* query slots of a block of the small kernel, of the tile kernel */
 constexpr int MAX_GROUP = 64;                     /* query heads per key/value head */
-constexpr int TILE_WAVES = 2;                     /* cut tiles are at most this often what runs at once */
-constexpr int HEADER_WORDS = 16;                  /* entries and merges of the small kernel, of the tile kernel */
-constexpr int ENTRY_WORDS = 8, MERGE_WORDS = 4;
+constexpr int HEADER_WORDS = 8;                   /* owners, total, share, whole: of a class */
+constexpr int OWNER_WORDS = 8, START_WORDS = 4, PIECE_WORDS = 8;
+constexpr int WHOLE_ROUNDS = 3; /* tiles are cut only where there are fewer than this many for every block */
 
-struct Entry { /* one block's work, for each key/value head */
-    int request, row0, rows;  /* rows row0 .. of the request's new rows */
-    int page0, page1;         /* pages of the request */
-    int part;                 /* where its state goes; -1: the block normalises and writes its rows itself */
-    int pad[2];
+struct Owner {
+    int request, row, rows; /* absolute first row */
+    int pos;                /* position of the first row */
+    int page0, pages;       /* pages of the request that its rows see; no pages: rows that are not served, to become zeros */
+    int before;             /* weights of the owners before it */
+    int pad;
 };
-struct Merge { /* an owner of several chunks */
-    int row, rows; /* absolute rows */
-    int part, parts;
+/* Where a block's part of the line begins. */
+struct Start {
+    int owner, head;
+    int local; /* place within the owner, whose overhead comes first */
+    int piece; /* tiles: the block's first piece; the next block's is behind its last */
 };
-static_assert(sizeof(Entry) == 4 * ENTRY_WORDS && sizeof(Merge) == 4 * MERGE_WORDS, "schedule layout");
+/* A block's share of an owner, ready for the tile kernel. */
+struct Piece {
+    int request, row, rows, pos; /* as the owner's */
+    int page0, pages;            /* of the request */
+    int head;
+    int part; /* where the state goes; -1: it is the whole owner, and the block writes its rows */
+};
+static_assert(sizeof(Owner) == 4 * OWNER_WORDS && sizeof(Start) == 4 * START_WORDS && sizeof(Piece) == 4 * PIECE_WORDS, "schedule layout");
 
-/* How many entries a schedule may aim at: every key/value head runs each of them. */
-static __host__ __device__ __forceinline__ int units_of(int blocks, int kv_heads) { return blocks / kv_heads > 1 ? blocks / kv_heads : 1; }
-
-static __host__ __device__ __forceinline__ int small_blocks(int blocks) { return blocks / 2 * 3; } /* three per SM instead of two */
-
-/* Bounds of a schedule, and where its parts lie. The tile kernel has the requests of more than SMALL_SLOTS query slots, the small kernel the
- * others; where no request may have so many, no tile kernel runs, and the small kernel also has what is too long and only gets zeros.
- * A chunk of the small kernel is at least total / (waves * units) pages: the owners that are cut are at most waves * units, their
- * chunks at most twice that. Tiles are cut only where all entries are then at most TILE_WAVES * units. */
 struct Class {
-    long long owners, entries, merges, parts;
+    long long owners; /* at most */
     int rows_per, slots; /* of an owner */
-    int units, waves;
+    int blocks, overhead, least; /* blocks that run at once; weight of an owner besides its pages; least share */
 };
 struct Caps {
     Class small, tile;
-    int smalls, tiles; /* whether the kernel has anything */
+    int smalls, tiles; /* whether the kernel has anything. Without tiles the small kernel also has what is too long and only gets zeros. */
 };
-static __host__ __device__ __forceinline__ Caps caps_of(int requests, long long rows, int max_fresh, int group, int kv_heads, int blocks) {
+/* `blocks`: SMs; three blocks of the small kernel run on each, two of the tile kernel. */
+static __host__ __device__ __forceinline__ Caps caps_of(int requests, long long rows, int max_fresh, int group, int blocks) {
     Caps c = {};
     const long long one_each = requests < rows ? requests : rows;
     const int few = SMALL_SLOTS / group; /* 0: even one row has too many slots */
-    c.smalls = few > 0, c.tiles = max_fresh > few;
+    c.smalls = few > 0 && rows > 0, c.tiles = max_fresh > few && rows > few;
     if (c.smalls) {
         c.small.rows_per = few;
         c.small.slots = (max_fresh < few ? max_fresh : few) * group;
-        c.small.units = units_of(small_blocks(blocks), kv_heads);
         c.small.owners = one_each + (c.tiles ? 0 : rows / few);
-        c.small.waves = 8;
-        c.small.merges = (long long)c.small.units * c.small.waves;
-        c.small.parts = 2 * c.small.merges;
-        c.small.entries = c.small.owners + c.small.parts;
+        c.small.blocks = 3 * blocks, c.small.overhead = 2, c.small.least = 6;
     }
     if (c.tiles) {
         const long long longer = rows / (few + 1); /* requests that have tiles */
         c.tile.rows_per = TILE_SLOTS / group;
         c.tile.slots = (max_fresh < c.tile.rows_per ? max_fresh : c.tile.rows_per) * group;
-        c.tile.units = units_of(blocks, kv_heads);
         c.tile.owners = rows / c.tile.rows_per + (longer < one_each ? longer : one_each);
-        c.tile.waves = TILE_WAVES;
-        c.tile.parts = (long long)c.tile.units * TILE_WAVES;
-        c.tile.merges = c.tile.parts / 2;
-        c.tile.entries = c.tile.owners > c.tile.parts ? c.tile.owners : c.tile.parts;
+        c.tile.blocks = 2 * blocks, c.tile.overhead = 4, c.tile.least = 8;
     }
     return c;
 }
-static __host__ __device__ __forceinline__ long long class_words(const Class &c) { return c.entries * ENTRY_WORDS + c.merges * MERGE_WORDS; }
-static __host__ __device__ __forceinline__ long long schedule_words(const Caps &c) { return HEADER_WORDS + class_words(c.small) + class_words(c.tile); }
-/* Offsets in a schedule, in words, and in a workspace, in floats. */
-static __host__ __device__ __forceinline__ long long entries_at(const Caps &c, int tile) { return HEADER_WORDS + (tile ? class_words(c.small) : 0); }
-static __host__ __device__ __forceinline__ long long merges_at(const Caps &c, int tile) {
-    return entries_at(c, tile) + (tile ? c.tile.entries : c.small.entries) * ENTRY_WORDS;
+/* A class in a schedule: header, owners, starts (of one block more than there are), for tiles the pieces: one per owner and head and one per cut. */
+static __host__ __device__ __forceinline__ long long starts_at(const Class &c) { return HEADER_WORDS + c.owners * OWNER_WORDS; }
+static __host__ __device__ __forceinline__ long long pieces_at(const Class &c) { return starts_at(c) + (c.blocks + 2) / 2 * 2 * START_WORDS; }
+static __host__ __device__ __forceinline__ long long class_words(const Class &c, bool tile) {
+    return c.owners ? pieces_at(c) + (tile ? (WHOLE_ROUNDS + 1ll) * c.blocks * PIECE_WORDS : 0) : 0;
 }
-static __host__ __device__ __forceinline__ long long parts_at(const Caps &c, int kv_heads, int tile) { return tile ? c.small.parts * kv_heads * c.small.slots * PART : 0; }
-static __host__ __device__ __forceinline__ long long workspace_floats(const Caps &c, int kv_heads) {
-    return parts_at(c, kv_heads, 1) + c.tile.parts * kv_heads * c.tile.slots * PART;
-}
+static __host__ __device__ __forceinline__ long long schedule_words(const Caps &c) { return class_words(c.small, false) + class_words(c.tile, true); }
+static __host__ __device__ __forceinline__ long long class_at(const Caps &c, int tile) { return tile ? class_words(c.small, false) : 0; }
+/* Floats of the workspace: two parts per block of each class. */
+static __host__ __device__ __forceinline__ long long parts_at(const Caps &c, int tile) { return tile ? 2ll * c.small.blocks * c.small.slots * PART : 0; }
+static __host__ __device__ __forceinline__ long long workspace_floats(const Caps &c) { return parts_at(c, 1) + 2ll * c.tile.blocks * c.tile.slots * PART; }
+
 static __host__ __forceinline__ bool sizes_ok(int requests, long long rows, int max_fresh, int group, int kv_heads, int blocks) {
     return requests > 0 && requests <= NCB_PLAN_REQUESTS && rows >= 0 && rows <= (1ll << 26) && max_fresh > 0 && group > 0 && group <= MAX_GROUP &&
-           kv_heads > 0 && kv_heads <= 65535 && blocks > 0 && blocks <= (1 << 20);
+           kv_heads > 0 && kv_heads <= 65535 && blocks > 0 && blocks <= (1 << 16);
 }
 
 struct PagedArgs { /* of paged_attn's kernels */
     ncb_paged p;
     Caps caps;
     float scale_log2;
+};
+
+/* A class's schedule as kernels read it. */
+struct Line {
+    const Owner *owners;
+    const Start *starts;
+    const Piece *pieces;
+    int n, heads, overhead;
+    long long total, share; /* of one key/value head; of a block */
+    bool whole;
+
+    __device__ __forceinline__ Line(const PagedArgs &args, int tile) {
+        const Class &c = tile ? args.caps.tile : args.caps.small;
+        const int *w = args.p.work + class_at(args.caps, tile);
+        const int4 header = *reinterpret_cast<const int4 *>(w);
+        owners = reinterpret_cast<const Owner *>(w + HEADER_WORDS);
+        starts = reinterpret_cast<const Start *>(w + starts_at(c));
+        pieces = reinterpret_cast<const Piece *>(w + pieces_at(c));
+        n = header.x, total = header.y, share = header.z, whole = header.w != 0;
+        heads = args.p.Hkv, overhead = c.overhead;
+    }
+    __device__ __forceinline__ long long all() const { return total * heads; }
+    /* First and last block that has pages of an owner. */
+    __device__ __forceinline__ int first_block(int head, const Owner &o) const { return (int)((head * total + o.before + overhead) / share); }
+    __device__ __forceinline__ int last_block(int head, const Owner &o) const { return (int)((head * total + o.before + overhead + max(o.pages, 1) - 1) / share); }
+};
+
+/* What a block of a class that is cut does, one piece after the other. */
+struct Walk {
+    Owner o;
+    int head, page0, page1; /* the piece: pages [page0, page1) of the owner's, for this key/value head */
+    int part;               /* as Piece's */
+
+    __device__ __forceinline__ Walk(const Owner *owners, int n, int overhead, int share, const Start &start, long long left, int block)
+        : owners(owners), n(n), overhead(overhead), at(start.owner), next_head(start.head), local(start.local), left((int)min((long long)share, left)), block(block) {}
+    /* The next piece; false at the end. */
+    __device__ __forceinline__ bool next() {
+        while (left > 0) {
+            o = owners[at], head = next_head;
+            const int pages = max(o.pages, 1), from = max(local - overhead, 0), to = min(local + left - overhead, pages);
+            const int used = overhead + pages - local; /* to the owner's end */
+            part = from == 0 && to == pages ? -1 : 2 * block + (from == 0);
+            page0 = from, page1 = min(to, o.pages);
+            left -= used, local = 0;
+            if (++at == n) at = 0, next_head++;
+            if (from < to) return true; /* else only (some of) its overhead lies here */
+        }
+        return false;
+    }
+
+private:
+    const Owner *owners;
+    int n, overhead, at, next_head, local, left, block;
 };
 
 } /* namespace paged */

@@ -15,7 +15,7 @@
  * What a row does not see must not reach it, not even as zero times a NaN or an infinity: scores are masked by selects, and a unit that is not
  * seen whole by every slot has its values looked at; if one is not finite, its products are made row by row over the keys seen.
  *
- * k_paged_merge: the states of owners that were cut, one warp per query slot.
+ * k_paged_tiles (paged_tiles.cuh), for the others: tcgen05. k_paged_merge: the states of owners that were cut.
  * Waits are bounded: when one expires NCB_DEV_WAIT_TIMEOUT is flagged and the block leaves after its copies in flight.
  */
 #include "paged_tiles.cuh"
@@ -146,16 +146,19 @@ template <bool E4M3, int NT> __global__ void __launch_bounds__(32 * WARPS, BLOCK
     __syncthreads();
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const int G = a.Hq / a.Hkv, jobs = a.work[0] * a.Hkv;
+    const int G = a.Hq / a.Hkv;
     const uint64_t once = policy_evict_first();
     uint32_t loads = 0; /* of this warp so far: the parity of its barrier */
-    for (int job = blockIdx.x; job < jobs; job += gridDim.x) {
-        const int kvh = job % a.Hkv;
-        const Entry e = reinterpret_cast<const Entry *>(a.work + entries_at(args.caps, 0))[job / a.Hkv];
-        const int slots = e.rows * G, units = (e.page1 - e.page0) * U::PER_PAGE;
-        const int first_pos = a.lens[e.request] - a.served[e.request] + e.row0, last_pos = first_pos + e.rows - 1;
-        const long long first_row = a.row_start[e.request] + e.row0;
-        const int *table = a.table + (size_t)e.request * a.width + e.page0;
+    const Line line(args, 0);
+    const Start start = line.starts[blockIdx.x];
+    if (blockIdx.x * line.share >= line.all()) return;
+    Walk walk(line.owners, line.n, line.overhead, (int)line.share, start, line.all() - blockIdx.x * line.share, blockIdx.x);
+    while (walk.next()) {
+        const Owner &e = walk.o;
+        const int kvh = walk.head, page0 = e.page0 + walk.page0, part_at = walk.part;
+        const int slots = e.rows * G, units = (walk.page1 - walk.page0) * U::PER_PAGE, first_pos = e.pos, last_pos = e.pos + e.rows - 1;
+        const long long first_row = e.row;
+        const int *table = a.table + (size_t)e.request * a.width + page0;
         auto begin_of = [&](int pos) { return a.window > 0 ? max(0, pos + 1 - a.window) : 0; }; /* the first position that the row at pos sees */
         /* Unit i into this warp's place; false where its page is not in the pool (nothing is fetched). */
         auto fetch = [&](int i, int page) {
@@ -228,7 +231,7 @@ template <bool E4M3, int NT> __global__ void __launch_bounds__(32 * WARPS, BLOCK
         }
         bool ok = true;
         for (int i = warp; i < units; i += WARPS) {
-            const int unit_pos = (e.page0 * U::PER_PAGE + i) * U::KEYS;
+            const int unit_pos = (page0 * U::PER_PAGE + i) * U::KEYS;
             const int next = i + WARPS < units ? table[(i + WARPS) / U::PER_PAGE] : 0;
             if (there && !__all_sync(0xffffffffu, mbar_wait(bar, loads & 1))) {
                 if (lane == 0) flag(a.status, NCB_DEV_WAIT_TIMEOUT), failed = 1;
@@ -432,12 +435,12 @@ template <bool E4M3, int NT> __global__ void __launch_bounds__(32 * WARPS, BLOCK
                 sum = fmaf(state_l[w][slot], f, sum);
                 if (f != 0.f) x.x = fmaf(v.x, f, x.x), x.y = fmaf(v.y, f, x.y), x.z = fmaf(v.z, f, x.z), x.w = fmaf(v.w, f, x.w);
             }
-            if (e.part < 0) {
+            if (part_at < 0) {
                 const float inv = sum > 0.f || sum != sum ? __fdiv_rn(1.f, E4M3 ? sum * P_SCALE : sum) : 0.f;
                 *reinterpret_cast<uint2 *>((bf16 *)a.out + (first_row + slot / G) * a.ldo + (size_t)(kvh * G + slot % G) * HEAD_DIM + 4 * lane) =
                     make_uint2(pack_bf16(x.x * inv, x.y * inv), pack_bf16(x.z * inv, x.w * inv));
             } else {
-                float *part = (float *)a.workspace + ((size_t)((long long)e.part * a.Hkv + kvh) * args.caps.small.slots + slot) * PART;
+                float *part = (float *)a.workspace + ((size_t)part_at * args.caps.small.slots + slot) * PART;
                 if (lane == 0) part[0] = top, part[1] = sum;
                 *reinterpret_cast<float4 *>(part + 4 + 4 * lane) = x;
             }
@@ -448,44 +451,43 @@ template <bool E4M3, int NT> __global__ void __launch_bounds__(32 * WARPS, BLOCK
     }
 }
 
-constexpr int MERGE_WARPS = 4;
+constexpr int MERGE_WARPS = 4, MERGE_SLOTS = 16;
 
-/* A warp per query slot of an owner that was cut; lanes have four dimensions each. */
+/* Joins the states of owners that were cut: a block per end of a piece of the line (and 16 of a tile's slots) looks whether an owner is cut there for the first
+ * time. A warp per query slot, four dimensions a lane. */
 __global__ void __launch_bounds__(32 * MERGE_WARPS) k_paged_merge(const PagedArgs args) {
     const ncb_paged &a = args.p;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const int lane = threadIdx.x & 31, G = a.Hq / a.Hkv, warps = gridDim.x * MERGE_WARPS;
-    long long job = (long long)blockIdx.x * MERGE_WARPS + threadIdx.x / 32;
-    for (int tile = 0; tile <= args.caps.tiles; tile++) {
-        const Class &cls = tile ? args.caps.tile : args.caps.small;
-        const Merge *merges = reinterpret_cast<const Merge *>(a.work + merges_at(args.caps, tile));
-        const float *parts = (const float *)a.workspace + parts_at(args.caps, a.Hkv, tile);
-        const long long jobs = (long long)a.work[2 * tile + 1] * a.Hkv * cls.slots;
-        for (; job < jobs; job += warps) {
-            const int slot = (int)(job % cls.slots), kvh = (int)(job / cls.slots % a.Hkv);
-            const Merge e = merges[job / cls.slots / a.Hkv];
-            if (slot >= e.rows * G) continue;
-            const float *part = parts + ((size_t)((long long)e.part * a.Hkv + kvh) * cls.slots + slot) * PART;
-            const size_t step = (size_t)a.Hkv * cls.slots * PART;
-            float top = -INFINITY, sum = 0.f;
-            for (int c = lane; c < e.parts; c += 32) top = fmaxf(top, part[c * step]);
+    const int smalls = args.caps.smalls ? args.caps.small.blocks : 0, tile = (int)blockIdx.x >= smalls, lane = threadIdx.x & 31, G = a.Hq / a.Hkv;
+    const Class &cls = tile ? args.caps.tile : args.caps.small;
+    const int groups = tile ? (cls.slots + MERGE_SLOTS - 1) / MERGE_SLOTS : 1, job = blockIdx.x - (tile ? smalls : 0), end = job / groups + 1, slot0 = job % groups * MERGE_SLOTS;
+    const Line line(args, tile);
+    const Start start = line.starts[end];
+    if (line.n == 0 || line.whole || end * line.share >= line.all()) return;
+    const int head = start.head;
+    const Owner o = line.owners[start.owner];
+    const int first = line.first_block(head, o), last = line.last_block(head, o);
+    if (first != end - 1 || last < end) return;
+    for (int slot = slot0 + (int)threadIdx.x / 32; slot < min(slot0 + MERGE_SLOTS, o.rows * G); slot += MERGE_WARPS) {
+        const float *parts = (const float *)a.workspace + parts_at(args.caps, tile);
+        auto part = [&](int b) { return parts + ((size_t)(2 * b + (b == first)) * cls.slots + slot) * PART; };
+        float top = -INFINITY, sum = 0.f;
+        for (int b = first + lane; b <= last; b += 32) top = fmaxf(top, part(b)[0]);
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-            float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+        float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-            for (int c = 0; c < e.parts; c++) {
-                const float2 ml = *reinterpret_cast<const float2 *>(part + c * step);
-                const float4 v = *reinterpret_cast<const float4 *>(part + c * step + 4 + 4 * lane);
-                const float f = scale_of(ml.x, ml.y, top);
-                sum = fmaf(ml.y, f, sum);
-                if (f != 0.f) x.x = fmaf(v.x, f, x.x), x.y = fmaf(v.y, f, x.y), x.z = fmaf(v.z, f, x.z), x.w = fmaf(v.w, f, x.w);
-            }
-            const float inv = sum > 0.f || sum != sum ? __fdiv_rn(1.f, a.e4m3 ? sum * P_SCALE : sum) : 0.f;
-            const uint2 y = make_uint2(pack_bf16(x.x * inv, x.y * inv), pack_bf16(x.z * inv, x.w * inv));
-            *reinterpret_cast<uint2 *>((bf16 *)a.out + (e.row + slot / G) * a.ldo + (size_t)(kvh * G + slot % G) * HEAD_DIM + 4 * lane) = y;
+        for (int b = first; b <= last; b++) {
+            const float2 ml = *reinterpret_cast<const float2 *>(part(b));
+            const float4 v = *reinterpret_cast<const float4 *>(part(b) + 4 + 4 * lane);
+            const float f = scale_of(ml.x, ml.y, top);
+            sum = fmaf(ml.y, f, sum);
+            if (f != 0.f) y.x = fmaf(v.x, f, y.x), y.y = fmaf(v.y, f, y.y), y.z = fmaf(v.z, f, y.z), y.w = fmaf(v.w, f, y.w);
         }
-        job -= jobs;
+        const float inv = sum > 0.f || sum != sum ? __fdiv_rn(1.f, a.e4m3 ? sum * P_SCALE : sum) : 0.f;
+        *reinterpret_cast<uint2 *>((bf16 *)a.out + (o.row + slot / G) * a.ldo + (size_t)(head * G + slot % G) * HEAD_DIM + 4 * lane) =
+            make_uint2(pack_bf16(y.x * inv, y.y * inv), pack_bf16(y.z * inv, y.w * inv));
     }
 }
 
@@ -507,14 +509,14 @@ template <bool E4M3, int NT> cudaError_t small(const CUtensorMap &map, const Pag
     constexpr int smem = Unit<E4M3>::SMEM;
     const cudaError_t rc = cudaFuncSetAttribute(k_paged_small<E4M3, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (rc != cudaSuccess) return rc;
-    const long long jobs = args.caps.small.entries * args.p.Hkv, most = small_blocks(args.p.blocks);
-    return launch(k_paged_small<E4M3, NT>, (unsigned)(jobs < most ? jobs : most), 32 * WARPS, smem, stream, map, args);
+    return launch(k_paged_small<E4M3, NT>, args.caps.small.blocks, 32 * WARPS, smem, stream, map, args);
 }
 template <bool E4M3> cudaError_t tile(const CUtensorMap &map_q, const CUtensorMap &map_kv, const PagedArgs &args, cudaStream_t stream) {
     constexpr int smem = tiles::Shape<E4M3>::SMEM;
     const cudaError_t rc = cudaFuncSetAttribute(tiles::k_paged_tiles<E4M3>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (rc != cudaSuccess) return rc;
-    return launch(tiles::k_paged_tiles<E4M3>, (unsigned)(args.caps.tile.entries * args.p.Hkv), E4M3 ? tiles::THREADS : 32 * tiles::WIDEN_WARP, smem, stream, map_q, map_kv, args);
+    const long long whole = args.caps.tile.owners * args.p.Hkv; /* blocks where no tile is cut */
+    return launch(tiles::k_paged_tiles<E4M3>, (unsigned)(whole > args.caps.tile.blocks ? whole : args.caps.tile.blocks), tiles::Shape<E4M3>::THREADS, smem, stream, map_q, map_kv, args);
 }
 
 /* The queries as [rows][heads][128] in boxes of 64 columns, the heads of a group and the rows of a tile. */
@@ -531,12 +533,11 @@ bool query_map(const ncb_paged &a, int rows_per, CUtensorMap *out) {
 
 extern "C" {
 
-int paged_attn_blocks(void) { return tiles::BLOCKS * 148; }
+int paged_attn_blocks(void) { return 148; } /* SMs */
 
 long long paged_attn_workspace_bytes(int requests, long long rows, int max_fresh, int Hq, int Hkv, int blocks) {
     if (Hq <= 0 || Hkv <= 0 || Hq % Hkv || !sizes_ok(requests, rows, max_fresh, Hq / Hkv, Hkv, blocks)) return -1;
-    const Caps c = caps_of(requests, rows, max_fresh, Hq / Hkv, Hkv, blocks);
-    return 4 * workspace_floats(c, Hkv);
+    return 4 * workspace_floats(caps_of(requests, rows, max_fresh, Hq / Hkv, blocks));
 }
 
 int paged_attn(const ncb_paged *args, void *stream) {
@@ -548,10 +549,10 @@ int paged_attn(const ncb_paged *args, void *stream) {
     if (a.rows == 0) return NCB_OK;
     if (!a.q || !a.pool || !a.out || !a.workspace || !a.table || !a.row_start || !a.served || !a.lens || !a.work) return NCB_ERR_ARG;
     if (((uintptr_t)a.q | (uintptr_t)a.pool | (uintptr_t)a.out | (uintptr_t)a.workspace | (uintptr_t)a.work) % 16 || a.ldq % 8 || a.ldo % 8) return NCB_ERR_ALIGN;
-    PagedArgs p = {a, caps_of(a.requests, a.rows, a.max_fresh, a.Hq / a.Hkv, a.Hkv, a.blocks), a.scale * LOG2_E};
+    PagedArgs p = {a, caps_of(a.requests, a.rows, a.max_fresh, a.Hq / a.Hkv, a.blocks), a.scale * LOG2_E};
     if (a.workspace_bytes < paged_attn_workspace_bytes(a.requests, a.rows, a.max_fresh, a.Hq, a.Hkv, a.blocks)) return NCB_ERR_WORKSPACE;
     const long long key_rows = (long long)a.n_pages * a.Hkv * 2 * PAGE_TOKENS;
-    if (key_rows > 0x7fffffffll || p.caps.small.entries * a.Hkv > 0x7fffffffll || p.caps.tile.entries * a.Hkv > 0x7fffffffll) return NCB_ERR_UNSUPPORTED;
+    if (key_rows > 0x7fffffffll || p.caps.tile.owners * a.Hkv > 0x7fffffffll) return NCB_ERR_UNSUPPORTED;
     CUtensorMap map = {}, map_q = {};
     const cudaStream_t s = (cudaStream_t)stream;
     if (p.caps.tiles) {
@@ -565,7 +566,8 @@ int paged_attn(const ncb_paged *args, void *stream) {
         const cudaError_t rc = a.e4m3 ? (one ? small<true, 1>(map, p, s) : small<true, 2>(map, p, s)) : (one ? small<false, 1>(map, p, s) : small<false, 2>(map, p, s));
         if (rc != cudaSuccess) return NCB_ERR_LAUNCH;
     }
-    return launch(k_paged_merge, 4 * 148, 32 * MERGE_WARPS, 0, s, p) == cudaSuccess ? NCB_OK : NCB_ERR_LAUNCH;
+    const int ends = (p.caps.smalls ? p.caps.small.blocks : 0) + (p.caps.tiles ? p.caps.tile.blocks * ((p.caps.tile.slots + MERGE_SLOTS - 1) / MERGE_SLOTS) : 0);
+    return launch(k_paged_merge, ends, 32 * MERGE_WARPS, 0, s, p) == cudaSuccess ? NCB_OK : NCB_ERR_LAUNCH;
 }
 
 } /* extern "C" */

@@ -54,24 +54,42 @@ def attention(q, k, v, first_pos, window):
     return out, size
 
 
-def schedule(words, requests, rows, max_new, group, units):
-    """[(rows an owner has at most, entries, merges, most parts)] of a schedule: the small kernel's, the tile kernel's, where they run."""
+def schedule(words, requests, rows, max_new, group, sms):
+    """[(rows an owner has at most, blocks, overhead, least share, [total, share, whole], owners, starts, pieces)] of a schedule's classes."""
     w = np.asarray(words)
-    few, per = 16 // group, 128 // group
-    each = min(requests, rows)
-    found, at = [], 16
-    small, tile = few > 0, max_new > few
-    if small:
-        merges = 8 * units[0]
-        found.append((0, few, each + (0 if tile else rows // few) + 2 * merges, merges))
-    if tile:
-        found.append((2, per, max(rows // per + min(rows // (few + 1), each), 2 * units[1]), units[1]))
-    out = []
-    for head, limit, entries, merges in found:
-        m = at + 8 * entries
-        out.append((limit, w[at:at + 8 * w[head]].reshape(-1, 8), w[m:m + 4 * w[head + 1]].reshape(-1, 4), 2 * merges))
-        at = m + 4 * merges
-    assert len(w) == -(-at // 4) * 4
-    assert small or not w[:2].any()
-    assert tile or not w[2:4].any()
-    return out
+    few, each = 16 // group, min(requests, rows)
+    classes = []
+    tiles = max_new > few and rows > few
+    if few and rows:
+        classes.append((few, each + (0 if tiles else rows // few), 3 * sms, 2, 6, 0))
+    if tiles:
+        per = 128 // group
+        classes.append((per, rows // per + min(rows // (few + 1), each), 2 * sms, 4, 8, 4 * 2 * sms))
+    found, at = [], 0
+    for per, most, blocks, overhead, least, room in classes:
+        n = int(w[at])
+        assert n <= most
+        owners = w[at + 8:at + 8 + 8 * n].reshape(-1, 8)
+        starts = at + 8 + 8 * most
+        pieces = starts + 4 * ((blocks + 2) // 2 * 2)
+        found.append((per, blocks, overhead, least, w[at + 1:at + 4].tolist(), owners, w[starts:starts + 4 * (blocks + 1)].reshape(-1, 4), w[pieces:pieces + 8 * room].reshape(-1, 8)))
+        at = pieces + 8 * room
+    assert at == len(w)
+    return found
+
+
+def pieces(owners, heads, blocks, overhead, total, share):
+    """What the blocks do with a class that is cut: (block, head, owner, page0, page1, part), and by (head, owner) the blocks whose parts are joined."""
+    done, joined = [], {}
+    for head in range(heads):
+        for i, o in enumerate(owners.tolist()):
+            first = head * total + o[6] + overhead
+            stop = first + max(o[5], 1)
+            b0, b1 = first // share, (stop - 1) // share
+            assert b1 < blocks
+            if b1 > b0:
+                joined[head, i] = [2 * b + (b == b0) for b in range(b0, b1 + 1)]
+            for b in range(b0, b1 + 1):
+                x, y = max(b * share, first), min((b + 1) * share, stop)
+                done.append((b, head, i, x - first, min(y - first, o[5]), -1 if b0 == b1 else 2 * b + (x == first)))
+    return done, joined
