@@ -17,7 +17,7 @@
 namespace {
 namespace paged {
 
-constexpr int SMALL_SLOTS = 16, TILE_SLOTS = 128; /* query slots of a block of the small kernel, of the tile kernel */
+constexpr int SMALL_SLOTS = 16, TILE_SLOTS = 256; /* query slots of a block of the small kernel, of the tile kernel (two tiles of 128) */
 constexpr int MAX_GROUP = 64;                     /* query heads per key/value head */
 constexpr int HEADER_WORDS = 8;                   /* owners, total, share, whole: of a class */
 constexpr int OWNER_WORDS = 8, START_WORDS = 4, PIECE_WORDS = 8;
@@ -54,7 +54,7 @@ struct Caps {
     Class small, tile;
     int smalls, tiles; /* whether the kernel has anything. Without tiles the small kernel also has what is too long and only gets zeros. */
 };
-/* `blocks`: SMs; three blocks of the small kernel run on each, two of the tile kernel. */
+/* `blocks`: SMs; three blocks of the small kernel run on each, one of the tile kernel. */
 static __host__ __device__ __forceinline__ Caps caps_of(int requests, long long rows, int max_fresh, int group, int blocks) {
     Caps c = {};
     const long long one_each = requests < rows ? requests : rows;
@@ -68,10 +68,10 @@ static __host__ __device__ __forceinline__ Caps caps_of(int requests, long long 
     }
     if (c.tiles) {
         const long long longer = rows / (few + 1); /* requests that have tiles */
-        c.tile.rows_per = TILE_SLOTS / group;
+        c.tile.rows_per = TILE_SLOTS / 2 / group * 2;
         c.tile.slots = (max_fresh < c.tile.rows_per ? max_fresh : c.tile.rows_per) * group;
         c.tile.owners = rows / c.tile.rows_per + (longer < one_each ? longer : one_each);
-        c.tile.blocks = 2 * blocks, c.tile.overhead = 4, c.tile.least = 8;
+        c.tile.blocks = blocks, c.tile.overhead = 4, c.tile.least = 8;
     }
     return c;
 }

@@ -556,7 +556,7 @@ int paged_attn(const ncb_paged *args, void *stream) {
     CUtensorMap map = {}, map_q = {};
     const cudaStream_t s = (cudaStream_t)stream;
     if (p.caps.tiles) {
-        if (!query_map(a, p.caps.tile.rows_per, &map_q)) return NCB_ERR_LAUNCH;
+        if (!query_map(a, p.caps.tile.rows_per / 2, &map_q)) return NCB_ERR_LAUNCH;
         if (!a.e4m3 && !tensor_map(a.pool, (int)key_rows, HEAD_DIM, PAGE_TOKENS, &map)) return NCB_ERR_LAUNCH;
         if ((a.e4m3 ? tile<true>(map_q, map, p, s) : tile<false>(map_q, map, p, s)) != cudaSuccess) return NCB_ERR_LAUNCH;
     }

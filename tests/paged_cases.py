@@ -63,8 +63,8 @@ def schedule(words, requests, rows, max_new, group, sms):
     if few and rows:
         classes.append((few, each + (0 if tiles else rows // few), 3 * sms, 2, 6, 0))
     if tiles:
-        per = 128 // group
-        classes.append((per, rows // per + min(rows // (few + 1), each), 2 * sms, 4, 8, 4 * 2 * sms))
+        per = 128 // group * 2
+        classes.append((per, rows // per + min(rows // (few + 1), each), sms, 4, 8, 4 * sms))
     found, at = [], 0
     for per, most, blocks, overhead, least, room in classes:
         n = int(w[at])
