@@ -516,7 +516,7 @@ template <bool E4M3> cudaError_t tile(const CUtensorMap &map_q, const CUtensorMa
     const cudaError_t rc = cudaFuncSetAttribute(tiles::k_paged_tiles<E4M3>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (rc != cudaSuccess) return rc;
     const long long whole = args.caps.tile.owners * args.p.Hkv; /* blocks where no tile is cut */
-    return launch(tiles::k_paged_tiles<E4M3>, (unsigned)(whole > args.caps.tile.blocks ? whole : args.caps.tile.blocks), tiles::Shape<E4M3>::THREADS, smem, stream, map_q, map_kv, args);
+    return launch(tiles::k_paged_tiles<E4M3>, (unsigned)(whole > args.caps.tile.blocks ? whole : args.caps.tile.blocks), tiles::THREADS, smem, stream, map_q, map_kv, args);
 }
 
 /* The queries as [rows][heads][128] in boxes of 64 columns, the heads of a group and the rows of a tile. */

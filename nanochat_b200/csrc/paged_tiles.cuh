@@ -4,18 +4,18 @@
  * thread, the probabilities back over their scores, O += P V with P as the A operand from there; two S buffers a tile, so that the next page's scores run
  * under this page's softmax, and one tile's MMAs under the other's.
  *   - one block per SM with both tiles, which share the pages in its ring: what brings a page there (TMA, or widening it) is done once for 256 slots. Each tile
- *     has softmax warps and a warp that issues its MMAs, which go at their own pace; a page's place is free when both have used it. Few warps with many
- *     registers: a thread holds its row's 64 scores and nothing is spilled (the shared memory leaves L1 no room for that);
+ *     has softmax warps and two that issue its MMAs, which go at their own pace; a page's place is free when both tiles have used it;
  *   - the block walks over the pieces of its part of the line (paged.cuh), the next piece's pages and queries coming under the end of this one;
  *   - the slots of a tile are packed by row and head, so that a chunk of few rows still fills the MMAs and a page is read
  *     once for all heads of its group; queries come as 3-d boxes (64 columns, the group's heads, a tile's rows);
  *   - pages are found through the block table; a page outside the pool is read as zeros and masked;
  *   - runs of pages, windows: rows may see nothing of a page at either end of their range, or nothing at all of a run;
- *   - O is rescaled only when a row's maximum has grown by more than 2^7 since the last time (the sum and O share the reference, so this is exact);
+ *   - probabilities are relative to a reference that need not be the maximum (the sum and O share it, so this is exact): a page's maximum is looked for only where a
+ *     probability turns out above 2^7, or a row has seen nothing yet; then the reference is raised, O rescaled and the page done again;
  *   - bf16 pages: a probability enters P V as one bf16 term, at most 2^-9 of it away: the tensor cores would need 512 cycles a page and tile in place of
  *     256 for two terms;
- *   - e4m3 pages: five warps widen a page to f16 in shared memory (keys in the form of a TMA box, values transposed as they lie), in place of a launch that
- *     widens a request's pages into a workspace of twice the pool's size. Queries are made f16 once per piece, each row times a power of two.
+ *   - e4m3 pages: four warps widen every fourth page each to f16 in shared memory (keys in the form of a TMA box, values transposed as they lie), in place
+ *     of a launch that widens a request's pages into a workspace of twice the pool's size. Queries are made f16 once per piece, each row times a power of two.
  * A position that a row does not see must not reach it: scores are masked, values are looked at in the pages that the border of some row crosses (three
  * at either end at most), and a page that holds one that is not finite there is multiplied row by row over the positions seen.
  */
@@ -30,17 +30,20 @@ namespace tiles {
 using namespace paged;
 using att::arrive;
 
-constexpr int ROWS = att::ROWS, KEYS = PAGE_TOKENS, TILE_WARPS = 4, COPY_WARP = 2 * TILE_WARPS, MMA_WARP = COPY_WARP + 1, WIDEN_WARP = MMA_WARP + 2;
+constexpr int ROWS = att::ROWS, KEYS = PAGE_TOKENS, TILE_WARPS = 4, SCORE_WARP = 2 * TILE_WARPS, VALUE_WARP = SCORE_WARP + 2, PAGE_WARP = VALUE_WARP + 2, PAGE_WARPS = 4;
+constexpr int THREADS = 32 * (PAGE_WARP + PAGE_WARPS); /* four warps to a scheduler: 128 registers a thread */
 constexpr float P_SCALE = 256.f, MIN_LOG2_VSCALE = -64.f;
-constexpr int MOST_ODD = 8;
+constexpr int MOST_ODD = 8, HALF = KEYS / 2;
+constexpr float C0 = 0.99992806f, C1 = 0.69326097f, C2 = 0.24261113f, C3 = 0.055171654f;
+constexpr float LARGE = 128.f; /* how far a probability (bf16: the sum of a page's) may be above 1 before its row's reference is raised */
 constexpr int TILE_COLUMNS = 256, AT_O = 2 * KEYS; /* tensor memory of a tile: S at 0 and 64, O at 128 */
 
 template <bool E4M3> struct Shape {
-    static constexpr int WIDEN_WARPS = E4M3 ? 5 : 1, THREADS = 32 * (WIDEN_WARP + WIDEN_WARPS); /* bf16: a warp that idles. 16 or 12 warps: 128 or 168 registers */
     static constexpr int Q_BYTES = 2 * ROWS * 128, K_BYTES = 2 * KEYS * 128, V_BYTES = K_BYTES; /* Q: of a tile */
-    static constexpr int STAGES = E4M3 ? 2 : 4, RAW_STAGES = E4M3 ? 4 : 0;
+    static constexpr int STAGES = E4M3 ? 2 : 4, RAW_STAGES = E4M3 ? PAGE_WARPS : 0; /* raw: a page's bytes, one for each page warp */
+    static_assert(!E4M3 || PAGE_WARPS <= 2 * STAGES, "a page warp's turns at a place are at most two phases apart");
     static constexpr int AT_K = 2 * Q_BYTES, AT_V = AT_K + STAGES * K_BYTES, AT_RAW = AT_V + STAGES * V_BYTES, AT_SCALE = AT_RAW + RAW_STAGES * PAGE_BYTES;
-    static constexpr int SCALE_FLOATS = 3 * KEYS, AT_FACTOR = AT_SCALE + (E4M3 ? STAGES * SCALE_FLOATS * 4 : 0), AT_BARS = AT_FACTOR + (E4M3 ? 2 * ROWS * 4 : 0);
+    static constexpr int SCALE_FLOATS = 3 * KEYS, AT_BARS = AT_SCALE + (E4M3 ? STAGES * SCALE_FLOATS * 4 : 0);
     static constexpr int SMEM = 1024 + AT_BARS + 1024;
     static_assert(SMEM <= 227 * 1024, "one block per SM");
 };
@@ -48,6 +51,26 @@ template <bool E4M3> struct Shape {
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap *map, int c0, int c1, int c2, uint32_t bar) {
     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
                  ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2) : "memory");
+}
+/* 2^x of two values without the special-function unit: x' = sat((x + 125) / 250) keeps x in [-125, 125], x = n + f with n the nearest whole number (left in the
+ * low bits of a sum with 1.5 * 2^23), 2^f by a cubic with least relative error on [-1/2, 1/2] (7.5e-5, a twentieth of what rounding to bf16 may
+ * take), n added to its exponent. */
+__device__ __forceinline__ void ex2_by_cubic(float &x, float &y, float score_x, float score_y, float slope, float offset) {
+    float a, b;
+    asm("fma.rn.sat.f32 %0, %1, %2, %3;" : "=f"(a) : "f"(score_x), "f"(slope), "f"(offset));
+    asm("fma.rn.sat.f32 %0, %1, %2, %3;" : "=f"(b) : "f"(score_y), "f"(slope), "f"(offset));
+    auto twice = [](float v) { return att::pair_of(v, v); };
+    constexpr float MAGIC = 12582912.f - 125.f;
+    float t0, t1, f0, f1;
+    const uint64_t ab = att::pair_of(a, b);
+    att::fma2(t0, t1, ab, twice(250.f), twice(MAGIC));
+    att::fma2(f0, f1, att::pair_of(t0, t1), twice(-1.f), twice(MAGIC));
+    att::fma2(f0, f1, ab, twice(250.f), att::pair_of(f0, f1));
+    const uint64_t f = att::pair_of(f0, f1);
+    att::fma2(x, y, f, twice(C3), twice(C2));
+    att::fma2(x, y, att::pair_of(x, y), f, twice(C1));
+    att::fma2(x, y, att::pair_of(x, y), f, twice(C0));
+    x = __int_as_float(__float_as_int(x) + (__float_as_int(t0) << 23)), y = __int_as_float(__float_as_int(y) + (__float_as_int(t1) << 23));
 }
 __device__ __forceinline__ float log2_of(float x) {
     float y;
@@ -57,21 +80,6 @@ __device__ __forceinline__ float log2_of(float x) {
 __device__ __forceinline__ uint32_t f16_pair(float x, float y) {
     const __half2 h = __floats2half2_rn(x, y);
     return *reinterpret_cast<const uint32_t *>(&h);
-}
-
-/* 64 consecutive columns of this thread's lane. One statement with its wait: nothing may use the registers in between. */
-__device__ __forceinline__ void tmem_load64(uint32_t taddr, float *v) {
-    uint32_t r[64];
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x64.b32 {"
-                 "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, "
-                 "%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, %48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, "
-                 "%62, %63}, [%64];\n\t"
-                 "tcgen05.wait::ld.sync.aligned;"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]), "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]), "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]), "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]), "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
-                 : "r"(taddr)
-                 : "memory");
-#pragma unroll
-    for (int i = 0; i < 64; i++) v[i] = __uint_as_float(r[i]);
 }
 
 /* What the MMAs of a page do, by a warp: each thread its row's probabilities (from tensor memory, as the MMA would read them) times the values of
@@ -125,7 +133,7 @@ __device__ __forceinline__ float query_row_to_f16(uint8_t *q, int row) {
     return __uint_as_float((uint32_t)(127 + down) << 23);
 }
 
-template <bool E4M3> __global__ void __launch_bounds__(Shape<E4M3>::THREADS, 1) k_paged_tiles(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_kv,
+template <bool E4M3> __global__ void __launch_bounds__(THREADS, 1) k_paged_tiles(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_kv,
                                                                                             const PagedArgs args) {
     using S = Shape<E4M3>;
     constexpr int STAGES = S::STAGES, RAW = E4M3 ? S::RAW_STAGES : 1;
@@ -142,27 +150,23 @@ template <bool E4M3> __global__ void __launch_bounds__(Shape<E4M3>::THREADS, 1) 
     auto v_full = [&](int k) { return bars + 64u + 8u * (k % STAGES); };
     auto v_free = [&](int k) { return bars + 96u + 8u * (k % STAGES); };
     auto raw_full = [&](int k) { return bars + 128u + 8u * (k % RAW); };
-    auto raw_free = [&](int k) { return bars + 160u + 8u * (k % RAW); };
-    const uint32_t q_full = bars + 192u, q_ready = bars + 200u, q_free = bars + 208u;
-    auto of_tile = [&](int x, int i) { return bars + 216u + 64u * x + 8u * i; };
+    auto of_tile = [&](int x, int i) { return bars + 160u + 80u * x + 8u * i; };
     auto s_full = [&](int x, int c) { return of_tile(x, c & 1); };
     auto p_ready = [&](int x, int c) { return of_tile(x, 2 + (c & 1)); };
     auto pv_done = [&](int x, int c) { return of_tile(x, 4 + (c & 1)); };
     auto looked = [&](int x) { return of_tile(x, 6); };
     auto o_free = [&](int x) { return of_tile(x, 7); };
+    auto q_full = [&](int x) { return of_tile(x, 8); };
+    auto q_ready = [&](int x) { return of_tile(x, 9); }; /* E4M3: f16 */
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
         for (int s = 0; s < 4; s++) {
-            mbar_init(bars + 8u * s, E4M3 ? S::WIDEN_WARPS : 1);
+            mbar_init(bars + 8u * s, 1);
             mbar_init(bars + 32u + 8u * s, 2);
-            mbar_init(bars + 64u + 8u * s, E4M3 ? S::WIDEN_WARPS : 1);
+            mbar_init(bars + 64u + 8u * s, 1);
             mbar_init(bars + 96u + 8u * s, 2);
             mbar_init(bars + 128u + 8u * s, 1);
-            mbar_init(bars + 160u + 8u * s, S::WIDEN_WARPS);
         }
-        mbar_init(q_full, 1);
-        mbar_init(q_ready, S::WIDEN_WARPS);
-        mbar_init(q_free, E4M3 ? 2 + 2 * TILE_WARPS : 2);
         for (int x = 0; x < 2; x++) {
             for (int c = 0; c < 2; c++) {
                 mbar_init(s_full(x, c), 1);
@@ -171,6 +175,8 @@ template <bool E4M3> __global__ void __launch_bounds__(Shape<E4M3>::THREADS, 1) 
             }
             mbar_init(looked(x), TILE_WARPS);
             mbar_init(o_free(x), TILE_WARPS);
+            mbar_init(q_full(x), 1);
+            mbar_init(q_ready(x), TILE_WARPS);
         }
         *failed = 0;
         for (int i = 0; i < 2 * MOST_ODD; i++) odd_of[i] = 0;
@@ -193,7 +199,7 @@ template <bool E4M3> __global__ void __launch_bounds__(Shape<E4M3>::THREADS, 1) 
         }
     }
     if (piece >= pieces) return; /* nothing to do, before any tensor memory is taken */
-    if (warp == MMA_WARP) {
+    if (warp == SCORE_WARP) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_slot)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -210,12 +216,13 @@ template <bool E4M3> __global__ void __launch_bounds__(Shape<E4M3>::THREADS, 1) 
         return false;
     };
     auto wait_all = [&](uint32_t bar, int use) { return (bool)__all_sync(0xffffffffu, wait(bar, use)); }; /* a warp */
-    auto load_piece = [&] {
+    auto piece_at = [&](int piece) {
         const int *w = a.work + class_at(args.caps, 1);
         if (!whole) return reinterpret_cast<const Piece *>(w + pieces_at(args.caps.tile))[piece];
         const Owner o = reinterpret_cast<const Owner *>(w + HEADER_WORDS)[piece];
         return Piece{o.request, o.row, o.rows, o.pos, o.page0, o.pages, (int)blockIdx.x % a.Hkv, -1};
     };
+    auto load_piece = [&] { return piece_at(piece); };
     auto begin_of = [&](int pos) { return a.window > 0 ? max(0, pos + 1 - a.window) : 0; };
     /* What tile x has of a piece: its rows and its first row's position; the pages that some row of it sees, from the piece's first; the border of some row's range
      * lies in the pages before lo and in those from hi on. */
@@ -232,31 +239,20 @@ template <bool E4M3> __global__ void __launch_bounds__(Shape<E4M3>::THREADS, 1) 
     };
     bool ok = true;
 
-    if (warp == COPY_WARP) {
-        if (lane == 0) {
-            const uint64_t keep = policy_evict_last();
-            int k = 0, v = 0, q = 0; /* copies begun */
-            for (; ok && piece < pieces; piece++) {
-                const Piece e = load_piece();
-                if (e.pages == 0) continue;
-                const int *table = a.table + (size_t)e.request * a.width + e.page0;
-                int page = table[0];
-                const int tiles = e.rows > rows_per ? 2 : 1, group = a.Hq / a.Hkv;
-                if (q > 0 && !(ok = wait(q_free, q - 1))) break;
-                mbar_expect_tx(q_full, tiles * 2 * rows_per * group * 128); /* a box is whole, whatever the tile uses of it */
-                for (int x = 0; x < tiles; x++)
-                    for (int j = 0; j < 2; j++) tma_load_3d(base + x * S::Q_BYTES + j * ROWS * 128, &map_q, 64 * j, e.head * group, e.row + x * rows_per, q_full);
-                q++;
-                for (int i = 0; i < e.pages; i++) {
-                    const int next = i + 1 < e.pages ? table[i + 1] : 0;
-                    const bool in = (unsigned)page < (unsigned)a.n_pages;
-                    if (!in) flag(a.status, NCB_DEV_BAD_PAGE);
-                    if (E4M3) {
-                        if (k >= RAW && !(ok = wait(raw_free(k), k / RAW - 1))) break;
-                        mbar_expect_tx(raw_full(k), PAGE_BYTES); /* outside the pool: page 0, masked and widened to zeros */
-                        bulk_load(base + S::AT_RAW + k % RAW * PAGE_BYTES, (const uint8_t *)a.pool + ((size_t)(in ? page : 0) * a.Hkv + e.head) * PAGE_BYTES, PAGE_BYTES, raw_full(k));
-                        k++;
-                    } else { /* outside the pool: a box behind its end, zeros */
+    if (warp >= PAGE_WARP) {
+        if (!E4M3) {
+            if (warp == PAGE_WARP && lane == 0) { /* copies keys and values */
+                const uint64_t keep = policy_evict_last();
+                int k = 0, v = 0; /* copies begun */
+                for (; ok && piece < pieces; piece++) {
+                    const Piece e = load_piece();
+                    const int *table = a.table + (size_t)e.request * a.width + e.page0;
+                    int page = e.pages > 0 ? table[0] : 0;
+                    for (int i = 0; i < e.pages; i++) {
+                        const int next = i + 1 < e.pages ? table[i + 1] : 0;
+                        const bool in = (unsigned)page < (unsigned)a.n_pages;
+                        if (!in) flag(a.status, NCB_DEV_BAD_PAGE);
+                        /* outside the pool: a box behind its end, zeros */
                         const int row = in ? (page * a.Hkv + e.head) * 2 * KEYS : a.n_pages * a.Hkv * 2 * KEYS, st = k % STAGES;
                         if (k >= STAGES && !(ok = wait(k_free(k), k / STAGES - 1))) break;
                         mbar_expect_tx(k_full(k), S::K_BYTES);
@@ -266,169 +262,195 @@ template <bool E4M3> __global__ void __launch_bounds__(Shape<E4M3>::THREADS, 1) 
                         mbar_expect_tx(v_full(v), S::V_BYTES);
                         for (int j = 0; j < 2; j++) tma_load(base + S::AT_V + st * S::V_BYTES + j * KEYS * 128, &map_kv, 64 * j, row + KEYS, v_full(v), keep);
                         v++;
+                        page = next;
                     }
-                    page = next;
+                }
+                if (*failed) { /* the block must not leave under copies still in flight */
+                    for (int i = max(0, k - STAGES); i < k; i++) mbar_wait(k_full(i), i / STAGES & 1);
+                    for (int i = max(0, v - STAGES); i < v; i++) mbar_wait(v_full(i), i / STAGES & 1);
                 }
             }
-            if (*failed) { /* the block must not leave under copies still in flight */
-                if (q > 0) mbar_wait(q_full, (q - 1) & 1);
-                const int stages = E4M3 ? RAW : STAGES;
-                for (int i = max(0, k - stages); i < k; i++) mbar_wait(E4M3 ? raw_full(i) : k_full(i), i / stages & 1);
-                for (int i = max(0, v - stages); i < v; i++) mbar_wait(v_full(i), i / stages & 1);
+        } else { /* every fourth page is this warp's: it fetches it, and widens it */
+            const int y = warp - PAGE_WARP;
+            int fetch_piece = piece, fetch_at = y, fetch_pages = -1, fetched = 0; /* the next page to fetch: its piece, its number there, and the block's pages before */
+            long long fetch_table = 0;
+            int fetch_head = 0;
+            auto fetch = [&] { /* false: there is none */
+                while (fetch_pages < 0 || fetch_at >= fetch_pages) {
+                    if (fetch_pages >= 0) fetch_at -= fetch_pages, fetch_piece++;
+                    if (fetch_piece >= pieces) return false;
+                    const Piece e = piece_at(fetch_piece);
+                    fetch_pages = e.pages, fetch_head = e.head, fetch_table = (long long)e.request * a.width + e.page0;
+                }
+                const int page = a.table[fetch_table + fetch_at], at = y;
+                const bool in = (unsigned)page < (unsigned)a.n_pages;
+                if (lane == 0) {
+                    if (!in) flag(a.status, NCB_DEV_BAD_PAGE);
+                    mbar_expect_tx(raw_full(at), PAGE_BYTES); /* outside the pool: page 0, masked and widened to zeros */
+                    bulk_load(base + S::AT_RAW + at * PAGE_BYTES, (const uint8_t *)a.pool + ((size_t)(in ? page : 0) * a.Hkv + fetch_head) * PAGE_BYTES, PAGE_BYTES, raw_full(at));
+                }
+                fetched++, fetch_at += PAGE_WARPS;
+                return true;
+            };
+            fetch();
+            int k = 0; /* the block's pages before the piece */
+            for (; ok && piece < pieces; piece++) {
+                const Piece e = load_piece();
+                const int *table = a.table + (size_t)e.request * a.width + e.page0;
+                for (int i = (y - k) & PAGE_WARPS - 1; i < e.pages; i += PAGE_WARPS) {
+                    const int ki = k + i;
+                    const uint8_t *page = raw + S::AT_RAW + ki % RAW * PAGE_BYTES;
+                    const bool in = (unsigned)table[i] < (unsigned)a.n_pages;
+                    /* a place's barriers are waited for phase by phase: first for the page before in that place, which another warp has put there */
+                    ok = wait_all(raw_full(ki), ki / RAW) && (ki < STAGES || (wait_all(k_full(ki), ki / STAGES - 1) && wait_all(k_free(ki), ki / STAGES - 1)));
+                    if (!ok) break;
+                    uint8_t *keys = raw + S::AT_K + ki % STAGES * S::K_BYTES;
+#pragma unroll 1
+                    for (int h = 0; h < 16; h += 8) {
+                        uint4 in4[8];
+#pragma unroll
+                        for (int n = 0; n < 8; n++) in4[n] = *reinterpret_cast<const uint4 *>(page + page_k_chunk(4 * (h + n) + (lane >> 3), lane & 7)); /* 16 codes of a key */
+#pragma unroll
+                        for (int n = 0; n < 8; n++) { /* -> 32 bytes: two chunks of a swizzled row */
+                            const int j = 4 * (h + n) + (lane >> 3), c = lane & 7;
+                            uint4 w[2];
+                            widen_e4m3x4(in4[n].x, w[0].x, w[0].y), widen_e4m3x4(in4[n].y, w[0].z, w[0].w);
+                            widen_e4m3x4(in4[n].z, w[1].x, w[1].y), widen_e4m3x4(in4[n].w, w[1].z, w[1].w);
+                            uint8_t *row = keys + (c >> 2) * KEYS * 128 + j * 128;
+                            const uint32_t chunk = ((2 * c & 7) ^ (j & 7)) << 4;
+                            *reinterpret_cast<uint4 *>(row + chunk) = w[0];
+                            *reinterpret_cast<uint4 *>(row + (chunk ^ 16)) = w[1];
+                        }
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) arrive(k_full(ki));
+                    if (ki >= STAGES && !(ok = wait_all(v_full(ki), ki / STAGES - 1) && wait_all(v_free(ki), ki / STAGES - 1))) break;
+                    uint8_t *values = raw + S::AT_V + ki % STAGES * S::V_BYTES;
+                    float *scales = reinterpret_cast<float *>(raw + S::AT_SCALE) + ki % STAGES * S::SCALE_FLOATS;
+#pragma unroll
+                    for (int j = lane; j < KEYS; j += 32) { /* score factor, log2 of the value's scale, its scale */
+                        const float vs = in ? reinterpret_cast<const float *>(page + PAGE_VS)[j] : 0.f;
+                        scales[j] = in ? reinterpret_cast<const float *>(page + PAGE_KS)[j] : 0.f;
+                        scales[KEYS + j] = fmaxf(log2_of(vs), MIN_LOG2_VSCALE);
+                        scales[2 * KEYS + j] = vs * P_SCALE;
+                    }
+                    const int used = in ? e.pos + e.rows - (e.page0 + i) * KEYS : 0; /* positions past the last row may hold anything: zeros */
+#pragma unroll 1
+                    for (int h = 0; h < 4; h += 2) { /* 16 positions of a dimension: four groups of 16, four times 32 dimensions */
+                        uint4 in4[8];
+#pragma unroll
+                        for (int n = 0; n < 8; n++) in4[n] = *reinterpret_cast<const uint4 *>(page + PAGE_V + (h + n / 4) * 2048 + (n % 4 * 32 + lane) * 16);
+                        if (used < KEYS) {
+#pragma unroll
+                            for (int n = 0; n < 8; n++)
+#pragma unroll
+                                for (int w = 0; w < 4; w++) {
+                                    const int on = used - 16 * (h + n / 4) - 4 * w;
+                                    (&in4[n].x)[w] = on >= 4 ? (&in4[n].x)[w] : on <= 0 ? 0u : (&in4[n].x)[w] & ((1u << (8 * on)) - 1u);
+                                }
+                        }
+#pragma unroll
+                        for (int n = 0; n < 8; n++) {
+                            uint4 w[2];
+                            widen_e4m3x4(in4[n].x, w[0].x, w[0].y), widen_e4m3x4(in4[n].y, w[0].z, w[0].w);
+                            widen_e4m3x4(in4[n].z, w[1].x, w[1].y), widen_e4m3x4(in4[n].w, w[1].z, w[1].w);
+                            uint8_t *row = values + (n % 4 * 32 + lane) * 128;
+                            const uint32_t chunk = (2 * (h + n / 4) ^ (lane & 7)) << 4;
+                            *reinterpret_cast<uint4 *>(row + chunk) = w[0];
+                            *reinterpret_cast<uint4 *>(row + (chunk ^ 16)) = w[1];
+                        }
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) arrive(v_full(ki));
+                    fetch(); /* into the place of this page, which the warp has read */
+                }
+                k += e.pages;
             }
+            if (*failed && lane == 0) /* the block must not leave under copies still in flight */
+                if (fetched > 0) mbar_wait(raw_full(y), (fetched - 1) & 1);
         }
-    } else if (warp == MMA_WARP || warp == MMA_WARP + 1) { /* a tile's MMAs: the warp goes through the loop together (elect_one) */
+    } else if (warp >= SCORE_WARP) { /* a tile's MMAs, scores and values each by a warp of their own (issuing them and the waits between take longer than the tensor
+                                        * cores need); it goes through the loop together (elect_one) */
         constexpr uint32_t F32 = 1u << 4, BF16_AB = E4M3 ? 0u : (1u << 7) | (1u << 10), M = (uint32_t)(ROWS >> 4) << 24;
         constexpr uint32_t score = F32 | BF16_AB | M | ((uint32_t)(KEYS >> 3) << 17);
         constexpr uint32_t value = F32 | BF16_AB | M | ((uint32_t)(HEAD_DIM >> 3) << 17) | (E4M3 ? 0u : 1u << 16);
-        const int x = __shfl_sync(0xffffffffu, warp - MMA_WARP, 0);
+        const int x = __shfl_sync(0xffffffffu, (warp - SCORE_WARP) & 1, 0);
         const uint32_t t = __shfl_sync(0xffffffffu, tmem, 0) + x * TILE_COLUMNS, b = __shfl_sync(0xffffffffu, base, 0);
-        int k = 0, c = 0, q = 0, used = 0, borders = 0; /* pages, pages of the tile, pieces, pieces that the tile had pages of, pages that its border crossed */
+        int k = 0, c = 0, used = 0, borders = 0; /* pages, pages of the tile, pieces that the tile had pages of, pages that its border crossed */
         for (; ok && piece < pieces; piece++) {
             const Piece e = load_piece();
             if (e.pages == 0) continue;
             const Tile tile = tile_of(e, x);
-            auto scores = [&](int i) { /* of the piece's page i; where the tile has no part in it the page only passes */
-                if (!wait_all(k_full(k + i), (k + i) / STAGES)) return false;
-                if (i >= tile.pages) {
-                    if (lane == 0) arrive(k_free(k + i));
-                    return true;
-                }
-                const int ci = c + i;
-                if (ci >= 2 && !wait_all(pv_done(x, ci), (ci - 2) >> 1)) return false; /* the buffer's probabilities have been used */
-                att::fence_after();
-                const uint32_t ks = b + S::AT_K + (k + i) % STAGES * S::K_BYTES, qs = b + x * S::Q_BYTES, d = t + (ci & 1) * KEYS;
-                if (elect_one()) {
-#pragma unroll
-                    for (int j = 0; j < 2; j++)
-#pragma unroll
-                        for (int h = 0; h < 4; h++)
-                            umma_bf16(d, umma_desc(qs + j * ROWS * 128 + h * 32), umma_desc(ks + j * KEYS * 128 + h * 32), score, (j | h) != 0);
-                    umma_commit(s_full(x, ci));
-                    umma_commit(k_free(k + i));
-                    if (i + 1 == tile.pages) umma_commit(q_free); /* the queries have been read for the last time */
-                }
-                __syncwarp();
-                return true;
-            };
-            ok = wait_all(E4M3 ? q_ready : q_full, q);
-            if (ok && tile.pages == 0 && lane == 0) arrive(q_free);
-            ok = ok && scores(0);
-            for (int i = 0; ok && i < e.pages; i++) {
-                ok = (i + 1 == e.pages || scores(i + 1)) && wait_all(v_full(k + i), (k + i) / STAGES);
-                if (!ok) break;
-                if (i >= tile.pages) {
-                    if (lane == 0) arrive(v_free(k + i));
-                    continue;
-                }
-                const int ci = c + i;
-                ok = wait_all(p_ready(x, ci), ci >> 1) && (i > 0 || used == 0 || wait_all(o_free(x), used - 1));
-                if (!ok) break;
-                att::fence_after();
-                const uint32_t vs = b + S::AT_V + (k + i) % STAGES * S::V_BYTES, p = t + (ci & 1) * KEYS;
-                bool by_mma = true;
-                if (i < tile.lo || i >= tile.hi) by_mma = odd_of[x * MOST_ODD + borders % MOST_ODD] != borders + 1, borders++;
-                if (elect_one()) {
-                    if (by_mma) {
-#pragma unroll
-                        for (int h = 0; h < KEYS / 16; h++) /* 16 keys: 8 columns of packed probabilities */
-                            att::umma_from_tmem(t + AT_O, p + h * 8, E4M3 ? umma_desc(vs + h * 32) : att::desc_by_rows(vs + h * 2048, KEYS * 128), value, (i | h) != 0);
+            if (warp < VALUE_WARP) {
+                if (tile.pages > 0) { /* its queries, when the products of the piece before have read theirs */
+                    if (used > 0 && !(ok = wait_all(s_full(x, c - 1), (c - 1) >> 1))) break;
+                    if (elect_one()) {
+                        const int group = a.Hq / a.Hkv;
+                        mbar_expect_tx(q_full(x), 2 * rows_per * group * 128); /* a box is whole, whatever the tile uses of it */
+                        for (int j = 0; j < 2; j++) tma_load_3d(b + x * S::Q_BYTES + j * ROWS * 128, &map_q, 64 * j, e.head * group, e.row + x * rows_per, q_full(x));
                     }
-                    umma_commit(pv_done(x, ci));
-                    umma_commit(v_free(k + i));
+                    __syncwarp();
+                    if (!(ok = wait_all(E4M3 ? q_ready(x) : q_full(x), used))) break;
                 }
-                __syncwarp();
-            }
-            k += e.pages, c += tile.pages, q++, used += tile.pages > 0;
-        }
-    } else if (warp >= WIDEN_WARP) {
-        if (E4M3) {
-            constexpr int T = 32 * S::WIDEN_WARPS, ROUNDS = (512 + T - 1) / T;
-            const int t = tid - 32 * WIDEN_WARP;
-            int k = 0, q = 0;
-            for (; ok && piece < pieces; piece++) {
-                const Piece e = load_piece();
-                if (e.pages == 0) continue;
-                const int *table = a.table + (size_t)e.request * a.width + e.page0;
-                int page_at = table[0];
-                if (!(ok = wait_all(q_full, q))) break;
-                for (int r = t; r < (e.rows > rows_per ? 2 : 1) * ROWS; r += T)
-                    reinterpret_cast<float *>(raw + S::AT_FACTOR)[r] = query_row_to_f16(raw + r / ROWS * S::Q_BYTES, r % ROWS);
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                __syncwarp();
-                if (lane == 0) arrive(q_ready);
-                q++;
-                for (int i = 0; i < e.pages; i++, k++) {
-                    const uint8_t *page = raw + S::AT_RAW + k % RAW * PAGE_BYTES;
-                    const bool in = (unsigned)page_at < (unsigned)a.n_pages;
-                    page_at = i + 1 < e.pages ? table[i + 1] : 0;
-                    ok = wait_all(raw_full(k), k / RAW);
+                for (int i = 0; ok && i < e.pages; i++, k++) {
+                    ok = wait_all(k_full(k), k / STAGES);
                     if (!ok) break;
-                    uint4 in4[ROUNDS];
-#pragma unroll
-                    for (int y = 0; y < ROUNDS; y++) /* 16 codes of a key */
-                        if (t + T * y < 512) in4[y] = *reinterpret_cast<const uint4 *>(page + page_k_chunk((t + T * y) >> 3, (t + T * y) & 7));
-                    if (k >= STAGES && !(ok = wait_all(k_free(k), k / STAGES - 1))) break;
-                    uint8_t *keys = raw + S::AT_K + k % STAGES * S::K_BYTES;
-#pragma unroll
-                    for (int y = 0; y < ROUNDS; y++) { /* -> 32 bytes: two chunks of a swizzled row */
-                        const int at = t + T * y, j = at >> 3, c = at & 7;
-                        if (at >= 512) break;
-                        uint4 w[2];
-                        widen_e4m3x4(in4[y].x, w[0].x, w[0].y), widen_e4m3x4(in4[y].y, w[0].z, w[0].w);
-                        widen_e4m3x4(in4[y].z, w[1].x, w[1].y), widen_e4m3x4(in4[y].w, w[1].z, w[1].w);
-                        uint8_t *row = keys + (c >> 2) * KEYS * 128 + j * 128;
-                        const uint32_t chunk = ((2 * c & 7) ^ (j & 7)) << 4;
-                        *reinterpret_cast<uint4 *>(row + chunk) = w[0];
-                        *reinterpret_cast<uint4 *>(row + (chunk ^ 16)) = w[1];
+                    if (i >= tile.pages) { /* the tile has no part in the page, which only passes */
+                        if (lane == 0) arrive(k_free(k));
+                        continue;
                     }
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    const int ci = c + i;
+                    ok = ci < 2 || wait_all(pv_done(x, ci), (ci - 2) >> 1); /* the buffer's probabilities have been used */
+                    if (!ok) break;
+                    att::fence_after();
+                    const uint32_t ks = b + S::AT_K + k % STAGES * S::K_BYTES, qs = b + x * S::Q_BYTES, d = t + (ci & 1) * KEYS;
+                    if (elect_one()) {
+#pragma unroll
+                        for (int j = 0; j < 2; j++)
+#pragma unroll
+                            for (int h = 0; h < 4; h++)
+                                umma_bf16(d, umma_desc(qs + j * ROWS * 128 + h * 32), umma_desc(ks + j * KEYS * 128 + h * 32), score, (j | h) != 0);
+                        umma_commit(s_full(x, ci));
+                        umma_commit(k_free(k));
+                    }
                     __syncwarp();
-                    if (lane == 0) arrive(k_full(k));
-#pragma unroll
-                    for (int y = 0; y < ROUNDS; y++) /* 16 positions of a dimension */
-                        if (t + T * y < 512) in4[y] = *reinterpret_cast<const uint4 *>(page + PAGE_V + (t + T * y) / 128 * 2048 + (t + T * y) % 128 * 16);
-                    const int used = in ? e.pos + e.rows - (e.page0 + i) * KEYS : 0; /* positions past the last row may hold anything: zeros */
-                    if (used < KEYS) {
-#pragma unroll
-                        for (int y = 0; y < ROUNDS; y++)
-#pragma unroll
-                            for (int w = 0; w < 4; w++) {
-                                const int on = used - 16 * ((t + T * y) / 128) - 4 * w;
-                                (&in4[y].x)[w] = on >= 4 ? (&in4[y].x)[w] : on <= 0 ? 0u : (&in4[y].x)[w] & ((1u << (8 * on)) - 1u);
-                            }
+                }
+            } else {
+                for (int i = 0; ok && i < e.pages; i++, k++) {
+                    ok = wait_all(v_full(k), k / STAGES);
+                    if (!ok) break;
+                    if (i >= tile.pages) {
+                        if (lane == 0) arrive(v_free(k));
+                        continue;
                     }
-                    if (k >= STAGES && !(ok = wait_all(v_free(k), k / STAGES - 1))) break;
-                    uint8_t *values = raw + S::AT_V + k % STAGES * S::V_BYTES;
-                    float *scales = reinterpret_cast<float *>(raw + S::AT_SCALE) + k % STAGES * S::SCALE_FLOATS;
-                    if (t < KEYS) { /* score factor, log2 of the value's scale, its scale */
-                        const float vs = in ? reinterpret_cast<const float *>(page + PAGE_VS)[t] : 0.f;
-                        scales[t] = in ? reinterpret_cast<const float *>(page + PAGE_KS)[t] : 0.f;
-                        scales[KEYS + t] = fmaxf(log2_of(vs), MIN_LOG2_VSCALE);
-                        scales[2 * KEYS + t] = vs * P_SCALE;
-                    }
+                    const int ci = c + i;
+                    ok = (i > 0 || used == 0 || wait_all(o_free(x), used - 1)) && wait_all(p_ready(x, ci), ci >> 1);
+                    if (!ok) break;
+                    att::fence_after();
+                    const uint32_t vs = b + S::AT_V + k % STAGES * S::V_BYTES, p = t + (ci & 1) * KEYS;
+                    bool by_mma = true;
+                    if (i < tile.lo || i >= tile.hi) by_mma = odd_of[x * MOST_ODD + borders % MOST_ODD] != borders + 1, borders++;
+                    if (elect_one()) {
+                        if (by_mma) {
 #pragma unroll
-                    for (int y = 0; y < ROUNDS; y++) {
-                        const int at = t + T * y, d = at & 127;
-                        if (at >= 512) break;
-                        uint4 w[2];
-                        widen_e4m3x4(in4[y].x, w[0].x, w[0].y), widen_e4m3x4(in4[y].y, w[0].z, w[0].w);
-                        widen_e4m3x4(in4[y].z, w[1].x, w[1].y), widen_e4m3x4(in4[y].w, w[1].z, w[1].w);
-                        uint8_t *row = values + d * 128;
-                        const uint32_t chunk = (2 * (at >> 7) ^ (d & 7)) << 4;
-                        *reinterpret_cast<uint4 *>(row + chunk) = w[0];
-                        *reinterpret_cast<uint4 *>(row + (chunk ^ 16)) = w[1];
+                            for (int h = 0; h < KEYS / 16; h++) /* 16 keys: 8 columns of packed probabilities */
+                                att::umma_from_tmem(t + AT_O, p + h * 8, E4M3 ? umma_desc(vs + h * 32) : att::desc_by_rows(vs + h * 2048, KEYS * 128), value, (i | h) != 0);
+                        }
+                        umma_commit(pv_done(x, ci));
+                        umma_commit(v_free(k));
                     }
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     __syncwarp();
-                    if (lane == 0) arrive(v_full(k)), arrive(raw_free(k));
                 }
             }
+            c += tile.pages, used += tile.pages > 0;
         }
+        if (warp < VALUE_WARP && *failed && used > 0) mbar_wait(q_full(x), (used - 1) & 1); /* the block must not leave under a copy still in flight */
     } else { /* softmax: a thread has a slot of its tile */
         const int x = warp / TILE_WARPS, slot = tid % (32 * TILE_WARPS), first = slot & ~31;
         const uint32_t t_mine = tmem + x * TILE_COLUMNS + ((uint32_t)first << 16), o_mine = t_mine + AT_O;
-        int k = 0, c = 0, q = 0, borders = 0;
+        int k = 0, c = 0, used = 0, borders = 0;
         for (; ok && piece < pieces; piece++) {
             const Piece e = load_piece();
             const Tile tile = tile_of(e, x);
@@ -440,20 +462,21 @@ template <bool E4M3> __global__ void __launch_bounds__(Shape<E4M3>::THREADS, 1) 
                     for (int d = 0; d < HEAD_DIM; d += 8) *reinterpret_cast<uint4 *>(out + d) = make_uint4(0u, 0u, 0u, 0u);
                 continue;
             }
-            float factor = args.scale_log2;
-            if (E4M3) {
-                if (!(ok = wait_all(q_ready, q))) break;
-                factor *= reinterpret_cast<const float *>(raw + S::AT_FACTOR)[x * ROWS + slot];
-                __syncwarp();
-                if (lane == 0) arrive(q_free); /* the factors have been read */
-            }
-            q++;
             float *part = (float *)a.workspace + parts_at(args.caps, 1) + ((size_t)max(e.part, 0) * args.caps.tile.slots + x * rows_per * G + slot) * PART;
             if (tile.pages == 0) { /* the tile has no part in this piece: an empty state */
                 if (on && e.part >= 0) part[0] = -INFINITY, part[1] = 0.f;
                 k += e.pages;
                 continue;
             }
+            float factor = args.scale_log2;
+            if (E4M3) { /* the thread's row to f16 */
+                if (!(ok = wait_all(q_full(x), used))) break;
+                factor *= query_row_to_f16(raw + x * S::Q_BYTES, slot);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) arrive(q_ready(x));
+            }
+            used++;
             const int last = tile.pos + mine - e.page0 * KEYS, begin = begin_of(tile.pos + mine) - e.page0 * KEYS; /* what the slot sees, from the piece's first key */
             /* the border of some row of the warp lies in the pages before my_lo and in those from my_hi on */
             const int my_lo = (__shfl_sync(0xffffffffu, begin, 31) + KEYS - 1) / KEYS, my_hi = (__shfl_sync(0xffffffffu, last, 0) + 1) / KEYS;
@@ -462,7 +485,6 @@ template <bool E4M3> __global__ void __launch_bounds__(Shape<E4M3>::THREADS, 1) 
             const uint64_t factor2 = att::pair_of(factor, factor);
             float m = -INFINITY;
             uint64_t sums[2] = {0, 0};
-            bool pending = true; /* some row of the warp may have had no finite score yet */
             int page = table[0];
             for (int i = 0; i < tile.pages; i++) {
                 const bool in = (unsigned)page < (unsigned)a.n_pages;
@@ -476,63 +498,114 @@ template <bool E4M3> __global__ void __launch_bounds__(Shape<E4M3>::THREADS, 1) 
                 const float *scales = reinterpret_cast<const float *>(raw + S::AT_SCALE) + ki % STAGES * S::SCALE_FLOATS;
                 auto scales_at = [&](int j, int which) { return *reinterpret_cast<const ulonglong2 *>(scales + which * KEYS + j); }; /* of four keys from j */
                 const bool border = i < tile.lo || i >= tile.hi;
-                float s[KEYS];
-                float reference = 0.f;
+                const bool plain = i >= my_lo && i < my_hi && in; /* every row of the warp sees the whole page */
                 if (!idle) {
-                    tmem_load64(s_mine, s);
-                    if (E4M3) {
+                    uint32_t packed[KEYS / 2]; /* probabilities */
+                    uint64_t sum[2];
+                    constexpr bool CUBIC = !E4M3;
+                    auto load_scores = [&](int h, float *s) { /* of half the page's keys, those from h on */
+                        tmem_load32(s_mine + h, s);
+                        if (E4M3) {
 #pragma unroll
-                        for (int j = 0; j < KEYS; j += 4) {
-                            const ulonglong2 f = scales_at(j, 0);
-                            att::mul2(s[j], s[j + 1], att::pair_of(s[j], s[j + 1]), f.x);
-                            att::mul2(s[j + 2], s[j + 3], att::pair_of(s[j + 2], s[j + 3]), f.y);
+                            for (int j = 0; j < HALF; j += 4) {
+                                const ulonglong2 f = scales_at(h + j, 0);
+                                att::mul2(s[j], s[j + 1], att::pair_of(s[j], s[j + 1]), f.x);
+                                att::mul2(s[j + 2], s[j + 3], att::pair_of(s[j + 2], s[j + 3]), f.y);
+                            }
                         }
-                    }
-                    if (i < my_lo || i >= my_hi || !in) { /* the border of some row crosses this warp's part of the page */
-                        const int to = in ? last - i * KEYS : -1, from = begin - i * KEYS; /* in the page */
+                        if (!plain) {
+                            const int to = in ? last - i * KEYS - h : -1, from = begin - i * KEYS - h;
 #pragma unroll
-                        for (int j = 0; j < KEYS; j++) s[j] = j > to || j < from ? -INFINITY : s[j];
-                    }
-                    float best[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                    for (int j = 0; j < KEYS; j += 4) {
-                        float y[4] = {s[j], s[j + 1], s[j + 2], s[j + 3]};
-                        if (E4M3) { /* the probabilities carry the value's scale: the maximum is that of score + log2(scale) */
-                            const ulonglong2 f = scales_at(j, 1);
-                            att::fma2(y[0], y[1], att::pair_of(y[0], y[1]), factor2, f.x);
-                            att::fma2(y[2], y[3], att::pair_of(y[2], y[3]), factor2, f.y);
+                            for (int j = 0; j < HALF; j++) s[j] = j > to || j < from ? -INFINITY : s[j];
                         }
-                        best[j / 4 % 2 * 2] = att::max3(best[j / 4 % 2 * 2], y[0], y[1]);
-                        best[j / 4 % 2 * 2 + 1] = att::max3(best[j / 4 % 2 * 2 + 1], y[2], y[3]);
-                    }
-                    float top = fmaxf(att::max3(best[0], best[1], best[2]), best[3]);
-                    if (!E4M3) top *= factor;
-                    if (i == 0) {
-                        m = top;
-                    } else if (__any_sync(0xffffffffu, top > m + att::RESCALE_LOG2)) {
-                        ok = wait_all(pv_done(x, ci - 1), (ci - 1) >> 1); /* O is complete up to the page before */
-                        if (!ok) break;
-                        att::fence_after();
-                        const bool grown = top > m + att::RESCALE_LOG2;
-                        const float f = grown ? (m == -INFINITY ? 0.f : ex2(m - top)) : 1.f;
-                        m = grown ? top : m;
-                        sums[0] = att::mul2(sums[0], att::pair_of(f, f)), sums[1] = att::mul2(sums[1], att::pair_of(f, f));
+                    };
+                    auto probabilities = [&](bool cubic) { /* whether some is large */
+                        const float reference = m == -INFINITY ? 0.f : m; /* where nothing counts yet the scores are -infinity or NaN: nothing, or NaN */
+                        const uint64_t minus = att::pair_of(-reference, -reference);
+                        const float slope = factor * (1.f / 250.f), offset = (125.f - reference) * (1.f / 250.f);
+                        __half2 most = __floats2half2_rn(0.f, 0.f);
+                        sum[0] = sum[1] = 0;
+#pragma unroll
+                        for (int h = 0; h < KEYS; h += HALF) {
+                            float s[HALF];
+                            load_scores(h, s);
+#pragma unroll
+                            for (int j = 0; j < HALF; j += 4) {
+                                ulonglong2 f;
+                                if (E4M3) f = scales_at(h + j, 2);
+#pragma unroll
+                                for (int p = 0; p < 2; p++) {
+                                    float y, z;
+                                    if (cubic && j % 8 == 4 && p == 1) { /* a quarter of them: the special-function unit would need 1,024 cycles a page for both tiles */
+                                        ex2_by_cubic(y, z, s[j + 2], s[j + 3], slope, offset);
+                                    } else {
+                                        att::fma2(y, z, att::pair_of(s[j + 2 * p], s[j + 2 * p + 1]), factor2, minus);
+                                        y = ex2(y), z = ex2(z);
+                                    }
+                                    const uint64_t yz = att::pair_of(y, z);
+                                    sum[p] = att::add2(sum[p], yz);
+                                    if (E4M3) {
+                                        att::mul2(y, z, yz, p ? f.y : f.x);
+                                        const __half2 w = __floats2half2_rn(y, z);
+                                        most = __hmax2_nan(most, w);
+                                        packed[(h + j) / 2 + p] = *reinterpret_cast<const uint32_t *>(&w);
+                                    } else {
+                                        const __nv_bfloat162 w = __floats2bfloat162_rn(y, z);
+                                        packed[(h + j) / 2 + p] = *reinterpret_cast<const uint32_t *>(&w);
+                                    }
+                                }
+                            }
+                        }
+                        if (E4M3) return !(__low2float(most) <= LARGE * P_SCALE && __high2float(most) <= LARGE * P_SCALE);
+                        const uint64_t both = att::add2(sum[0], sum[1]);
+                        return !(__uint_as_float((uint32_t)both) + __uint_as_float((uint32_t)(both >> 32)) <= LARGE);
+                    };
+                    /* Probabilities against the reference that holds, without looking for the page's maximum: only where one (or their sum) turns out above 2^7, or nothing
+                     * holds yet, is it looked for and the page done again, for the rows that need it. */
+                    const bool raise = on & ((CUBIC && plain ? probabilities(true) : probabilities(false)) | (m == -INFINITY));
+                    if (__any_sync(0xffffffffu, raise)) {
+                        float best[2] = {-INFINITY, -INFINITY};
 #pragma unroll 1
-                        for (int d = 0; d < HEAD_DIM; d += 16) {
-                            float y[16];
-                            uint32_t z[16];
-                            att::tmem_load16(o_mine + d, y);
+                        for (int h = 0; h < KEYS; h += HALF) {
+                            float s[HALF];
+                            load_scores(h, s);
 #pragma unroll
-                            for (int j = 0; j < 16; j++) z[j] = __float_as_uint(y[j] * f);
-                            att::tmem_store16(o_mine + d, z);
+                            for (int j = 0; j < HALF; j += 4) {
+                                float y[4] = {s[j], s[j + 1], s[j + 2], s[j + 3]};
+                                if (E4M3) { /* the probabilities carry the value's scale: the maximum is that of score + log2(scale) */
+                                    const ulonglong2 f = scales_at(h + j, 1);
+                                    att::fma2(y[0], y[1], att::pair_of(y[0], y[1]), factor2, f.x);
+                                    att::fma2(y[2], y[3], att::pair_of(y[2], y[3]), factor2, f.y);
+                                }
+                                best[0] = att::max3(best[0], y[0], y[1]);
+                                best[1] = att::max3(best[1], y[2], y[3]);
+                            }
                         }
+                        float top = fmaxf(best[0], best[1]);
+                        if (!E4M3) top *= factor;
+                        const bool grown = raise && top > m;
+                        if (i > 0 && __any_sync(0xffffffffu, grown)) {
+                            ok = wait_all(pv_done(x, ci - 1), (ci - 1) >> 1); /* O is complete up to the page before */
+                            if (!ok) break;
+                            att::fence_after();
+                            const float f = !grown ? 1.f : m == -INFINITY ? 0.f : ex2(m - top);
+                            sums[0] = att::mul2(sums[0], att::pair_of(f, f)), sums[1] = att::mul2(sums[1], att::pair_of(f, f));
+#pragma unroll 1
+                            for (int d = 0; d < HEAD_DIM; d += 16) {
+                                float y[16];
+                                uint32_t z[16];
+                                att::tmem_load16(o_mine + d, y);
+#pragma unroll
+                                for (int j = 0; j < 16; j++) z[j] = __float_as_uint(y[j] * f);
+                                att::tmem_store16(o_mine + d, z);
+                            }
+                        }
+                        m = grown ? top : m;
+                        probabilities(false);
                     }
-                    reference = m;
-                    if (pending) {
-                        const bool none = m == -INFINITY;
-                        pending = __any_sync(0xffffffffu, none);
-                        reference = none ? 0.f : m; /* its scores are -infinity or NaN: nothing, or NaN */
-                    }
+                    sums[0] = att::add2(sums[0], sum[0]), sums[1] = att::add2(sums[1], sum[1]);
+                    att::tmem_store16(s_mine, packed);
+                    att::tmem_store16(s_mine + KEYS / 4, packed + KEYS / 4);
                 }
                 if (border) {
                     ok = wait_all(v_full(ki), ki / STAGES);
@@ -553,35 +626,7 @@ template <bool E4M3> __global__ void __launch_bounds__(Shape<E4M3>::THREADS, 1) 
                         arrive(looked(x));
                     }
                 }
-                if (!idle) {
-                    const uint64_t minus = att::pair_of(-reference, -reference);
-#pragma unroll
-                    for (int h = 0; h < KEYS; h += 32) {
-                        uint32_t packed[16];
-#pragma unroll
-                        for (int j = 0; j < 32; j += 4) {
-                            ulonglong2 f;
-                            if (E4M3) f = scales_at(h + j, 2);
-#pragma unroll
-                            for (int p = 0; p < 2; p++) {
-                                float y, z;
-                                att::fma2(y, z, att::pair_of(s[h + j + 2 * p], s[h + j + 2 * p + 1]), factor2, minus);
-                                y = ex2(y), z = ex2(z);
-                                const uint64_t yz = att::pair_of(y, z);
-                                sums[p] = att::add2(sums[p], yz);
-                                if (E4M3) {
-                                    att::mul2(y, z, yz, p ? f.y : f.x);
-                                    packed[j / 2 + p] = f16_pair(y, z);
-                                } else {
-                                    const __nv_bfloat162 w = __floats2bfloat162_rn(y, z);
-                                    packed[j / 2 + p] = *reinterpret_cast<const uint32_t *>(&w);
-                                }
-                            }
-                        }
-                        att::tmem_store16(s_mine + h / 2, packed);
-                    }
-                    att::tmem_wait_store();
-                }
+                if (!idle) att::tmem_wait_store();
                 att::fence_before();
                 __syncwarp();
                 if (border) {
@@ -626,7 +671,7 @@ template <bool E4M3> __global__ void __launch_bounds__(Shape<E4M3>::THREADS, 1) 
     }
     att::fence_before();
     __syncthreads();
-    if (warp == MMA_WARP) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    if (warp == SCORE_WARP) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
 }
 
 } /* namespace tiles */
