@@ -103,7 +103,7 @@ __device__ void schedule(const ncb_page_plan &a, const Requests &r, int window, 
     }
     const long long all = weight * a.kv_heads, share = min(max((all + c.blocks - 1) / c.blocks, (long long)c.least), 0x7fffffffll);
     /* Enough tiles for every block: the GPU's own order balances them, and states of cut ones (128 slots each) would cost more than that leaves. */
-    const bool whole = tile && (long long)owners * a.kv_heads >= (long long)WHOLE_ROUNDS * c.blocks;
+    const bool whole = tile ? (long long)owners * a.kv_heads >= (long long)WHOLE_ROUNDS * c.blocks : a.width <= WHOLE_WIDTH;
     if (tid == 0) *reinterpret_cast<int4 *>(work) = make_int4(owners, (int)weight, (int)share, whole);
     if (whole || owners == 0) return;
     __syncthreads();
@@ -130,12 +130,12 @@ __device__ void schedule(const ncb_page_plan &a, const Requests &r, int window, 
         if (tile) { /* the block's pieces: counted, then written */
             int mine = 0;
             if (on)
-                for (Walk walk(records, owners, c.overhead, (int)share, start, all - x, b); walk.next();) mine++;
+                for (Walk walk(records, owners, c.overhead, start, (int)min(share, all - x), b); walk.next();) mine++;
             const long long to = count + block_sum_before(mine, sums, &total);
             start.piece = (int)to;
             if (on) {
                 int i = 0;
-                for (Walk walk(records, owners, c.overhead, (int)share, start, all - x, b); walk.next() && to + i < (WHOLE_ROUNDS + 1ll) * c.blocks; i++)
+                for (Walk walk(records, owners, c.overhead, start, (int)min(share, all - x), b); walk.next() && to + i < (WHOLE_ROUNDS + 1ll) * c.blocks; i++)
                     pieces[to + i] = Piece{walk.o.request, walk.o.row, walk.o.rows, walk.o.pos, walk.o.page0 + walk.page0, walk.page1 - walk.page0, walk.head, walk.part};
             }
             count += total;

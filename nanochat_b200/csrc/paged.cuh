@@ -7,8 +7,8 @@
  * key/value heads, one after the other, is a line of length total * heads, and block b has the piece [b * share, (b + 1) * share) of it, wherever owners
  * begin and end: every block has the same to do, whatever the lengths are. A block leaves at most two owners unfinished, the one that it goes on with
  * from the block before it and the one that the next block goes on with: their states go to parts 2 b and 2 b + 1, and whoever joins them finds
- * them from the sums alone. Where tiles are so many that they fill the GPU several times over, none is cut (WHOLE): each is a block's, the
- * longest first, and no state is written or read.
+ * them from the sums alone. Where tiles are so many that they fill the GPU several times over, or small owners have few pages at most, none is cut: each is a
+ * block's, tiles the longest first, and no state is written or read.
  */
 #pragma once
 
@@ -22,6 +22,7 @@ constexpr int MAX_GROUP = 64;                     /* query heads per key/value h
 constexpr int HEADER_WORDS = 8;                   /* owners, total, share, whole: of a class */
 constexpr int OWNER_WORDS = 8, START_WORDS = 4, PIECE_WORDS = 8;
 constexpr int WHOLE_ROUNDS = 3; /* tiles are cut only where there are fewer than this many for every block */
+constexpr int WHOLE_WIDTH = 16; /* small owners are cut only where a request may have more pages than this: the launch that joins states costs more than it saves */
 
 struct Owner {
     int request, row, rows; /* absolute first row */
@@ -129,8 +130,9 @@ struct Walk {
     int head, page0, page1; /* the piece: pages [page0, page1) of the owner's, for this key/value head */
     int part;               /* as Piece's */
 
-    __device__ __forceinline__ Walk(const Owner *owners, int n, int overhead, int share, const Start &start, long long left, int block)
-        : owners(owners), n(n), overhead(overhead), at(start.owner), next_head(start.head), local(start.local), left((int)min((long long)share, left)), block(block) {}
+    /* From `start` on, `left` of the line. */
+    __device__ __forceinline__ Walk(const Owner *owners, int n, int overhead, const Start &start, int left, int block)
+        : owners(owners), n(n), overhead(overhead), at(start.owner), next_head(start.head), local(start.local), left(left), block(block) {}
     /* The next piece; false at the end. */
     __device__ __forceinline__ bool next() {
         while (left > 0) {

@@ -5,7 +5,7 @@
  *
  * k_paged_small, for requests of at most 16 query slots (new rows x the heads of a key/value head's group): bound by the stream of pages. A block of
  * four warps takes an entry of the schedule and a key/value head; each warp fetches every fourth unit (an e4m3 page, half a bf16 page) into a place of its
- * own, consumes it and fetches its next: three blocks per SM keep twelve units of 16 KB in flight or in use, and no warp waits for another until the entry ends.
+ * own, consumes it and fetches its next: three blocks per SM keep twelve units of 16 KB in flight or in use, and no warp waits for another until the piece ends.
  * The CACHE is the A operand of both products (m16n8k16: 16 keys, or 16 dims of V^T), the slots its 8 columns (two tiles of them for more than 8), so
  * that few slots waste little; score accumulators become the B operand of V^T P by 8 x 8 transposes.
  *   - bf16 pages: a probability enters as two bf16 terms (hi + lo, 16 bits): one term would double the error of the bf16 output, and the
@@ -18,13 +18,15 @@
  * k_paged_tiles (paged_tiles.cuh), for the others: tcgen05. k_paged_merge: the states of owners that were cut.
  * Waits are bounded: when one expires NCB_DEV_WAIT_TIMEOUT is flagged and the block leaves after its copies in flight.
  */
+#include <atomic>
+
 #include "paged_tiles.cuh"
 
 namespace {
 
 using namespace paged;
 
-constexpr int WARPS = 4, BLOCKS_PER_SM = 3;
+constexpr int WARPS = 4, DEEP = 3;
 constexpr float LOG2_E = 1.4426950408889634f;
 constexpr float P_SCALE = 256.f; /* keeps small folded probabilities among f16's normal numbers; an exact power of two */
 constexpr float MIN_LOG2_VSCALE = -64.f;
@@ -32,12 +34,13 @@ constexpr int BOX_ROWS = 32, BOX_BYTES = BOX_ROWS * 128;
 
 /* What a warp fetches and consumes at a time: an e4m3 page, or half a bf16 page (four boxes of 32 rows x 64 columns, swizzled: keys' columns 0 .. 63
  * and 64 .. 127, then the values'). */
-template <bool E4M3> struct Unit {
+template <bool E4M3, int DEPTH> struct Unit {
     static constexpr int KEYS = E4M3 ? PAGE_TOKENS : PAGE_TOKENS / 2, PER_PAGE = PAGE_TOKENS / KEYS;
     static constexpr int BYTES = E4M3 ? PAGE_BYTES : 4 * BOX_BYTES;
-    static constexpr int SMEM = 1024 + WARPS * BYTES; /* 1024: swizzled boxes are aligned by hand */
-    static_assert(BLOCKS_PER_SM * (SMEM + 2048) <= 228 * 1024, "blocks per SM");
-    static_assert(WARPS * SMALL_SLOTS * PART * 4 <= WARPS * BYTES, "the warps' states lie where their units were");
+    static constexpr int PLACES = WARPS * DEPTH, BLOCKS = DEPTH == 1 ? 3 : 1; /* blocks per SM */
+    static constexpr int SMEM = 1024 + PLACES * BYTES; /* 1024: swizzled boxes are aligned by hand */
+    static_assert(BLOCKS * (SMEM + 2048) <= 228 * 1024, "blocks per SM");
+    static_assert(WARPS * SMALL_SLOTS * PART * 4 <= PLACES * BYTES, "the warps' states lie where their units were");
 };
 
 __device__ __forceinline__ float lg2(float x) {
@@ -125,20 +128,21 @@ template <bool E4M3> __device__ __forceinline__ bool strange_values(const uint8_
     return __any_sync(0xffffffffu, strange);
 }
 
-template <bool E4M3, int NT> __global__ void __launch_bounds__(32 * WARPS, BLOCKS_PER_SM) k_paged_small(const __grid_constant__ CUtensorMap map, const PagedArgs args) {
-    using U = Unit<E4M3>;
+template <bool E4M3, int NT, int DEPTH> __global__ void __launch_bounds__(32 * WARPS, (Unit<E4M3, DEPTH>::BLOCKS)) k_paged_small(const __grid_constant__ CUtensorMap map, const PagedArgs args) {
+    using U = Unit<E4M3, DEPTH>;
     constexpr int TILES = U::KEYS / 16; /* of 16 keys */
     extern __shared__ __align__(128) uint8_t raw[];
-    __shared__ __align__(8) uint64_t bars[WARPS];
+    __shared__ __align__(8) uint64_t bars[U::PLACES];
     __shared__ int failed;
     __shared__ float state_m[WARPS][8 * NT], state_l[WARPS][8 * NT];
     const ncb_paged &a = args.p;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     uint8_t *smem = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
-    const uint8_t *unit = smem + warp * U::BYTES;
-    const uint32_t unit_u = smem_u32(unit), bar = smem_u32(bars + warp);
+    /* the warp's n-th unit has its place n % DEPTH */
+    auto place = [&](uint32_t n) { return smem + (warp * DEPTH + n % DEPTH) * U::BYTES; };
+    auto bar = [&](uint32_t n) { return smem_u32(bars + warp * DEPTH + n % DEPTH); };
     if (tid == 0) {
-        for (int w = 0; w < WARPS; w++) mbar_init(smem_u32(bars + w), 1);
+        for (int w = 0; w < U::PLACES; w++) mbar_init(smem_u32(bars + w), 1);
         failed = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -148,11 +152,20 @@ template <bool E4M3, int NT> __global__ void __launch_bounds__(32 * WARPS, BLOCK
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int G = a.Hq / a.Hkv;
     const uint64_t once = policy_evict_first();
-    uint32_t loads = 0; /* of this warp so far: the parity of its barrier */
+    uint32_t begun = 0, done = 0, there = 0; /* units of this warp; which places hold one that is in the pool */
     const Line line(args, 0);
-    const Start start = line.starts[blockIdx.x];
-    if (blockIdx.x * line.share >= line.all()) return;
-    Walk walk(line.owners, line.n, line.overhead, (int)line.share, start, line.all() - blockIdx.x * line.share, blockIdx.x);
+    Start start = {(int)blockIdx.x / a.Hkv, (int)blockIdx.x % a.Hkv, 0, 0};
+    long long left;
+    if (line.whole) {
+        if (start.owner >= line.n) return;
+        left = line.overhead + max(line.owners[start.owner].pages, 1);
+    } else {
+        start = line.starts[blockIdx.x];
+        left = line.all() - blockIdx.x * line.share;
+        if (left <= 0) return;
+        left = min(left, line.share);
+    }
+    Walk walk(line.owners, line.n, line.overhead, start, (int)left, blockIdx.x);
     while (walk.next()) {
         const Owner &e = walk.o;
         const int kvh = walk.head, page0 = e.page0 + walk.page0, part_at = walk.part;
@@ -160,25 +173,32 @@ template <bool E4M3, int NT> __global__ void __launch_bounds__(32 * WARPS, BLOCK
         const long long first_row = e.row;
         const int *table = a.table + (size_t)e.request * a.width + page0;
         auto begin_of = [&](int pos) { return a.window > 0 ? max(0, pos + 1 - a.window) : 0; }; /* the first position that the row at pos sees */
-        /* Unit i into this warp's place; false where its page is not in the pool (nothing is fetched). */
+        /* The piece's unit i, of this page, into the warp's next place; a page that is not in the pool is left out. */
         auto fetch = [&](int i, int page) {
-            if ((unsigned)page >= (unsigned)a.n_pages) {
-                if (lane == 0) flag(a.status, NCB_DEV_BAD_PAGE);
-                return false;
+            const bool in = (unsigned)page < (unsigned)a.n_pages;
+            const uint32_t to = smem_u32(place(begun)), full = bar(begun), bit = 1u << begun % DEPTH;
+            there = in ? there | bit : there & ~bit;
+            begun++;
+            if (lane != 0) return;
+            if (!in) {
+                flag(a.status, NCB_DEV_BAD_PAGE);
+                att::arrive(full);
+                return;
             }
-            if (lane == 0) {
-                mbar_expect_tx(bar, U::BYTES);
-                if (E4M3) {
-                    bulk_load_once(unit_u, (const uint8_t *)a.pool + ((size_t)page * a.Hkv + kvh) * PAGE_BYTES, PAGE_BYTES, bar, once);
-                } else {
-                    const int row = (page * a.Hkv + kvh) * 2 * PAGE_TOKENS + i % U::PER_PAGE * BOX_ROWS;
+            mbar_expect_tx(full, U::BYTES);
+            if (E4M3) {
+                bulk_load_once(to, (const uint8_t *)a.pool + ((size_t)page * a.Hkv + kvh) * PAGE_BYTES, PAGE_BYTES, full, once);
+            } else {
+                const int row = (page * a.Hkv + kvh) * 2 * PAGE_TOKENS + i % U::PER_PAGE * BOX_ROWS;
 #pragma unroll
-                    for (int x = 0; x < 4; x++) tma_load(unit_u + x * BOX_BYTES, &map, 64 * (x & 1), row + (x >> 1) * PAGE_TOKENS, bar, once);
-                }
+                for (int x = 0; x < 4; x++) tma_load(to + x * BOX_BYTES, &map, 64 * (x & 1), row + (x >> 1) * PAGE_TOKENS, full, once);
             }
-            return true;
         };
-        bool there = warp < units && fetch(warp, table[warp / U::PER_PAGE]);
+#pragma unroll
+        for (int d = 0; d < DEPTH; d++) {
+            const int i = warp + d * WARPS;
+            if (i < units) fetch(i, table[i / U::PER_PAGE]);
+        }
         /* ---- queries: column n = lane / 4 of tile nt is slot 8 nt + n; k slots (2t, 2t+1), (2t+8, 2t+9) of step s are dims 16 s + 2 t .. and + 8, or (E4M3)
          * 16 s + 4 t .. + 3, as the cache bytes arrive ---- */
         uint32_t qb[NT][8][2];
@@ -229,18 +249,19 @@ template <bool E4M3, int NT> __global__ void __launch_bounds__(32 * WARPS, BLOCK
 #pragma unroll
                 for (int x = 0; x < 4; x++) o[nt][d][x] = 0.f;
         }
-        bool ok = true;
         for (int i = warp; i < units; i += WARPS) {
             const int unit_pos = (page0 * U::PER_PAGE + i) * U::KEYS;
-            const int next = i + WARPS < units ? table[(i + WARPS) / U::PER_PAGE] : 0;
-            if (there && !__all_sync(0xffffffffu, mbar_wait(bar, loads & 1))) {
+            const int ahead = i + DEPTH * WARPS, next = ahead < units ? table[ahead / U::PER_PAGE] : 0;
+            const uint8_t *unit = place(done);
+            const uint32_t unit_u = smem_u32(unit);
+            if (!__all_sync(0xffffffffu, mbar_wait(bar(done), done / DEPTH & 1))) {
                 if (lane == 0) flag(a.status, NCB_DEV_WAIT_TIMEOUT), failed = 1;
-                mbar_wait(bar, loads & 1); /* nobody leaves under a copy */
-                ok = false;
+                for (uint32_t n = done; n < begun; n++) mbar_wait(bar(n), n / DEPTH & 1); /* nobody leaves under a copy */
+                break;
             }
-            loads += there;
-            if (!ok) break;
-            if (there && unit_pos <= last_pos && unit_pos + U::KEYS > any_from) {
+            const bool in = there >> done % DEPTH & 1;
+            done++;
+            if (in && unit_pos <= last_pos && unit_pos + U::KEYS > any_from) {
                 /* ---- scores: tile k, element x: key row lane / 4 (x < 2) or 8 + lane / 4 of the tile, slots 2 t + x % 2. Rows are keys in order, or (E4M3) rows r and
                  * 8 + r keys 4 (r / 2) + r % 2 and 2 more, so that their transposes meet four consecutive bytes of V^T ---- */
                 const int row[2] = {E4M3 ? 4 * (g >> 1) + (g & 1) : g, E4M3 ? 4 * (g >> 1) + (g & 1) + 2 : g + 8};
@@ -407,7 +428,7 @@ template <bool E4M3, int NT> __global__ void __launch_bounds__(32 * WARPS, BLOCK
                 }
             }
             __syncwarp(); /* every lane has read the unit */
-            there = i + WARPS < units && fetch(i + WARPS, next);
+            if (ahead < units) fetch(ahead, next);
         }
         __syncthreads(); /* every warp has finished with its units: their states go there */
         float *mine = reinterpret_cast<float *>(smem) + warp * 8 * NT * PART;
@@ -459,7 +480,7 @@ __global__ void __launch_bounds__(32 * MERGE_WARPS) k_paged_merge(const PagedArg
     const ncb_paged &a = args.p;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const int smalls = args.caps.smalls ? args.caps.small.blocks : 0, tile = (int)blockIdx.x >= smalls, lane = threadIdx.x & 31, G = a.Hq / a.Hkv;
+    const int smalls = args.caps.smalls && a.width > WHOLE_WIDTH ? args.caps.small.blocks : 0, tile = (int)blockIdx.x >= smalls, lane = threadIdx.x & 31, G = a.Hq / a.Hkv;
     const Class &cls = tile ? args.caps.tile : args.caps.small;
     const int groups = tile ? (cls.slots + MERGE_SLOTS - 1) / MERGE_SLOTS : 1, job = blockIdx.x - (tile ? smalls : 0), end = job / groups + 1, slot0 = job % groups * MERGE_SLOTS;
     const Line line(args, tile);
@@ -505,15 +526,36 @@ template <typename... Args> cudaError_t launch(void (*kernel)(Args...), unsigned
     return cudaLaunchKernelEx(&config, kernel, Args(args)...);
 }
 
-template <bool E4M3, int NT> cudaError_t small(const CUtensorMap &map, const PagedArgs &args, cudaStream_t stream) {
-    constexpr int smem = Unit<E4M3>::SMEM;
-    const cudaError_t rc = cudaFuncSetAttribute(k_paged_small<E4M3, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+/* Opts a kernel in to its dynamic shared memory, once per device. */
+template <typename Kernel> cudaError_t allow_smem(Kernel kernel, int bytes, std::atomic<unsigned long long> &ready) {
+    int device;
+    cudaError_t rc = cudaGetDevice(&device);
     if (rc != cudaSuccess) return rc;
-    return launch(k_paged_small<E4M3, NT>, args.caps.small.blocks, 32 * WARPS, smem, stream, map, args);
+    const unsigned long long bit = device < 64 ? 1ull << device : 0;
+    if (ready.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+    rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (rc == cudaSuccess) ready.fetch_or(bit, std::memory_order_relaxed);
+    return rc;
+}
+
+template <bool E4M3, int NT, int DEPTH> cudaError_t small(const CUtensorMap &map, const PagedArgs &args, long long blocks, cudaStream_t stream) {
+    constexpr int smem = Unit<E4M3, DEPTH>::SMEM;
+    static std::atomic<unsigned long long> ready{0};
+    const cudaError_t rc = allow_smem(k_paged_small<E4M3, NT, DEPTH>, smem, ready);
+    if (rc != cudaSuccess) return rc;
+    return launch(k_paged_small<E4M3, NT, DEPTH>, (unsigned)blocks, 32 * WARPS, smem, stream, map, args);
+}
+/* Where owners are whole and there is at most one for every SM, a warp has three units in flight instead of one: the call is then as long as its longest owner, not as
+ * its bytes. */
+template <bool E4M3, int NT> cudaError_t small(const CUtensorMap &map, const PagedArgs &args, cudaStream_t stream) {
+    const bool whole = args.p.width <= WHOLE_WIDTH;
+    const long long blocks = whole ? args.caps.small.owners * args.p.Hkv : args.caps.small.blocks;
+    return whole && blocks <= args.p.blocks ? small<E4M3, NT, DEEP>(map, args, blocks, stream) : small<E4M3, NT, 1>(map, args, blocks, stream);
 }
 template <bool E4M3> cudaError_t tile(const CUtensorMap &map_q, const CUtensorMap &map_kv, const PagedArgs &args, cudaStream_t stream) {
     constexpr int smem = tiles::Shape<E4M3>::SMEM;
-    const cudaError_t rc = cudaFuncSetAttribute(tiles::k_paged_tiles<E4M3>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    static std::atomic<unsigned long long> ready{0};
+    const cudaError_t rc = allow_smem(tiles::k_paged_tiles<E4M3>, smem, ready);
     if (rc != cudaSuccess) return rc;
     const long long whole = args.caps.tile.owners * args.p.Hkv; /* blocks where no tile is cut */
     return launch(tiles::k_paged_tiles<E4M3>, (unsigned)(whole > args.caps.tile.blocks ? whole : args.caps.tile.blocks), tiles::THREADS, smem, stream, map_q, map_kv, args);
@@ -552,7 +594,7 @@ int paged_attn(const ncb_paged *args, void *stream) {
     PagedArgs p = {a, caps_of(a.requests, a.rows, a.max_fresh, a.Hq / a.Hkv, a.blocks), a.scale * LOG2_E};
     if (a.workspace_bytes < paged_attn_workspace_bytes(a.requests, a.rows, a.max_fresh, a.Hq, a.Hkv, a.blocks)) return NCB_ERR_WORKSPACE;
     const long long key_rows = (long long)a.n_pages * a.Hkv * 2 * PAGE_TOKENS;
-    if (key_rows > 0x7fffffffll || p.caps.tile.owners * a.Hkv > 0x7fffffffll) return NCB_ERR_UNSUPPORTED;
+    if (key_rows > 0x7fffffffll || p.caps.tile.owners * a.Hkv > 0x7fffffffll || p.caps.small.owners * a.Hkv > 0x7fffffffll) return NCB_ERR_UNSUPPORTED;
     CUtensorMap map = {}, map_q = {};
     const cudaStream_t s = (cudaStream_t)stream;
     if (p.caps.tiles) {
@@ -566,7 +608,8 @@ int paged_attn(const ncb_paged *args, void *stream) {
         const cudaError_t rc = a.e4m3 ? (one ? small<true, 1>(map, p, s) : small<true, 2>(map, p, s)) : (one ? small<false, 1>(map, p, s) : small<false, 2>(map, p, s));
         if (rc != cudaSuccess) return NCB_ERR_LAUNCH;
     }
-    const int ends = (p.caps.smalls ? p.caps.small.blocks : 0) + (p.caps.tiles ? p.caps.tile.blocks * ((p.caps.tile.slots + MERGE_SLOTS - 1) / MERGE_SLOTS) : 0);
+    const int ends = (p.caps.smalls && a.width > WHOLE_WIDTH ? p.caps.small.blocks : 0) + (p.caps.tiles ? p.caps.tile.blocks * ((p.caps.tile.slots + MERGE_SLOTS - 1) / MERGE_SLOTS) : 0);
+    if (ends == 0) return NCB_OK;
     return launch(k_paged_merge, ends, 32 * MERGE_WARPS, 0, s, p) == cudaSuccess ? NCB_OK : NCB_ERR_LAUNCH;
 }
 

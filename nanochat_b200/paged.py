@@ -13,6 +13,7 @@ NativeError, what only the device can see is ORed into `status` (NCB_DEV_* bits)
 
 import contextlib
 import ctypes
+import functools
 
 import torch
 from torch import Tensor
@@ -21,20 +22,30 @@ from .kv_cache import HEAD_DIM, PAGE_TOKENS, PagedKVCache, cache_pages
 from .native import PLAN_WINDOWS, Paged, Plan, check, cuda_library, pointer, stream
 
 _READY = contextlib.nullcontext()
+_INT, _BF16, _F32 = torch.int32, torch.bfloat16, torch.float32
 
 
 def on_device_of(t: Tensor):
     """The launches below go to the current stream of the current device: make it the tensors' one."""
     assert t.is_cuda, "the operands live on a CUDA device"
-    return _READY if t.device.index == torch._C._cuda_getDevice() else torch.cuda.device(t.device)
+    return _READY if t.get_device() == torch._C._cuda_getDevice() else torch.cuda.device(t.device)
 
 
 def _words(t: Tensor, *shape: int) -> bool:
-    return t.dtype == torch.int32 and t.shape == shape and t.is_contiguous()
+    return t.dtype is _INT and t.shape == shape and t.is_contiguous()
 
 
 def address(t: "Tensor | None") -> "int | None":
     return None if t is None else t.data_ptr()
+
+
+@functools.cache
+def _sizes(requests: int, rows: int, max_new: int, Hq: int, Hkv: int) -> tuple[int, int, int]:
+    """(blocks, words of a schedule, bytes of a workspace) of plans of this size; words -1: none."""
+    attn = cuda_library("paged_attn")
+    blocks = attn.paged_attn_blocks()
+    return (blocks, cuda_library("page_plan").page_plan_words(requests, rows, max_new, Hq // Hkv, Hkv, blocks),
+            attn.paged_attn_workspace_bytes(requests, rows, max_new, Hq, Hkv, blocks))
 
 
 class PageTable:
@@ -83,22 +94,24 @@ class PagePlan:
     def __init__(self, pages: PageTable, rows: int, max_new: int, Hq: int, Hkv: int, windows: "tuple[int, ...]" = (0,)):
         assert Hkv > 0 and Hq > 0 and Hq % Hkv == 0 and 0 < len(windows) <= PLAN_WINDOWS and len(set(windows)) == len(windows)
         self.pages, self.rows, self.max_new, self.Hq, self.Hkv, self.windows = pages, rows, max_new, Hq, Hkv, tuple(windows)
-        n, group = pages.requests, Hq // Hkv
-        self.blocks = cuda_library("paged_attn").paged_attn_blocks()
-        words = cuda_library("page_plan").page_plan_words(n, rows, max_new, group, Hkv, self.blocks)
+        n = pages.requests
+        self.blocks, words, self.workspace_bytes = _sizes(n, rows, max_new, Hq, Hkv)
         if words < 0:
             raise ValueError(f"no plan for {n} requests, {rows} rows, at most {max_new} a request, {Hq} heads over {Hkv}")
-        at = (3 * n + 1 + 3 * rows + 3) // 4 * 4
-        flat = self._flat = torch.empty(at + words * len(windows), dtype=torch.int32, device=pages.device)
-        self.row_start, self.fresh, self.lens, self.pos, self.place, self.request, _, self.work = flat.split(
-            [n + 1, n, n, rows, rows, rows, at - (3 * n + 1 + 3 * rows), words * len(windows)])
-        self._at = {w: self.work.data_ptr() + 4 * words * i for i, w in enumerate(self.windows)}
+        used, per = 3 * n + 1 + 3 * rows, words * len(windows)
+        at = (used + 3) // 4 * 4
+        flat = torch.empty(at + per, dtype=_INT, device=pages.device)
+        self.row_start, self.fresh, self.lens, self.pos, self.place, self.request, _, self.work = torch.split_with_sizes(
+            flat, [n + 1, n, n, rows, rows, rows, at - used, per])
+        self.own_lens = self.lens
         base = flat.data_ptr()
-        places = [base + 4 * i for i in (0, n + 1, 2 * n + 1, 3 * n + 1, 3 * n + 1 + rows, 3 * n + 1 + 2 * rows)]
-        self._args = Plan(pages.table.data_ptr(), None, None, pages.free.data_ptr(), pages.free_count.data_ptr(), None, *places, self.work.data_ptr(),
-                          pages.ticket.data_ptr(), None, rows, n, pages.width, pages.n_pages, max_new, group, Hkv, self.blocks, len(windows),
-                          (ctypes.c_int * PLAN_WINDOWS)(*windows))
-        self._own_lens = places[2]
+        work = base + 4 * at
+        self._schedules = {w: work + 4 * words * i for i, w in enumerate(windows)}
+        after = base + 4 * (n + 1)
+        rows_at = base + 4 * (3 * n + 1)
+        self._args = bytes(Plan(pages.table.data_ptr(), None, None, pages.free.data_ptr(), pages.free_count.data_ptr(), None, base, after, None, rows_at,
+                                rows_at + 4 * rows, rows_at + 8 * rows, work, pages.ticket.data_ptr(), None, rows, n, pages.width, pages.n_pages, max_new,
+                                Hq // Hkv, Hkv, self.blocks, len(windows), (ctypes.c_int * PLAN_WINDOWS)(*windows)))
 
 
 def page_plan(pages: PageTable, cached: Tensor, new: Tensor, rows: int, *, max_new: int, Hq: int, Hkv: int, windows: "tuple[int, ...]" = (0,),
@@ -119,11 +132,12 @@ def page_plan(pages: PageTable, cached: Tensor, new: Tensor, rows: int, *, max_n
             plan = PagePlan(pages, rows, max_new, Hq, Hkv, windows)
         elif plan.pages is not pages or (plan.rows, plan.max_new, plan.Hq, plan.Hkv, plan.windows) != (rows, max_new, Hq, Hkv, tuple(windows)):
             raise ValueError("the plan was made for other sizes or another table")
-        plan.lens = plan.lens if lens is None else lens
-        args = plan._args
-        args.cached, args.fresh, args.status = cached.data_ptr(), new.data_ptr(), address(status)
-        args.lens = plan.lens.data_ptr()
+        plan.lens = plan.own_lens if lens is None else lens
+        args = Plan.from_buffer_copy(plan._args)
+        args.cached, args.fresh, args.lens = cached.data_ptr(), new.data_ptr(), plan.lens.data_ptr()
         args.free_left = (pages.free_count if free_left is None else free_left).data_ptr()
+        if status is not None:
+            args.status = status.data_ptr()
         check(cuda_library("page_plan").page_plan(ctypes.byref(args), stream()), "page_plan")
     return plan
 
@@ -133,20 +147,24 @@ def paged_append(qkv: Tensor, q_gain: Tensor, k_gain: Tensor, cos: Tensor, sin: 
     """kv_append into a pool of pages: norm + rotate q and k, and store k and v at place[row] = page * 64 + position % 64 (a plan's
     pos and place; int32 (rows,), no place twice), quantised to e4m3 with a scale per row and head, or in bf16, as the pool is.
     Same bits as kv_append. Rows with a negative position or place are idle: nothing is written for them. Returns q_out (rows, Hq, 128) bf16."""
-    rows, Hkv = qkv.shape[0], cache.kv_heads
-    assert qkv.dtype == torch.bfloat16 and qkv.stride(-1) == 1 and qkv.shape[1] == (Hq + 2 * Hkv) * HEAD_DIM
+    (rows, width), Hkv, pages = qkv.shape, cache.kv_heads, cache.pages
+    stride, step = qkv.stride()
+    assert qkv.dtype is _BF16 and step == 1 and width == (Hq + 2 * Hkv) * HEAD_DIM
+    if rows <= 1:
+        stride = width  # of a single row it says nothing
     assert _words(pos, rows) and _words(place, rows)
     assert cos.shape == sin.shape and cos.shape[1] == HEAD_DIM // 2 and cos.is_contiguous() and sin.is_contiguous()
-    assert q_gain.dtype == k_gain.dtype == cos.dtype == sin.dtype == torch.float32
+    assert q_gain.dtype is k_gain.dtype is cos.dtype is sin.dtype is _F32
     assert q_gain.shape == k_gain.shape == (HEAD_DIM,) and q_gain.is_contiguous() and k_gain.is_contiguous()
     if q_out is None:
-        q_out = torch.empty((rows, Hq, HEAD_DIM), dtype=torch.bfloat16, device=qkv.device)
-    assert q_out.dtype == torch.bfloat16 and q_out.shape == (rows, Hq, HEAD_DIM) and q_out.is_contiguous()
+        q_out = qkv.new_empty((rows, Hq, HEAD_DIM))
+    else:
+        assert q_out.dtype is _BF16 and q_out.shape == (rows, Hq, HEAD_DIM) and q_out.is_contiguous()
     with on_device_of(qkv):
         check(cuda_library("paged_append").paged_append(
             qkv.data_ptr(), q_gain.data_ptr(), k_gain.data_ptr(), cos.data_ptr(), sin.data_ptr(), pos.data_ptr(), place.data_ptr(),
-            q_out.data_ptr(), cache.pages.data_ptr(), rows, Hq, Hkv, qkv.stride(0), cos.shape[0], cache.n_pages, cache.e4m3, address(status),
-            stream()), "paged_append")
+            q_out.data_ptr(), pages.data_ptr(), rows, Hq, Hkv, stride, cos.shape[0], cache.n_pages, cache.e4m3, address(status), stream()),
+            "paged_append")
     return q_out
 
 
@@ -155,30 +173,34 @@ def paged_attention(q: Tensor, cache: PagedKVCache, plan: PagePlan, window: int 
     """Causal attention of a step's rows over their requests' pages, whose positions already hold the step's own (paged_append): the
     row at position p attends (p - window, p], or [0, p] with window 0. q (rows, Hq, 128) bf16, heads contiguous, row stride free;
     `window` is one that the plan was made with. Rows of requests that the plan did not serve become zeros; rows behind the last
-    request are left as they were in `out`. workspace: uint8, workspace_bytes_for(plan) bytes, for calls that no other stream overlaps
+    request are left as they were in `out`. workspace: uint8, plan.workspace_bytes long, for calls that no other stream overlaps
     (default: a new one). Returns out (rows, Hq, 128) bf16."""
-    rows, Hq = plan.rows, plan.Hq
-    assert q.dtype == torch.bfloat16 and q.shape == (rows, Hq, HEAD_DIM) and q.stride(2) == 1 and q.stride(1) == HEAD_DIM
+    rows, Hq, pages = plan.rows, plan.Hq, plan.pages
+    shape = (rows, Hq, HEAD_DIM)
+    ldq, head, step = q.stride()
+    assert q.dtype is _BF16 and q.shape == shape and step == 1 and (head == HEAD_DIM or Hq == 1)
+    if rows <= 1:
+        ldq = Hq * HEAD_DIM  # strides of single rows say nothing
     assert cache.kv_heads == plan.Hkv
-    work = plan._at.get(window)
+    work = plan._schedules.get(window)
     if work is None:
         raise ValueError(f"the plan has schedules for windows {plan.windows}, not {window}")
-    pages = plan.pages
     if cache.n_pages != pages.n_pages:
         raise ValueError(f"a pool of {cache.n_pages} pages, a table over {pages.n_pages}")
     if out is None:
-        out = torch.empty((rows, Hq, HEAD_DIM), dtype=torch.bfloat16, device=q.device)
-    assert out.dtype == torch.bfloat16 and out.shape == (rows, Hq, HEAD_DIM) and out.stride(2) == 1 and out.stride(1) == HEAD_DIM
+        out, ldo = q.new_empty(shape), Hq * HEAD_DIM
+    else:
+        ldo, head, step = out.stride()
+        assert out.dtype is _BF16 and out.shape == shape and step == 1 and (head == HEAD_DIM or Hq == 1)
+        if rows <= 1:
+            ldo = Hq * HEAD_DIM
     if workspace is None:
-        workspace = torch.empty(workspace_bytes_for(plan), dtype=torch.uint8, device=q.device)
+        workspace, size = q.new_empty(plan.workspace_bytes, dtype=torch.uint8), plan.workspace_bytes
+    else:
+        size = workspace.numel() * workspace.element_size()
     args = Paged(q.data_ptr(), cache.pages.data_ptr(), out.data_ptr(), workspace.data_ptr(), pages.table.data_ptr(), plan.row_start.data_ptr(),
-                 plan.fresh.data_ptr(), plan.lens.data_ptr(), work, address(status), rows, q.stride(0), out.stride(0), workspace.numel(),
-                 pages.requests, pages.width, pages.n_pages, plan.max_new, Hq, plan.Hkv, cache.e4m3, window, plan.blocks,
-                 HEAD_DIM ** -0.5 if softmax_scale is None else softmax_scale)
+                 plan.fresh.data_ptr(), plan.lens.data_ptr(), work, address(status), rows, ldq, ldo, size, pages.requests, pages.width, pages.n_pages,
+                 plan.max_new, Hq, plan.Hkv, cache.e4m3, window, plan.blocks, HEAD_DIM ** -0.5 if softmax_scale is None else softmax_scale)
     with on_device_of(q):
         check(cuda_library("paged_attn").paged_attn(ctypes.byref(args), stream()), "paged_attn")
     return out
-
-
-def workspace_bytes_for(plan: PagePlan) -> int:
-    return cuda_library("paged_attn").paged_attn_workspace_bytes(plan.pages.requests, plan.rows, plan.max_new, plan.Hq, plan.Hkv, plan.blocks)

@@ -72,7 +72,7 @@ def check_schedule(plan, want, cached, new, rows, group, Hkv, max_new):
                 before += max(pages, 1) + overhead
             assert total == before and share == max(-(-total * Hkv // blocks), least)
             tile = per != 16 // group
-            assert whole == (tile and len(owners) * Hkv >= 3 * blocks)
+            assert whole == (len(owners) * Hkv >= 3 * blocks if tile else plan.pages.width <= 16)
             if whole or len(owners) == 0 or len(owners) * Hkv > 100000:
                 continue
             done, joined = plain.pieces(owners, Hkv, blocks, overhead, total, share)
@@ -232,12 +232,12 @@ class Pool:
     """A pool whose every byte that no request wrote is NaN (codes and scales too), with requests of lens positions, of which a plan
     (`plan`, with spare rows behind the last) has just added the last new."""
 
-    def __init__(self, dtype, Hq, Hkv, lens, new, window=0, seed=0, tail=3, free=None):
+    def __init__(self, dtype, Hq, Hkv, lens, new, window=0, seed=0, tail=3, free=None, width=1):
         gen = torch.Generator().manual_seed(seed)
         held = [-(-n // PAGE) for n in lens]
         self.n_pages, self.rows = sum(held) + 3, sum(new)
         cached, status = [n - k for n, k in zip(lens, new)], words([0])
-        self.pages, *_ = make_table(cached, self.n_pages, max(held + [1]) + 1, free=free, seed=seed)
+        self.pages, *_ = make_table(cached, self.n_pages, max(held + [1, width - 1]) + 1, free=free, seed=seed)
         self.plan = ncb.page_plan(self.pages, words(cached), words(new), self.rows + tail, max_new=max(new + [1]), Hq=Hq, Hkv=Hkv, windows=(window,),
                                   status=status)
         self.status = status.item()
@@ -271,9 +271,9 @@ class Pool:
         self.cache.write(row, args[0][0], args[1][0], args[0][1], args[1][1], start=start)
 
 
-def run_attention(dtype, Hq, Hkv, lens, new, window=0, seed=0, tail=3, scale_q=1.0):
+def run_attention(dtype, Hq, Hkv, lens, new, window=0, seed=0, tail=3, scale_q=1.0, width=1):
     """The last new[b] of request b's lens[b] positions attend. Checks every row against 64 bits; returns the pieces."""
-    pool = Pool(dtype, Hq, Hkv, lens, new, window, seed, tail)
+    pool = Pool(dtype, Hq, Hkv, lens, new, window, seed, tail, width=width)
     rows, plan, status = pool.rows, pool.plan, words([0])
     q = (pool.q.float() * scale_q).bfloat16()
     out = torch.full((rows + tail, Hq, 128), 7.0, dtype=torch.bfloat16, device="cuda")
@@ -298,18 +298,20 @@ def check_rows(pool, q, out, lens, new, window):
 DTYPES = [torch.float8_e4m3fn, torch.bfloat16]
 
 
+@pytest.mark.parametrize("width", [1, 40])  # tables of few pages: no owner is cut
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("heads", [(1, 1), (4, 1), (8, 2), (9, 3), (5, 5), (12, 1), (16, 2), (32, 1), (40, 1), (64, 1)])
 @pytest.mark.parametrize("lens, new", [([1], [1]), ([64, 1, 65, 63], [1, 1, 1, 1]), ([200, 130, 64, 700], [1, 0, 3, 17]), ([513, 40], [70, 40])])
-def test_attention_shapes(dtype, heads, lens, new):
-    run_attention(dtype, *heads, lens, new, seed=len(lens))
+def test_attention_shapes(dtype, heads, lens, new, width):
+    run_attention(dtype, *heads, lens, new, seed=len(lens), width=width)
 
 
+@pytest.mark.parametrize("width", [1, 40])
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("window", [1, 2, 63, 64, 65, 100, 1000])
 @pytest.mark.parametrize("lens, new", [([300, 64, 129], [1, 1, 1]), ([300, 500, 20], [5, 130, 20])])
-def test_attention_windows(dtype, window, lens, new):
-    run_attention(dtype, 8, 2, lens, new, window=window, seed=7)
+def test_attention_windows(dtype, window, lens, new, width):
+    run_attention(dtype, 8, 2, lens, new, window=window, seed=7, width=width)
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -318,12 +320,13 @@ def test_attention_long_contexts_are_split(dtype, lens, new):
     run_attention(dtype, 8, 2, lens, new, seed=9)
 
 
+@pytest.mark.parametrize("width", [1, 40])
 @pytest.mark.parametrize("dtype", DTYPES)
-def test_attention_of_many_small_requests(dtype):
+def test_attention_of_many_small_requests(dtype, width):
     rng = np.random.default_rng(3)
     lens = rng.integers(1, 150, 600).tolist()
     new = [min(n, int(k)) for n, k in zip(lens, rng.integers(0, 4, 600))]
-    run_attention(dtype, 4, 2, lens, new, seed=11)
+    run_attention(dtype, 4, 2, lens, new, seed=11, width=width)
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
