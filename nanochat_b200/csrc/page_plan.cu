@@ -105,7 +105,11 @@ __device__ void schedule(const ncb_page_plan &a, const Requests &r, int window, 
     /* Enough tiles for every block: the GPU's own order balances them, and states of cut ones (128 slots each) would cost more than that leaves. */
     const bool whole = tile ? (long long)owners * a.kv_heads >= (long long)WHOLE_ROUNDS * c.blocks : a.width <= WHOLE_WIDTH;
     if (tid == 0) *reinterpret_cast<int4 *>(work) = make_int4(owners, (int)weight, (int)share, whole);
-    if (whole || owners == 0) return;
+    Join *joins = reinterpret_cast<Join *>(work + joins_at(c));
+    if (whole || owners == 0) {
+        for (int b = tid; b < c.blocks; b += THREADS) joins[b].slots = 0;
+        return;
+    }
     __syncthreads();
     Start *starts = reinterpret_cast<Start *>(work + starts_at(c));
     Piece *pieces = reinterpret_cast<Piece *>(work + pieces_at(c));
@@ -141,6 +145,16 @@ __device__ void schedule(const ncb_page_plan &a, const Requests &r, int window, 
             count += total;
         }
         if (b <= c.blocks) starts[b] = start;
+        if (b > 0 && b <= c.blocks) { /* an owner that this block goes on with, the block before having begun with it? */
+            Join join = {};
+            if (on && start.local > c.overhead) {
+                const Owner &o = records[start.owner];
+                const long long begin = start.head * weight + (listed ? before[start.owner] : o.before) + c.overhead;
+                const int first = (int)(begin / share), end = (int)((begin + max(o.pages, 1) - 1) / share);
+                if (first == b - 1) join = Join{o.row, o.rows * a.group, start.head, first, end, {}};
+            }
+            joins[b - 1] = join;
+        }
     }
 }
 

@@ -6,8 +6,7 @@
  * An owner weighs its pages and OVERHEAD (what a block spends on it besides); `before` are the exclusive sums of the weights, `total` their sum. The work of all
  * key/value heads, one after the other, is a line of length total * heads, and block b has the piece [b * share, (b + 1) * share) of it, wherever owners
  * begin and end: every block has the same to do, whatever the lengths are. A block leaves at most two owners unfinished, the one that it goes on with
- * from the block before it and the one that the next block goes on with: their states go to parts 2 b and 2 b + 1, and whoever joins them finds
- * them from the sums alone. Where tiles are so many that they fill the GPU several times over, or small owners have few pages at most, none is cut: each is a
+ * from the block before it and the one that the next block goes on with: their states go to parts 2 b and 2 b + 1, and the schedule lists which parts are joined. Where tiles are so many that they fill the GPU several times over, or small owners have few pages at most, none is cut: each is a
  * block's, tiles the longest first, and no state is written or read.
  */
 #pragma once
@@ -20,7 +19,7 @@ namespace paged {
 constexpr int SMALL_SLOTS = 16, TILE_SLOTS = 256; /* query slots of a block of the small kernel, of the tile kernel (two tiles of 128) */
 constexpr int MAX_GROUP = 64;                     /* query heads per key/value head */
 constexpr int HEADER_WORDS = 8;                   /* owners, total, share, whole: of a class */
-constexpr int OWNER_WORDS = 8, START_WORDS = 4, PIECE_WORDS = 8;
+constexpr int OWNER_WORDS = 8, START_WORDS = 4, PIECE_WORDS = 8, JOIN_WORDS = 8;
 constexpr int WHOLE_ROUNDS = 3; /* tiles are cut only where there are fewer than this many for every block */
 constexpr int WHOLE_WIDTH = 16; /* small owners are cut only where a request may have more pages than this: the launch that joins states costs more than it saves */
 
@@ -44,7 +43,14 @@ struct Piece {
     int head;
     int part; /* where the state goes; -1: it is the whole owner, and the block writes its rows */
 };
-static_assert(sizeof(Owner) == 4 * OWNER_WORDS && sizeof(Start) == 4 * START_WORDS && sizeof(Piece) == 4 * PIECE_WORDS, "schedule layout");
+/* What k_paged_merge does at the end of a block's part of the line where an owner is cut for the first time: its states are part 2 first + 1 and parts
+ * 2 b of the blocks b behind. */
+struct Join {
+    int row, slots, head; /* the owner's first row; its query slots; none: nothing to do */
+    int first, last;      /* blocks */
+    int pad[3];
+};
+static_assert(sizeof(Join) == 4 * JOIN_WORDS && sizeof(Owner) == 4 * OWNER_WORDS && sizeof(Start) == 4 * START_WORDS && sizeof(Piece) == 4 * PIECE_WORDS, "schedule layout");
 
 struct Class {
     long long owners; /* at most */
@@ -76,9 +82,10 @@ static __host__ __device__ __forceinline__ Caps caps_of(int requests, long long 
     }
     return c;
 }
-/* A class in a schedule: header, owners, starts (of one block more than there are), for tiles the pieces: one per owner and head and one per cut. */
+/* A class in a schedule: header, owners, starts (of one block more than there are), joins (one per block), for tiles the pieces: one per owner and head and one per cut. */
 static __host__ __device__ __forceinline__ long long starts_at(const Class &c) { return HEADER_WORDS + c.owners * OWNER_WORDS; }
-static __host__ __device__ __forceinline__ long long pieces_at(const Class &c) { return starts_at(c) + (c.blocks + 2) / 2 * 2 * START_WORDS; }
+static __host__ __device__ __forceinline__ long long joins_at(const Class &c) { return starts_at(c) + (c.blocks + 2) / 2 * 2 * START_WORDS; }
+static __host__ __device__ __forceinline__ long long pieces_at(const Class &c) { return joins_at(c) + (long long)c.blocks * JOIN_WORDS; }
 static __host__ __device__ __forceinline__ long long class_words(const Class &c, bool tile) {
     return c.owners ? pieces_at(c) + (tile ? (WHOLE_ROUNDS + 1ll) * c.blocks * PIECE_WORDS : 0) : 0;
 }
@@ -119,9 +126,6 @@ struct Line {
         heads = args.p.Hkv, overhead = c.overhead;
     }
     __device__ __forceinline__ long long all() const { return total * heads; }
-    /* First and last block that has pages of an owner. */
-    __device__ __forceinline__ int first_block(int head, const Owner &o) const { return (int)((head * total + o.before + overhead) / share); }
-    __device__ __forceinline__ int last_block(int head, const Owner &o) const { return (int)((head * total + o.before + overhead + max(o.pages, 1) - 1) / share); }
 };
 
 /* What a block of a class that is cut does, one piece after the other. */

@@ -472,44 +472,68 @@ template <bool E4M3, int NT, int DEPTH> __global__ void __launch_bounds__(32 * W
     }
 }
 
-constexpr int MERGE_WARPS = 4, MERGE_SLOTS = 16;
+constexpr int MERGE_WARPS = 8, MERGE_SLOTS = 16;
 
-/* Joins the states of owners that were cut: a block per end of a piece of the line (and 16 of a tile's slots) looks whether an owner is cut there for the first
- * time. A warp per query slot, four dimensions a lane. */
+/* Joins the states of N slots of an owner from `slot0` on: a warp, four dimensions a lane, TOGETHER states of each slot in flight. */
+template <int N, int TOGETHER> __device__ __forceinline__ void join_slots(const ncb_paged &a, const Join &join, const float *parts, int part_slots, int slot0, int lane) {
+    const int slots = min(N, join.slots - slot0), G = a.Hq / a.Hkv;
+    if (slots <= 0) return;
+    float top[N], sum[N];
+    float4 y[N];
+#pragma unroll
+    for (int x = 0; x < N; x++) top[x] = -INFINITY, sum[x] = 0.f, y[x] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int b0 = join.first; b0 <= join.last; b0 += TOGETHER) {
+        float2 ml[N][TOGETHER];
+        float4 v[N][TOGETHER];
+#pragma unroll
+        for (int i = 0; i < TOGETHER; i++)
+#pragma unroll
+            for (int x = 0; x < N; x++) {
+                ml[x][i] = make_float2(-INFINITY, 0.f), v[x][i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (b0 + i > join.last || x >= slots) continue;
+                const float *part = parts + ((size_t)(2 * (b0 + i) + (b0 + i == join.first)) * part_slots + slot0 + x) * PART;
+                ml[x][i] = *reinterpret_cast<const float2 *>(part);
+                v[x][i] = *reinterpret_cast<const float4 *>(part + 4 + 4 * lane);
+            }
+#pragma unroll
+        for (int x = 0; x < N; x++) {
+            float most = top[x];
+#pragma unroll
+            for (int i = 0; i < TOGETHER; i++) most = fmaxf(most, ml[x][i].x);
+            const float old = scale_of(top[x], sum[x], most);
+            top[x] = most, sum[x] *= old, y[x].x *= old, y[x].y *= old, y[x].z *= old, y[x].w *= old;
+#pragma unroll
+            for (int i = 0; i < TOGETHER; i++) {
+                const float f = scale_of(ml[x][i].x, ml[x][i].y, most);
+                sum[x] = fmaf(ml[x][i].y, f, sum[x]);
+                if (f != 0.f) y[x].x = fmaf(v[x][i].x, f, y[x].x), y[x].y = fmaf(v[x][i].y, f, y[x].y), y[x].z = fmaf(v[x][i].z, f, y[x].z), y[x].w = fmaf(v[x][i].w, f, y[x].w);
+            }
+        }
+    }
+#pragma unroll
+    for (int x = 0; x < N; x++) {
+        if (x >= slots) break;
+        const int slot = slot0 + x;
+        const float inv = sum[x] > 0.f || sum[x] != sum[x] ? __fdiv_rn(1.f, a.e4m3 ? sum[x] * P_SCALE : sum[x]) : 0.f;
+        *reinterpret_cast<uint2 *>((bf16 *)a.out + ((size_t)join.row + slot / G) * a.ldo + (size_t)(join.head * G + slot % G) * HEAD_DIM + 4 * lane) =
+            make_uint2(pack_bf16(y[x].x * inv, y[x].y * inv), pack_bf16(y[x].z * inv, y[x].w * inv));
+    }
+}
+
+/* The states of owners that were cut: a block per join of the schedule (and 16 of a tile's slots). Nothing but the record comes before the states, so that with few of them the
+ * launch is as long as three reads one after the other. */
 __global__ void __launch_bounds__(32 * MERGE_WARPS) k_paged_merge(const PagedArgs args) {
     const ncb_paged &a = args.p;
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const int smalls = args.caps.smalls && a.width > WHOLE_WIDTH ? args.caps.small.blocks : 0, tile = (int)blockIdx.x >= smalls, lane = threadIdx.x & 31, G = a.Hq / a.Hkv;
+    const int smalls = args.caps.smalls && a.width > WHOLE_WIDTH ? args.caps.small.blocks : 0, tile = (int)blockIdx.x >= smalls, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const Class &cls = tile ? args.caps.tile : args.caps.small;
-    const int groups = tile ? (cls.slots + MERGE_SLOTS - 1) / MERGE_SLOTS : 1, job = blockIdx.x - (tile ? smalls : 0), end = job / groups + 1, slot0 = job % groups * MERGE_SLOTS;
-    const Line line(args, tile);
-    const Start start = line.starts[end];
-    if (line.n == 0 || line.whole || end * line.share >= line.all()) return;
-    const int head = start.head;
-    const Owner o = line.owners[start.owner];
-    const int first = line.first_block(head, o), last = line.last_block(head, o);
-    if (first != end - 1 || last < end) return;
-    for (int slot = slot0 + (int)threadIdx.x / 32; slot < min(slot0 + MERGE_SLOTS, o.rows * G); slot += MERGE_WARPS) {
-        const float *parts = (const float *)a.workspace + parts_at(args.caps, tile);
-        auto part = [&](int b) { return parts + ((size_t)(2 * b + (b == first)) * cls.slots + slot) * PART; };
-        float top = -INFINITY, sum = 0.f;
-        for (int b = first + lane; b <= last; b += 32) top = fmaxf(top, part(b)[0]);
-#pragma unroll
-        for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-        float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-        for (int b = first; b <= last; b++) {
-            const float2 ml = *reinterpret_cast<const float2 *>(part(b));
-            const float4 v = *reinterpret_cast<const float4 *>(part(b) + 4 + 4 * lane);
-            const float f = scale_of(ml.x, ml.y, top);
-            sum = fmaf(ml.y, f, sum);
-            if (f != 0.f) y.x = fmaf(v.x, f, y.x), y.y = fmaf(v.y, f, y.y), y.z = fmaf(v.z, f, y.z), y.w = fmaf(v.w, f, y.w);
-        }
-        const float inv = sum > 0.f || sum != sum ? __fdiv_rn(1.f, a.e4m3 ? sum * P_SCALE : sum) : 0.f;
-        *reinterpret_cast<uint2 *>((bf16 *)a.out + (o.row + slot / G) * a.ldo + (size_t)(head * G + slot % G) * HEAD_DIM + 4 * lane) =
-            make_uint2(pack_bf16(y.x * inv, y.y * inv), pack_bf16(y.z * inv, y.w * inv));
-    }
+    const int groups = tile ? (cls.slots + MERGE_SLOTS - 1) / MERGE_SLOTS : 1, job = blockIdx.x - (tile ? smalls : 0);
+    const float *parts = (const float *)a.workspace + parts_at(args.caps, tile);
+    /* The next launch's blocks do not come before this one's have left: on SMs that still hold some of these they spread unevenly, and a call of 171 us that followed another
+     * one took 240. */
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const Join join = reinterpret_cast<const Join *>(a.work + class_at(args.caps, tile) + joins_at(cls))[job / groups];
+    if (join.slots <= MERGE_WARPS) join_slots<1, 8>(a, join, parts, cls.slots, job % groups * MERGE_SLOTS + warp, lane);
+    else join_slots<2, 4>(a, join, parts, cls.slots, job % groups * MERGE_SLOTS + 2 * warp, lane);
 }
 
 template <typename... Args> cudaError_t launch(void (*kernel)(Args...), unsigned grid, int threads, int smem, cudaStream_t stream, const Args &...args) {
@@ -526,14 +550,16 @@ template <typename... Args> cudaError_t launch(void (*kernel)(Args...), unsigned
     return cudaLaunchKernelEx(&config, kernel, Args(args)...);
 }
 
-/* Opts a kernel in to its dynamic shared memory, once per device. */
+/* Opts a kernel in to its dynamic shared memory, once per device, and asks for the split of an SM's memory that gives most to it: all kernels of a call do, so that an SM
+ * on which the one before has not ended takes as many blocks as another. */
 template <typename Kernel> cudaError_t allow_smem(Kernel kernel, int bytes, std::atomic<unsigned long long> &ready) {
     int device;
     cudaError_t rc = cudaGetDevice(&device);
     if (rc != cudaSuccess) return rc;
     const unsigned long long bit = device < 64 ? 1ull << device : 0;
     if (ready.load(std::memory_order_relaxed) & bit) return cudaSuccess;
-    rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    rc = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+    if (rc == cudaSuccess && bytes) rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (rc == cudaSuccess) ready.fetch_or(bit, std::memory_order_relaxed);
     return rc;
 }
@@ -610,6 +636,8 @@ int paged_attn(const ncb_paged *args, void *stream) {
     }
     const int ends = (p.caps.smalls && a.width > WHOLE_WIDTH ? p.caps.small.blocks : 0) + (p.caps.tiles ? p.caps.tile.blocks * ((p.caps.tile.slots + MERGE_SLOTS - 1) / MERGE_SLOTS) : 0);
     if (ends == 0) return NCB_OK;
+    static std::atomic<unsigned long long> ready{0};
+    if (allow_smem(k_paged_merge, 0, ready) != cudaSuccess) return NCB_ERR_LAUNCH;
     return launch(k_paged_merge, ends, 32 * MERGE_WARPS, 0, s, p) == cudaSuccess ? NCB_OK : NCB_ERR_LAUNCH;
 }
 

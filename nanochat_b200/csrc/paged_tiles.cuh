@@ -14,7 +14,7 @@
  *     probability turns out above 2^7, or a row has seen nothing yet; then the reference is raised, O rescaled and the page done again;
  *   - bf16 pages: a probability enters P V as one bf16 term, at most 2^-9 of it away: the tensor cores would need 512 cycles a page and tile in place of
  *     256 for two terms;
- *   - e4m3 pages: four warps widen every fourth page each to f16 in shared memory (keys in the form of a TMA box, values transposed as they lie), in place
+ *   - e4m3 pages: four warps widen a quarter of every page each to f16 in shared memory (keys in the form of a TMA box, values transposed as they lie), in place
  *     of a launch that widens a request's pages into a workspace of twice the pool's size. Queries are made f16 once per piece, each row times a power of two.
  * A position that a row does not see must not reach it: scores are masked, values are looked at in the pages that the border of some row crosses (three
  * at either end at most), and a page that holds one that is not finite there is multiplied row by row over the positions seen.
@@ -40,8 +40,7 @@ constexpr int TILE_COLUMNS = 256, AT_O = 2 * KEYS; /* tensor memory of a tile: S
 
 template <bool E4M3> struct Shape {
     static constexpr int Q_BYTES = 2 * ROWS * 128, K_BYTES = 2 * KEYS * 128, V_BYTES = K_BYTES; /* Q: of a tile */
-    static constexpr int STAGES = E4M3 ? 2 : 4, RAW_STAGES = E4M3 ? PAGE_WARPS : 0; /* raw: a page's bytes, one for each page warp */
-    static_assert(!E4M3 || PAGE_WARPS <= 2 * STAGES, "a page warp's turns at a place are at most two phases apart");
+    static constexpr int STAGES = E4M3 ? 2 : 4, RAW_STAGES = E4M3 ? 4 : 0; /* raw: a page's bytes */
     static constexpr int AT_K = 2 * Q_BYTES, AT_V = AT_K + STAGES * K_BYTES, AT_RAW = AT_V + STAGES * V_BYTES, AT_SCALE = AT_RAW + RAW_STAGES * PAGE_BYTES;
     static constexpr int SCALE_FLOATS = 3 * KEYS, AT_BARS = AT_SCALE + (E4M3 ? STAGES * SCALE_FLOATS * 4 : 0);
     static constexpr int SMEM = 1024 + AT_BARS + 1024;
@@ -150,6 +149,7 @@ template <bool E4M3> __global__ void __launch_bounds__(THREADS, 1) k_paged_tiles
     auto v_full = [&](int k) { return bars + 64u + 8u * (k % STAGES); };
     auto v_free = [&](int k) { return bars + 96u + 8u * (k % STAGES); };
     auto raw_full = [&](int k) { return bars + 128u + 8u * (k % RAW); };
+    auto raw_free = [&](int k) { return bars + 320u + 8u * (k % RAW); };
     auto of_tile = [&](int x, int i) { return bars + 160u + 80u * x + 8u * i; };
     auto s_full = [&](int x, int c) { return of_tile(x, c & 1); };
     auto p_ready = [&](int x, int c) { return of_tile(x, 2 + (c & 1)); };
@@ -161,11 +161,12 @@ template <bool E4M3> __global__ void __launch_bounds__(THREADS, 1) k_paged_tiles
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
         for (int s = 0; s < 4; s++) {
-            mbar_init(bars + 8u * s, 1);
+            mbar_init(bars + 8u * s, E4M3 ? PAGE_WARPS : 1);
             mbar_init(bars + 32u + 8u * s, 2);
-            mbar_init(bars + 64u + 8u * s, 1);
+            mbar_init(bars + 64u + 8u * s, E4M3 ? PAGE_WARPS : 1);
             mbar_init(bars + 96u + 8u * s, 2);
             mbar_init(bars + 128u + 8u * s, 1);
+            mbar_init(bars + 320u + 8u * s, PAGE_WARPS);
         }
         for (int x = 0; x < 2; x++) {
             for (int c = 0; c < 2; c++) {
@@ -270,106 +271,102 @@ template <bool E4M3> __global__ void __launch_bounds__(THREADS, 1) k_paged_tiles
                     for (int i = max(0, v - STAGES); i < v; i++) mbar_wait(v_full(i), i / STAGES & 1);
                 }
             }
-        } else { /* every fourth page is this warp's: it fetches it, and widens it */
+        } else { /* a quarter of every page is this warp's to widen: a place of the two is empty no longer than that takes. The first warp fetches pages */
             const int y = warp - PAGE_WARP;
-            int fetch_piece = piece, fetch_at = y, fetch_pages = -1, fetched = 0; /* the next page to fetch: its piece, its number there, and the block's pages before */
+            int fetch_piece = piece, fetch_at = 0, fetch_pages = -1, fetched = 0; /* the next page to fetch: its piece, its number there, and the block's pages before */
             long long fetch_table = 0;
             int fetch_head = 0;
-            auto fetch = [&] { /* false: there is none */
+            auto fetch = [&] {
                 while (fetch_pages < 0 || fetch_at >= fetch_pages) {
-                    if (fetch_pages >= 0) fetch_at -= fetch_pages, fetch_piece++;
-                    if (fetch_piece >= pieces) return false;
+                    if (fetch_pages >= 0) fetch_at = 0, fetch_piece++;
+                    if (fetch_piece >= pieces) return;
                     const Piece e = piece_at(fetch_piece);
                     fetch_pages = e.pages, fetch_head = e.head, fetch_table = (long long)e.request * a.width + e.page0;
                 }
-                const int page = a.table[fetch_table + fetch_at], at = y;
+                const int page = a.table[fetch_table + fetch_at];
                 const bool in = (unsigned)page < (unsigned)a.n_pages;
                 if (lane == 0) {
                     if (!in) flag(a.status, NCB_DEV_BAD_PAGE);
-                    mbar_expect_tx(raw_full(at), PAGE_BYTES); /* outside the pool: page 0, masked and widened to zeros */
-                    bulk_load(base + S::AT_RAW + at * PAGE_BYTES, (const uint8_t *)a.pool + ((size_t)(in ? page : 0) * a.Hkv + fetch_head) * PAGE_BYTES, PAGE_BYTES, raw_full(at));
+                    mbar_expect_tx(raw_full(fetched), PAGE_BYTES); /* outside the pool: page 0, masked and widened to zeros */
+                    bulk_load(base + S::AT_RAW + fetched % RAW * PAGE_BYTES, (const uint8_t *)a.pool + ((size_t)(in ? page : 0) * a.Hkv + fetch_head) * PAGE_BYTES, PAGE_BYTES,
+                              raw_full(fetched));
                 }
-                fetched++, fetch_at += PAGE_WARPS;
-                return true;
+                fetched++, fetch_at++;
             };
-            fetch();
-            int k = 0; /* the block's pages before the piece */
+            if (y == 0)
+                for (int i = 0; i < RAW; i++) fetch();
+            int k = 0; /* the block's pages */
             for (; ok && piece < pieces; piece++) {
                 const Piece e = load_piece();
                 const int *table = a.table + (size_t)e.request * a.width + e.page0;
-                for (int i = (y - k) & PAGE_WARPS - 1; i < e.pages; i += PAGE_WARPS) {
-                    const int ki = k + i;
-                    const uint8_t *page = raw + S::AT_RAW + ki % RAW * PAGE_BYTES;
-                    const bool in = (unsigned)table[i] < (unsigned)a.n_pages;
-                    /* a place's barriers are waited for phase by phase: first for the page before in that place, which another warp has put there */
-                    ok = wait_all(raw_full(ki), ki / RAW) && (ki < STAGES || (wait_all(k_full(ki), ki / STAGES - 1) && wait_all(k_free(ki), ki / STAGES - 1)));
+                int number = e.pages > 0 ? table[0] : 0;
+                for (int i = 0; i < e.pages; i++, k++) {
+                    const uint8_t *page = raw + S::AT_RAW + k % RAW * PAGE_BYTES;
+                    const bool in = (unsigned)number < (unsigned)a.n_pages;
+                    number = i + 1 < e.pages ? table[i + 1] : 0;
+                    if (y == 0 && k > 0) { /* into the place of the page before, which all have read */
+                        if (!(ok = wait_all(raw_free(k - 1), (k - 1) / RAW))) break;
+                        fetch();
+                    }
+                    ok = wait_all(raw_full(k), k / RAW) && (k < STAGES || wait_all(k_free(k), k / STAGES - 1));
                     if (!ok) break;
-                    uint8_t *keys = raw + S::AT_K + ki % STAGES * S::K_BYTES;
-#pragma unroll 1
-                    for (int h = 0; h < 16; h += 8) {
-                        uint4 in4[8];
+                    uint8_t *keys = raw + S::AT_K + k % STAGES * S::K_BYTES;
+                    uint4 in4[4];
 #pragma unroll
-                        for (int n = 0; n < 8; n++) in4[n] = *reinterpret_cast<const uint4 *>(page + page_k_chunk(4 * (h + n) + (lane >> 3), lane & 7)); /* 16 codes of a key */
+                    for (int n = 0; n < 4; n++) in4[n] = *reinterpret_cast<const uint4 *>(page + page_k_chunk(16 * y + 4 * n + (lane >> 3), lane & 7)); /* 16 codes of a key */
 #pragma unroll
-                        for (int n = 0; n < 8; n++) { /* -> 32 bytes: two chunks of a swizzled row */
-                            const int j = 4 * (h + n) + (lane >> 3), c = lane & 7;
-                            uint4 w[2];
-                            widen_e4m3x4(in4[n].x, w[0].x, w[0].y), widen_e4m3x4(in4[n].y, w[0].z, w[0].w);
-                            widen_e4m3x4(in4[n].z, w[1].x, w[1].y), widen_e4m3x4(in4[n].w, w[1].z, w[1].w);
-                            uint8_t *row = keys + (c >> 2) * KEYS * 128 + j * 128;
-                            const uint32_t chunk = ((2 * c & 7) ^ (j & 7)) << 4;
-                            *reinterpret_cast<uint4 *>(row + chunk) = w[0];
-                            *reinterpret_cast<uint4 *>(row + (chunk ^ 16)) = w[1];
-                        }
+                    for (int n = 0; n < 4; n++) { /* -> 32 bytes: two chunks of a swizzled row */
+                        const int j = 16 * y + 4 * n + (lane >> 3), c = lane & 7;
+                        uint4 w[2];
+                        widen_e4m3x4(in4[n].x, w[0].x, w[0].y), widen_e4m3x4(in4[n].y, w[0].z, w[0].w);
+                        widen_e4m3x4(in4[n].z, w[1].x, w[1].y), widen_e4m3x4(in4[n].w, w[1].z, w[1].w);
+                        uint8_t *row = keys + (c >> 2) * KEYS * 128 + j * 128;
+                        const uint32_t chunk = ((2 * c & 7) ^ (j & 7)) << 4;
+                        *reinterpret_cast<uint4 *>(row + chunk) = w[0];
+                        *reinterpret_cast<uint4 *>(row + (chunk ^ 16)) = w[1];
                     }
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     __syncwarp();
-                    if (lane == 0) arrive(k_full(ki));
-                    if (ki >= STAGES && !(ok = wait_all(v_full(ki), ki / STAGES - 1) && wait_all(v_free(ki), ki / STAGES - 1))) break;
-                    uint8_t *values = raw + S::AT_V + ki % STAGES * S::V_BYTES;
-                    float *scales = reinterpret_cast<float *>(raw + S::AT_SCALE) + ki % STAGES * S::SCALE_FLOATS;
+                    if (lane == 0) arrive(k_full(k));
 #pragma unroll
-                    for (int j = lane; j < KEYS; j += 32) { /* score factor, log2 of the value's scale, its scale */
+                    for (int n = 0; n < 4; n++) in4[n] = *reinterpret_cast<const uint4 *>(page + PAGE_V + y * 2048 + (n * 32 + lane) * 16); /* 16 positions of a dimension */
+                    if (k >= STAGES && !(ok = wait_all(v_free(k), k / STAGES - 1))) break;
+                    uint8_t *values = raw + S::AT_V + k % STAGES * S::V_BYTES;
+                    float *scales = reinterpret_cast<float *>(raw + S::AT_SCALE) + k % STAGES * S::SCALE_FLOATS;
+                    if (lane < 16) { /* score factor, log2 of the value's scale, its scale */
+                        const int j = 16 * y + lane;
                         const float vs = in ? reinterpret_cast<const float *>(page + PAGE_VS)[j] : 0.f;
                         scales[j] = in ? reinterpret_cast<const float *>(page + PAGE_KS)[j] : 0.f;
                         scales[KEYS + j] = fmaxf(log2_of(vs), MIN_LOG2_VSCALE);
                         scales[2 * KEYS + j] = vs * P_SCALE;
                     }
-                    const int used = in ? e.pos + e.rows - (e.page0 + i) * KEYS : 0; /* positions past the last row may hold anything: zeros */
-#pragma unroll 1
-                    for (int h = 0; h < 4; h += 2) { /* 16 positions of a dimension: four groups of 16, four times 32 dimensions */
-                        uint4 in4[8];
+                    const int used = (in ? e.pos + e.rows - (e.page0 + i) * KEYS : 0) - 16 * y; /* positions past the last row may hold anything: zeros */
+                    if (used < 16) {
 #pragma unroll
-                        for (int n = 0; n < 8; n++) in4[n] = *reinterpret_cast<const uint4 *>(page + PAGE_V + (h + n / 4) * 2048 + (n % 4 * 32 + lane) * 16);
-                        if (used < KEYS) {
+                        for (int n = 0; n < 4; n++)
 #pragma unroll
-                            for (int n = 0; n < 8; n++)
+                            for (int w = 0; w < 4; w++) {
+                                const int on = used - 4 * w;
+                                (&in4[n].x)[w] = on >= 4 ? (&in4[n].x)[w] : on <= 0 ? 0u : (&in4[n].x)[w] & ((1u << (8 * on)) - 1u);
+                            }
+                    }
 #pragma unroll
-                                for (int w = 0; w < 4; w++) {
-                                    const int on = used - 16 * (h + n / 4) - 4 * w;
-                                    (&in4[n].x)[w] = on >= 4 ? (&in4[n].x)[w] : on <= 0 ? 0u : (&in4[n].x)[w] & ((1u << (8 * on)) - 1u);
-                                }
-                        }
-#pragma unroll
-                        for (int n = 0; n < 8; n++) {
-                            uint4 w[2];
-                            widen_e4m3x4(in4[n].x, w[0].x, w[0].y), widen_e4m3x4(in4[n].y, w[0].z, w[0].w);
-                            widen_e4m3x4(in4[n].z, w[1].x, w[1].y), widen_e4m3x4(in4[n].w, w[1].z, w[1].w);
-                            uint8_t *row = values + (n % 4 * 32 + lane) * 128;
-                            const uint32_t chunk = (2 * (h + n / 4) ^ (lane & 7)) << 4;
-                            *reinterpret_cast<uint4 *>(row + chunk) = w[0];
-                            *reinterpret_cast<uint4 *>(row + (chunk ^ 16)) = w[1];
-                        }
+                    for (int n = 0; n < 4; n++) {
+                        uint4 w[2];
+                        widen_e4m3x4(in4[n].x, w[0].x, w[0].y), widen_e4m3x4(in4[n].y, w[0].z, w[0].w);
+                        widen_e4m3x4(in4[n].z, w[1].x, w[1].y), widen_e4m3x4(in4[n].w, w[1].z, w[1].w);
+                        uint8_t *row = values + (n * 32 + lane) * 128;
+                        const uint32_t chunk = (2 * y ^ (lane & 7)) << 4;
+                        *reinterpret_cast<uint4 *>(row + chunk) = w[0];
+                        *reinterpret_cast<uint4 *>(row + (chunk ^ 16)) = w[1];
                     }
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     __syncwarp();
-                    if (lane == 0) arrive(v_full(ki));
-                    fetch(); /* into the place of this page, which the warp has read */
+                    if (lane == 0) arrive(v_full(k)), arrive(raw_free(k));
                 }
-                k += e.pages;
             }
-            if (*failed && lane == 0) /* the block must not leave under copies still in flight */
-                if (fetched > 0) mbar_wait(raw_full(y), (fetched - 1) & 1);
+            if (*failed && y == 0 && lane == 0) /* the block must not leave under copies still in flight */
+                for (int i = max(0, fetched - RAW); i < fetched; i++) mbar_wait(raw_full(i), i / RAW & 1);
         }
     } else if (warp >= SCORE_WARP) { /* a tile's MMAs, scores and values each by a warp of their own (issuing them and the waits between take longer than the tensor
                                         * cores need); it goes through the loop together (elect_one) */

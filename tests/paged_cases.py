@@ -55,7 +55,7 @@ def attention(q, k, v, first_pos, window):
 
 
 def schedule(words, requests, rows, max_new, group, sms):
-    """[(rows an owner has at most, blocks, overhead, least share, [total, share, whole], owners, starts, pieces)] of a schedule's classes."""
+    """[(rows an owner has at most, blocks, overhead, least share, [total, share, whole], owners, starts, joins, pieces)] of a schedule's classes."""
     w = np.asarray(words)
     few, each = 16 // group, min(requests, rows)
     classes = []
@@ -71,8 +71,10 @@ def schedule(words, requests, rows, max_new, group, sms):
         assert n <= most
         owners = w[at + 8:at + 8 + 8 * n].reshape(-1, 8)
         starts = at + 8 + 8 * most
-        pieces = starts + 4 * ((blocks + 2) // 2 * 2)
-        found.append((per, blocks, overhead, least, w[at + 1:at + 4].tolist(), owners, w[starts:starts + 4 * (blocks + 1)].reshape(-1, 4), w[pieces:pieces + 8 * room].reshape(-1, 8)))
+        joins = starts + 4 * ((blocks + 2) // 2 * 2)
+        pieces = joins + 8 * blocks
+        found.append((per, blocks, overhead, least, w[at + 1:at + 4].tolist(), owners, w[starts:starts + 4 * (blocks + 1)].reshape(-1, 4),
+                      w[joins:pieces].reshape(-1, 8), w[pieces:pieces + 8 * room].reshape(-1, 8)))
         at = pieces + 8 * room
     assert at == len(w)
     return found

@@ -56,12 +56,14 @@ def check_schedule(plan, want, cached, new, rows, group, Hkv, max_new):
     each = len(plan.work) // len(plan.windows)
     for w, window in enumerate(plan.windows):
         cover = []
-        for per, blocks, overhead, least, (total, share, whole), owners, starts, listed in plain.schedule(
+        for per, blocks, overhead, least, (total, share, whole), owners, starts, joins, listed in plain.schedule(
                 plan.work[w * each:(w + 1) * each].tolist(), plan.pages.requests, rows, max_new, group, plan.blocks):
             before = 0
             for b, row, count, pos, page0, pages, at, _ in owners.tolist():
                 row0 = row - want["row_start"][b]
                 assert 0 < count <= per and row0 % per == 0
+                if group <= 16 and max_new > 16 // group:  # both classes
+                    assert (want["row_start"][b + 1] - want["row_start"][b] > 16 // group) == (per != 16 // group) or want["row_start"][b + 1] > rows
                 cover += range(row, row + count)
                 if want["fresh"][b]:
                     first, last = cached[b] + row0, cached[b] + row0 + count - 1
@@ -73,11 +75,15 @@ def check_schedule(plan, want, cached, new, rows, group, Hkv, max_new):
             assert total == before and share == max(-(-total * Hkv // blocks), least)
             tile = per != 16 // group
             assert whole == (len(owners) * Hkv >= 3 * blocks if tile else plan.pages.width <= 16)
+            if whole or len(owners) == 0:
+                assert not joins[:, 1].any()
             if whole or len(owners) == 0 or len(owners) * Hkv > 100000:
                 continue
             done, joined = plain.pieces(owners, Hkv, blocks, overhead, total, share)
             parts = sorted(p[5] for p in done if p[5] >= 0)
             assert parts == sorted(set(parts)) == sorted(x for j in joined.values() for x in j)
+            want_joins = {j[0] // 2: [owners[i, 1], owners[i, 2] * group, head, j[0] // 2, j[-1] // 2] for (head, i), j in joined.items()}
+            assert {b: j[:5] for b, j in enumerate(joins.tolist()) if j[1]} == want_joins
             assert sum(p[4] - p[3] for p in done) == Hkv * int(owners[:, 5].sum())
             ends = owners[:, 6] + np.maximum(owners[:, 5], 1) + overhead
             for blk, (o, head, local, _) in enumerate(starts.tolist()):
