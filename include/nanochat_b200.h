@@ -668,15 +668,15 @@ int paged_append(const void *qkv, const void *q_gain, const void *k_gain, const 
                  void *status, void *stream);
 
 /* ---- library paged_attn ------------------------------------------------------------------------------------------------
- * Causal attention of every request's new rows over its pages, after page_plan and paged_append: row i of request b, at position
- * p = lens[b] - served[b] + i, attends positions (p - window, p]. q bf16 [rows][ldq], out bf16 [rows][ldo]: Hq heads of 128. `work` is
+ * Causal attention of every request's new rows over its pages, after page_plan and paged_append: the row at position p of a request
+ * attends its positions (p - window, p]. q bf16 [rows][ldq], out bf16 [rows][ldo]: Hq heads of 128. `work` is
  * page_plan's schedule for this window, made with the same requests, rows, max_fresh, group and kv_heads; `blocks` of page_plan is
  * paged_attn_blocks(). Rows of requests that were not served become zeros; rows behind the last request are left as they were.
  * workspace: paged_attn_workspace_bytes(), 16-byte aligned, for calls on one stream at a time. */
 typedef struct {
     const void *q, *pool;
     void *out, *workspace;
-    const int *table, *row_start, *served, *lens, *work;
+    const int *table, *work;
     int *status;
     long long rows, ldq, ldo, workspace_bytes;
     int requests, width, n_pages, max_fresh, Hq, Hkv, e4m3, window, blocks;

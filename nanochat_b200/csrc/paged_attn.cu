@@ -615,7 +615,7 @@ int paged_attn(const ncb_paged *args, void *stream) {
     if (!sizes_ok(a.requests, a.rows, a.max_fresh, a.Hq / a.Hkv, a.Hkv, a.blocks)) return NCB_ERR_ARG;
     if (a.ldq < (long long)a.Hq * HEAD_DIM || a.ldo < (long long)a.Hq * HEAD_DIM) return NCB_ERR_ARG;
     if (a.rows == 0) return NCB_OK;
-    if (!a.q || !a.pool || !a.out || !a.workspace || !a.table || !a.row_start || !a.served || !a.lens || !a.work) return NCB_ERR_ARG;
+    if (!a.q || !a.pool || !a.out || !a.workspace || !a.table || !a.work) return NCB_ERR_ARG;
     if (((uintptr_t)a.q | (uintptr_t)a.pool | (uintptr_t)a.out | (uintptr_t)a.workspace | (uintptr_t)a.work) % 16 || a.ldq % 8 || a.ldo % 8) return NCB_ERR_ALIGN;
     PagedArgs p = {a, caps_of(a.requests, a.rows, a.max_fresh, a.Hq / a.Hkv, a.blocks), a.scale * LOG2_E};
     if (a.workspace_bytes < paged_attn_workspace_bytes(a.requests, a.rows, a.max_fresh, a.Hq, a.Hkv, a.blocks)) return NCB_ERR_WORKSPACE;

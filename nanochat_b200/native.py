@@ -105,7 +105,7 @@ class Plan(ctypes.Structure):
 
 class Paged(ctypes.Structure):
     """ncb_paged of include/nanochat_b200.h, field for field."""
-    _fields_ = [(n, c_ptr) for n in ("q", "pool", "out", "workspace", "table", "row_start", "served", "lens", "work", "status")] + \
+    _fields_ = [(n, c_ptr) for n in ("q", "pool", "out", "workspace", "table", "work", "status")] + \
                [(n, c_ll) for n in ("rows", "ldq", "ldo", "workspace_bytes")] + \
                [(n, c_int) for n in ("requests", "width", "n_pages", "max_fresh", "Hq", "Hkv", "e4m3", "window", "blocks")] + \
                [("scale", c_float)]

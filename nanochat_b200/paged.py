@@ -25,10 +25,12 @@ _READY = contextlib.nullcontext()
 _INT, _BF16, _F32 = torch.int32, torch.bfloat16, torch.float32
 
 
-def on_device_of(t: Tensor):
+def on_device_of(*operands: "Tensor | None"):
     """The launches below go to the current stream of the current device: make it the tensors' one."""
-    assert t.is_cuda, "the operands live on a CUDA device"
-    return _READY if t.get_device() == torch._C._cuda_getDevice() else torch.cuda.device(t.device)
+    device = operands[0].get_device()  # -1 for what is not on a GPU
+    for t in operands:
+        assert t is None or t.get_device() == device >= 0, "the operands live on one CUDA device"
+    return _READY if device == torch._C._cuda_getDevice() else torch.cuda.device(device)
 
 
 def _words(t: Tensor, *shape: int) -> bool:
@@ -39,13 +41,19 @@ def address(t: "Tensor | None") -> "int | None":
     return None if t is None else t.data_ptr()
 
 
-@functools.cache
-def _sizes(requests: int, rows: int, max_new: int, Hq: int, Hkv: int) -> tuple[int, int, int]:
-    """(blocks, words of a schedule, bytes of a workspace) of plans of this size; words -1: none."""
+@functools.lru_cache(maxsize=1024)
+def _layout(requests: int, rows: int, max_new: int, Hq: int, Hkv: int, windows: "tuple[int, ...]"):
+    """Of plans of this size: (blocks, words of a window's schedule, bytes of a workspace, words of the plan's parts, the native arguments that only
+    sizes decide); words -1: none."""
+    assert Hkv > 0 and Hq > 0 and Hq % Hkv == 0 and 0 < len(windows) <= PLAN_WINDOWS and len(set(windows)) == len(windows)
     attn = cuda_library("paged_attn")
     blocks = attn.paged_attn_blocks()
-    return (blocks, cuda_library("page_plan").page_plan_words(requests, rows, max_new, Hq // Hkv, Hkv, blocks),
-            attn.paged_attn_workspace_bytes(requests, rows, max_new, Hq, Hkv, blocks))
+    words = cuda_library("page_plan").page_plan_words(requests, rows, max_new, Hq // Hkv, Hkv, blocks)
+    workspace = attn.paged_attn_workspace_bytes(requests, rows, max_new, Hq, Hkv, blocks)
+    parts = [words * len(windows), requests + 1, requests, requests, rows, rows, rows]
+    sizes = Plan(rows=rows, requests=requests, max_fresh=max_new, group=Hq // Hkv, kv_heads=Hkv, blocks=blocks, n_windows=len(windows),
+                 windows=(ctypes.c_int * PLAN_WINDOWS)(*windows))
+    return blocks, words, workspace, parts, bytes(sizes)
 
 
 class PageTable:
@@ -78,7 +86,7 @@ class PageTable:
     def release(self, which: Tensor, status: Tensor | None = None) -> None:
         """Requests with which[b] != 0 (int32 (requests,)) give back the pages of their lens[b] positions and hold none."""
         assert _words(which, self.requests)
-        with on_device_of(self.table):
+        with on_device_of(self.table, which, status):
             check(cuda_library("page_plan").page_release(
                 pointer(self.table), pointer(self.lens), pointer(which), pointer(self.free), pointer(self.free_count), self.requests, self.width,
                 self.n_pages, pointer(status), stream()), "page_release")
@@ -92,26 +100,22 @@ class PagePlan:
     each of `windows`, for Hq query heads over Hkv."""
 
     def __init__(self, pages: PageTable, rows: int, max_new: int, Hq: int, Hkv: int, windows: "tuple[int, ...]" = (0,)):
-        assert Hkv > 0 and Hq > 0 and Hq % Hkv == 0 and 0 < len(windows) <= PLAN_WINDOWS and len(set(windows)) == len(windows)
         self.pages, self.rows, self.max_new, self.Hq, self.Hkv, self.windows = pages, rows, max_new, Hq, Hkv, tuple(windows)
         n = pages.requests
-        self.blocks, words, self.workspace_bytes = _sizes(n, rows, max_new, Hq, Hkv)
+        self.blocks, words, self.workspace_bytes, parts, sizes = _layout(n, rows, max_new, Hq, Hkv, self.windows)
         if words < 0:
             raise ValueError(f"no plan for {n} requests, {rows} rows, at most {max_new} a request, {Hq} heads over {Hkv}")
-        used, per = 3 * n + 1 + 3 * rows, words * len(windows)
-        at = (used + 3) // 4 * 4
-        flat = torch.empty(at + per, dtype=_INT, device=pages.device)
-        self.row_start, self.fresh, self.lens, self.pos, self.place, self.request, _, self.work = torch.split_with_sizes(
-            flat, [n + 1, n, n, rows, rows, rows, at - used, per])
+        flat = pages.table.new_empty(sum(parts))
+        self.work, self.row_start, self.fresh, self.lens, self.pos, self.place, self.request = flat.split_with_sizes(parts)
         self.own_lens = self.lens
-        base = flat.data_ptr()
-        work = base + 4 * at
-        self._schedules = {w: work + 4 * words * i for i, w in enumerate(windows)}
-        after = base + 4 * (n + 1)
-        rows_at = base + 4 * (3 * n + 1)
-        self._args = bytes(Plan(pages.table.data_ptr(), None, None, pages.free.data_ptr(), pages.free_count.data_ptr(), None, base, after, None, rows_at,
-                                rows_at + 4 * rows, rows_at + 8 * rows, work, pages.ticket.data_ptr(), None, rows, n, pages.width, pages.n_pages, max_new,
-                                Hq // Hkv, Hkv, self.blocks, len(windows), (ctypes.c_int * PLAN_WINDOWS)(*windows)))
+        self._args = args = Plan.from_buffer_copy(sizes)
+        args.table, args.free_pages, args.free_count, args.ticket = pages.table.data_ptr(), pages.free.data_ptr(), pages.free_count.data_ptr(), pages.ticket.data_ptr()
+        args.width, args.n_pages = pages.width, pages.n_pages
+        args.work = work = flat.data_ptr()
+        args.row_start = at = work + 4 * parts[0]
+        args.served, args.pos = at + 4 * (n + 1), at + 4 * (3 * n + 1)
+        args.place, args.request = args.pos + 4 * rows, args.pos + 8 * rows
+        self._schedules = {w: work + 4 * words * i for i, w in enumerate(self.windows)}
 
 
 def page_plan(pages: PageTable, cached: Tensor, new: Tensor, rows: int, *, max_new: int, Hq: int, Hkv: int, windows: "tuple[int, ...]" = (0,),
@@ -127,13 +131,13 @@ def page_plan(pages: PageTable, cached: Tensor, new: Tensor, rows: int, *, max_n
     assert _words(cached, n) and _words(new, n)
     assert lens is None or _words(lens, n)
     assert free_left is None or _words(free_left, 1)
-    with on_device_of(pages.table):
+    with on_device_of(pages.table, cached, new, lens, free_left, status):
         if plan is None:
             plan = PagePlan(pages, rows, max_new, Hq, Hkv, windows)
         elif plan.pages is not pages or (plan.rows, plan.max_new, plan.Hq, plan.Hkv, plan.windows) != (rows, max_new, Hq, Hkv, tuple(windows)):
             raise ValueError("the plan was made for other sizes or another table")
         plan.lens = plan.own_lens if lens is None else lens
-        args = Plan.from_buffer_copy(plan._args)
+        args = Plan.from_buffer_copy(plan._args)  # a call's own
         args.cached, args.fresh, args.lens = cached.data_ptr(), new.data_ptr(), plan.lens.data_ptr()
         args.free_left = (pages.free_count if free_left is None else free_left).data_ptr()
         if status is not None:
@@ -160,7 +164,7 @@ def paged_append(qkv: Tensor, q_gain: Tensor, k_gain: Tensor, cos: Tensor, sin: 
         q_out = qkv.new_empty((rows, Hq, HEAD_DIM))
     else:
         assert q_out.dtype is _BF16 and q_out.shape == (rows, Hq, HEAD_DIM) and q_out.is_contiguous()
-    with on_device_of(qkv):
+    with on_device_of(qkv, q_gain, k_gain, cos, sin, pos, place, pages, q_out, status):
         check(cuda_library("paged_append").paged_append(
             qkv.data_ptr(), q_gain.data_ptr(), k_gain.data_ptr(), cos.data_ptr(), sin.data_ptr(), pos.data_ptr(), place.data_ptr(),
             q_out.data_ptr(), pages.data_ptr(), rows, Hq, Hkv, stride, cos.shape[0], cache.n_pages, cache.e4m3, address(status), stream()),
@@ -198,9 +202,9 @@ def paged_attention(q: Tensor, cache: PagedKVCache, plan: PagePlan, window: int 
         workspace, size = q.new_empty(plan.workspace_bytes, dtype=torch.uint8), plan.workspace_bytes
     else:
         size = workspace.numel() * workspace.element_size()
-    args = Paged(q.data_ptr(), cache.pages.data_ptr(), out.data_ptr(), workspace.data_ptr(), pages.table.data_ptr(), plan.row_start.data_ptr(),
-                 plan.fresh.data_ptr(), plan.lens.data_ptr(), work, address(status), rows, ldq, ldo, size, pages.requests, pages.width, pages.n_pages,
+    args = Paged(q.data_ptr(), cache.pages.data_ptr(), out.data_ptr(), workspace.data_ptr(), pages.table.data_ptr(), work,
+                 address(status), rows, ldq, ldo, size, pages.requests, pages.width, pages.n_pages,
                  plan.max_new, Hq, plan.Hkv, cache.e4m3, window, plan.blocks, HEAD_DIM ** -0.5 if softmax_scale is None else softmax_scale)
-    with on_device_of(q):
+    with on_device_of(q, cache.pages, pages.table, out, workspace, status):
         check(cuda_library("paged_attn").paged_attn(ctypes.byref(args), stream()), "paged_attn")
     return out

@@ -424,6 +424,28 @@ def test_pages_outside_the_pool_are_flagged_and_left_out(dtype):
         assert status.item() == 16 and torch.equal(out[1], want[1]) and out[0].isfinite().all()
 
 
+def test_operands_of_another_device_are_refused():
+    pages = ncb.PageTable(4, 2, 2 * PAGE)
+    new, other = words([1, 1]), torch.tensor([1, 1], dtype=torch.int32)
+    with pytest.raises(AssertionError):
+        ncb.page_plan(pages, pages.lens, other, 2, max_new=1, Hq=4, Hkv=2)
+    with pytest.raises(AssertionError):
+        pages.release(other)
+    plan = ncb.page_plan(pages, pages.lens, new, 2, max_new=1, Hq=4, Hkv=2)
+    cos, sin = ncb.rotary_table(2 * PAGE, 1e4, "cuda")
+    cache, gain = ncb.PagedKVCache(4, 2), torch.ones(128, device="cuda")
+    operands = [torch.zeros(2, 8 * 128, dtype=torch.bfloat16, device="cuda"), gain, gain, cos, sin, plan.pos, plan.place]
+    for i in range(len(operands)):
+        with pytest.raises(AssertionError):
+            ncb.paged_append(*operands[:i], operands[i].cpu(), *operands[i + 1:], cache, 4)
+    q = ncb.paged_append(*operands, cache, 4)
+    for bad in (dict(q=q.cpu()), dict(out=q.cpu()), dict(workspace=torch.empty(plan.workspace_bytes, dtype=torch.uint8)),
+                dict(cache=ncb.PagedKVCache(4, 2, device="cpu"))):
+        with pytest.raises(AssertionError):
+            ncb.paged_attention(**(dict(q=q, cache=cache, plan=plan) | bad))
+
+
+
 def test_calls_on_two_streams():
     """Two plans and their calls at once: each has its own workspace."""
     pool, plan, q, out = run_attention(torch.bfloat16, 8, 2, [20000, 70], [1, 10], seed=5)
