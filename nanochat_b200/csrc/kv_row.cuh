@@ -78,9 +78,9 @@ static __device__ __forceinline__ uint64_t fma2_rn(uint64_t a, uint64_t b, uint6
     return r;
 }
 
-/* x1, x2 (this lane's 8 + 8 values) -> normed, gained, rotated values rounded to bf16 and widened again. */
-static __device__ __forceinline__ void norm_rotate(float *x1, float *x2, const float *gain, const float *cs,
-                                                   const float *sn, int o) {
+/* x1, x2 (this lane's 8 + 8 values) -> normed, gained, rotated values rounded to bf16 and widened again. cos_of(q) and sin_of(q): the
+ * row's cosines and sines of dims o + q .. o + q + 3. */
+template <typename Cos, typename Sin> static __device__ __forceinline__ void norm_rotate_by(float *x1, float *x2, const float *gain, int o, Cos cos_of, Sin sin_of) {
     float ss = 0.f;
 #pragma unroll
     for (int i = 0; i < VEC; i += 2) {
@@ -95,7 +95,7 @@ static __device__ __forceinline__ void norm_rotate(float *x1, float *x2, const f
 #pragma unroll
     for (int q = 0; q < VEC; q += 4) { /* four dims and their partners at a time: 16 table values live, not 32 */
         const float4 g1 = *reinterpret_cast<const float4 *>(gain + o + q), g2 = *reinterpret_cast<const float4 *>(gain + HALF + o + q);
-        const float4 cc = *reinterpret_cast<const float4 *>(cs + o + q), s = *reinterpret_cast<const float4 *>(sn + o + q);
+        const float4 cc = cos_of(q), s = sin_of(q);
         const uint64_t g1v[2] = {pair_of(g1.x, g1.y), pair_of(g1.z, g1.w)}, g2v[2] = {pair_of(g2.x, g2.y), pair_of(g2.z, g2.w)};
         const uint64_t cv[2] = {pair_of(cc.x, cc.y), pair_of(cc.z, cc.w)}, sv[2] = {pair_of(s.x, s.y), pair_of(s.z, s.w)};
 #pragma unroll
@@ -108,6 +108,11 @@ static __device__ __forceinline__ void norm_rotate(float *x1, float *x2, const f
             x1[at] = z1.x, x1[at + 1] = z1.y, x2[at] = z2.x, x2[at + 1] = z2.y;
         }
     }
+}
+
+static __device__ __forceinline__ void norm_rotate(float *x1, float *x2, const float *gain, const float *cs, const float *sn, int o) {
+    norm_rotate_by(x1, x2, gain, o, [&](int q) { return *reinterpret_cast<const float4 *>(cs + o + q); },
+                   [&](int q) { return *reinterpret_cast<const float4 *>(sn + o + q); });
 }
 
 /* The optional value-embedding mix of a v head row (the reference's attn_prologue, model/kernels/decode.cu:482-494):
