@@ -23,7 +23,7 @@ constexpr int OWNER_WORDS = 8, START_WORDS = 4, PIECE_WORDS = 8, JOIN_WORDS = 8;
 constexpr int WHOLE_ROUNDS = 3; /* tiles are cut only where there are fewer than this many for every block */
 constexpr int WHOLE_WIDTH = 16; /* small owners are cut only where a request may have more pages than this: the launch that joins states costs more than it saves */
 
-struct Owner {
+struct alignas(16) Owner {
     int request, row, rows; /* absolute first row */
     int pos;                /* position of the first row */
     int page0, pages;       /* pages of the request that its rows see; no pages: rows that are not served, to become zeros */
@@ -31,7 +31,7 @@ struct Owner {
     int pad;
 };
 /* Where a block's part of the line begins. */
-struct Start {
+struct alignas(16) Start {
     int owner, head;
     int local; /* place within the owner, whose overhead comes first */
     int piece; /* tiles: the block's first piece; the next block's is behind its last */
@@ -106,6 +106,15 @@ struct PagedArgs { /* of paged_attn's kernels */
     float scale_log2;
 };
 
+/* A record of the schedule, not through L1. */
+template <typename Record> __device__ __forceinline__ Record of_l2(const Record *from) {
+    static_assert(sizeof(Record) % 16 == 0, "in vectors");
+    Record to;
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(Record) / 16; i++) reinterpret_cast<int4 *>(&to)[i] = __ldcg(reinterpret_cast<const int4 *>(from) + i);
+    return to;
+}
+
 /* A class's schedule as kernels read it. */
 struct Line {
     const Owner *owners;
@@ -118,7 +127,7 @@ struct Line {
     __device__ __forceinline__ Line(const PagedArgs &args, int tile) {
         const Class &c = tile ? args.caps.tile : args.caps.small;
         const int *w = args.p.work + class_at(args.caps, tile);
-        const int4 header = *reinterpret_cast<const int4 *>(w);
+        const int4 header = of_l2(reinterpret_cast<const int4 *>(w));
         owners = reinterpret_cast<const Owner *>(w + HEADER_WORDS);
         starts = reinterpret_cast<const Start *>(w + starts_at(c));
         pieces = reinterpret_cast<const Piece *>(w + pieces_at(c));
@@ -140,7 +149,7 @@ struct Walk {
     /* The next piece; false at the end. */
     __device__ __forceinline__ bool next() {
         while (left > 0) {
-            o = owners[at], head = next_head;
+            o = of_l2(owners + at), head = next_head;
             const int pages = max(o.pages, 1), from = max(local - overhead, 0), to = min(local + left - overhead, pages);
             const int used = overhead + pages - local; /* to the owner's end */
             part = from == 0 && to == pages ? -1 : 2 * block + (from == 0);

@@ -148,7 +148,10 @@ template <bool E4M3, int NT, int DEPTH> __global__ void __launch_bounds__(32 * W
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
     __syncthreads();
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    /* Behind the tile kernel of the same call there is nothing to wait for, since its blocks began after the launches before the call: these blocks fill SMs that its last ones
+     * leave idle. (What they read was written before; it is read past L1, which need not have been emptied since.) They end after it, so that whoever waits for them
+     * waits for both. */
+    if (!args.caps.tiles) asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int G = a.Hq / a.Hkv;
     const uint64_t once = policy_evict_first();
@@ -157,13 +160,10 @@ template <bool E4M3, int NT, int DEPTH> __global__ void __launch_bounds__(32 * W
     Start start = {(int)blockIdx.x / a.Hkv, (int)blockIdx.x % a.Hkv, 0, 0};
     long long left;
     if (line.whole) {
-        if (start.owner >= line.n) return;
-        left = line.overhead + max(line.owners[start.owner].pages, 1);
+        left = start.owner < line.n ? line.overhead + max(of_l2(line.owners + start.owner).pages, 1) : 0;
     } else {
-        start = line.starts[blockIdx.x];
-        left = line.all() - blockIdx.x * line.share;
-        if (left <= 0) return;
-        left = min(left, line.share);
+        start = of_l2(line.starts + blockIdx.x);
+        left = max(0ll, min(line.all() - blockIdx.x * line.share, line.share));
     }
     Walk walk(line.owners, line.n, line.overhead, start, (int)left, blockIdx.x);
     while (walk.next()) {
@@ -197,7 +197,7 @@ template <bool E4M3, int NT, int DEPTH> __global__ void __launch_bounds__(32 * W
 #pragma unroll
         for (int d = 0; d < DEPTH; d++) {
             const int i = warp + d * WARPS;
-            if (i < units) fetch(i, table[i / U::PER_PAGE]);
+            if (i < units) fetch(i, __ldcg(table + i / U::PER_PAGE));
         }
         /* ---- queries: column n = lane / 4 of tile nt is slot 8 nt + n; k slots (2t, 2t+1), (2t+8, 2t+9) of step s are dims 16 s + 2 t .. and + 8, or (E4M3)
          * 16 s + 4 t .. + 3, as the cache bytes arrive ---- */
@@ -214,7 +214,7 @@ template <bool E4M3, int NT, int DEPTH> __global__ void __launch_bounds__(32 * W
                 uint2 u[8];
 #pragma unroll
                 for (int s = 0; s < 8; s++) {
-                    u[s] = on ? *reinterpret_cast<const uint2 *>(src + 16 * s + 4 * t) : make_uint2(0u, 0u);
+                    u[s] = on ? __ldcg(reinterpret_cast<const uint2 *>(src + 16 * s + 4 * t)) : make_uint2(0u, 0u);
                     most = fmaxf(most, fmaxf(fmaxf(fabsf(__uint_as_float(u[s].x << 16)), fabsf(__uint_as_float(u[s].x & 0xffff0000u))),
                                              fmaxf(fabsf(__uint_as_float(u[s].y << 16)), fabsf(__uint_as_float(u[s].y & 0xffff0000u)))));
                 }
@@ -231,8 +231,8 @@ template <bool E4M3, int NT, int DEPTH> __global__ void __launch_bounds__(32 * W
             } else {
 #pragma unroll
                 for (int s = 0; s < 8; s++) {
-                    qb[nt][s][0] = on ? *reinterpret_cast<const uint32_t *>(src + 16 * s + 2 * t) : 0u;
-                    qb[nt][s][1] = on ? *reinterpret_cast<const uint32_t *>(src + 16 * s + 8 + 2 * t) : 0u;
+                    qb[nt][s][0] = on ? __ldcg(reinterpret_cast<const unsigned *>(src + 16 * s + 2 * t)) : 0u;
+                    qb[nt][s][1] = on ? __ldcg(reinterpret_cast<const unsigned *>(src + 16 * s + 8 + 2 * t)) : 0u;
                 }
             }
 #pragma unroll
@@ -251,7 +251,7 @@ template <bool E4M3, int NT, int DEPTH> __global__ void __launch_bounds__(32 * W
         }
         for (int i = warp; i < units; i += WARPS) {
             const int unit_pos = (page0 * U::PER_PAGE + i) * U::KEYS;
-            const int ahead = i + DEPTH * WARPS, next = ahead < units ? table[ahead / U::PER_PAGE] : 0;
+            const int ahead = i + DEPTH * WARPS, next = ahead < units ? __ldcg(table + ahead / U::PER_PAGE) : 0;
             const uint8_t *unit = place(done);
             const uint32_t unit_u = smem_u32(unit);
             if (!__all_sync(0xffffffffu, mbar_wait(bar(done), done / DEPTH & 1))) {
@@ -470,6 +470,7 @@ template <bool E4M3, int NT, int DEPTH> __global__ void __launch_bounds__(32 * W
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); /* the states were written where the next units will be copied */
         __syncthreads();
     }
+    if (args.caps.tiles) asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 constexpr int MERGE_WARPS = 8, MERGE_SLOTS = 16;
