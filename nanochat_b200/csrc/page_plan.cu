@@ -79,6 +79,7 @@ __device__ void schedule(const ncb_page_plan &a, const Requests &r, int window, 
     Owner *records = reinterpret_cast<Owner *>(work + HEADER_WORDS);
     int *before = r.page_end; /* the sums once more, for the searches below (nobody reads the pages' in this block) */
     long long weight = 0;
+    int heaviest = 0;
     for (int from = 0; from < owners; from += THREADS) {
         const int o = from + tid;
         Owner w = {};
@@ -98,12 +99,15 @@ __device__ void schedule(const ncb_page_plan &a, const Requests &r, int window, 
             w.before = (int)sum;
             records[o] = w;
             if (o < a.requests) before[o] = w.before;
+            heaviest = max(heaviest, max(w.pages, 1) + c.overhead);
         }
         weight += total;
     }
     const long long all = weight * a.kv_heads, share = min(max((all + c.blocks - 1) / c.blocks, (long long)c.least), 0x7fffffffll);
     /* Enough tiles for every block: the GPU's own order balances them, and states of cut ones (128 slots each) would cost more than that leaves. */
-    const bool whole = tile ? (long long)owners * a.kv_heads >= (long long)WHOLE_ROUNDS * c.blocks : a.width <= WHOLE_WIDTH;
+    const long long each = (long long)owners * a.kv_heads;
+    bool whole = tile ? each >= (long long)WHOLE_ROUNDS * c.blocks : a.width <= WHOLE_WIDTH;
+    if (each <= c.blocks && !whole) whole = !__syncthreads_or(heaviest > share + c.slack);
     if (tid == 0) *reinterpret_cast<int4 *>(work) = make_int4(owners, (int)weight, (int)share, whole);
     Join *joins = reinterpret_cast<Join *>(work + joins_at(c));
     if (whole || owners == 0) {

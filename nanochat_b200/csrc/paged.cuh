@@ -6,8 +6,8 @@
  * An owner weighs its pages and OVERHEAD (what a block spends on it besides); `before` are the exclusive sums of the weights, `total` their sum. The work of all
  * key/value heads, one after the other, is a line of length total * heads, and block b has the piece [b * share, (b + 1) * share) of it, wherever owners
  * begin and end: every block has the same to do, whatever the lengths are. A block leaves at most two owners unfinished, the one that it goes on with
- * from the block before it and the one that the next block goes on with: their states go to parts 2 b and 2 b + 1, and the schedule lists which parts are joined. Where tiles are so many that they fill the GPU several times over, or small owners have few pages at most, none is cut: each is a
- * block's, tiles the longest first, and no state is written or read.
+ * from the block before it and the one that the next block goes on with: their states go to parts 2 b and 2 b + 1, and the schedule lists which parts are joined. Where tiles are so many that they fill the GPU several times over, where small owners have few pages at most, or where there is a
+ * block for every owner and the longest is little longer than a block's share, none is cut: each is a block's, tiles the longest first, and no state is written or read.
  */
 #pragma once
 
@@ -21,7 +21,12 @@ constexpr int MAX_GROUP = 64;                     /* query heads per key/value h
 constexpr int HEADER_WORDS = 8;                   /* owners, total, share, whole: of a class */
 constexpr int OWNER_WORDS = 8, START_WORDS = 4, PIECE_WORDS = 8, JOIN_WORDS = 8;
 constexpr int WHOLE_ROUNDS = 3; /* tiles are cut only where there are fewer than this many for every block */
-constexpr int WHOLE_WIDTH = 16; /* small owners are cut only where a request may have more pages than this: the launch that joins states costs more than it saves */
+/* Small owners are cut only where a request may have more pages than this: the launch that joins states costs more than it saves (three users of up to 11 pages, 10 heads:
+ * 12.6 us whole, 13.5 cut; the host needs a launch less). */
+constexpr int WHOLE_WIDTH = 16;
+/* What the cut of an owner costs, in pages: its overhead once more and the states (33 requests of 5 rows behind a window of 512, 16 heads over 4: 34.0 us cut, 31.7
+ * whole; 100 of 2,000 positions: 43.4, 41.5; with no bound at all a mixed step went from 91 to 126). */
+constexpr int SMALL_SLACK = 6, TILE_SLACK = 8;
 
 struct alignas(16) Owner {
     int request, row, rows; /* absolute first row */
@@ -56,6 +61,7 @@ struct Class {
     long long owners; /* at most */
     int rows_per, slots; /* of an owner */
     int blocks, overhead, least; /* blocks that run at once; weight of an owner besides its pages; least share */
+    int slack;                   /* what an owner may weigh above a block's share and still not be cut */
 };
 struct Caps {
     Class small, tile;
@@ -71,14 +77,14 @@ static __host__ __device__ __forceinline__ Caps caps_of(int requests, long long 
         c.small.rows_per = few;
         c.small.slots = (max_fresh < few ? max_fresh : few) * group;
         c.small.owners = one_each + (c.tiles ? 0 : rows / few);
-        c.small.blocks = 3 * blocks, c.small.overhead = 2, c.small.least = 6;
+        c.small.blocks = 3 * blocks, c.small.overhead = 2, c.small.least = 6, c.small.slack = SMALL_SLACK;
     }
     if (c.tiles) {
         const long long longer = rows / (few + 1); /* requests that have tiles */
         c.tile.rows_per = TILE_SLOTS / 2 / group * 2;
         c.tile.slots = (max_fresh < c.tile.rows_per ? max_fresh : c.tile.rows_per) * group;
         c.tile.owners = rows / c.tile.rows_per + (longer < one_each ? longer : one_each);
-        c.tile.blocks = blocks, c.tile.overhead = 4, c.tile.least = 8;
+        c.tile.blocks = blocks, c.tile.overhead = 4, c.tile.least = 8, c.tile.slack = TILE_SLACK;
     }
     return c;
 }

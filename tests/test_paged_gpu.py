@@ -74,7 +74,9 @@ def check_schedule(plan, want, cached, new, rows, group, Hkv, max_new):
                 before += max(pages, 1) + overhead
             assert total == before and share == max(-(-total * Hkv // blocks), least)
             tile = per != 16 // group
-            assert whole == (len(owners) * Hkv >= 3 * blocks if tile else plan.pages.width <= 16)
+            heaviest = max(owners[:, 5].clip(1), default=0) + overhead
+            fit = len(owners) * Hkv <= blocks and heaviest <= share + (8 if tile else 6)
+            assert whole == (fit or (len(owners) * Hkv >= 3 * blocks if tile else plan.pages.width <= 16))
             if whole or len(owners) == 0:
                 assert not joins[:, 1].any()
             if whole or len(owners) == 0 or len(owners) * Hkv > 100000:
