@@ -579,13 +579,17 @@ template <bool E4M3, int NT> cudaError_t small(const CUtensorMap &map, const Pag
     const long long blocks = whole ? args.caps.small.owners * args.p.Hkv : args.caps.small.blocks;
     return whole && blocks <= args.p.blocks ? small<E4M3, NT, DEEP>(map, args, blocks, stream) : small<E4M3, NT, 1>(map, args, blocks, stream);
 }
-template <bool E4M3> cudaError_t tile(const CUtensorMap &map_q, const CUtensorMap &map_kv, const PagedArgs &args, cudaStream_t stream) {
+template <bool E4M3, bool TWICE> cudaError_t tile(const CUtensorMap &map_q, const CUtensorMap &map_kv, const PagedArgs &args, cudaStream_t stream) {
     constexpr int smem = tiles::Shape<E4M3>::SMEM;
     static std::atomic<unsigned long long> ready{0};
-    const cudaError_t rc = allow_smem(tiles::k_paged_tiles<E4M3>, smem, ready);
+    const cudaError_t rc = allow_smem(tiles::k_paged_tiles<E4M3, TWICE>, smem, ready);
     if (rc != cudaSuccess) return rc;
     const long long whole = args.caps.tile.owners * args.p.Hkv; /* blocks where no tile is cut */
-    return launch(tiles::k_paged_tiles<E4M3>, (unsigned)(whole > args.caps.tile.blocks ? whole : args.caps.tile.blocks), tiles::THREADS, smem, stream, map_q, map_kv, args);
+    return launch(tiles::k_paged_tiles<E4M3, TWICE>, (unsigned)(whole > args.caps.tile.blocks ? whole : args.caps.tile.blocks), tiles::THREADS, smem, stream, map_q, map_kv, args);
+}
+
+template <bool E4M3> cudaError_t tile(const CUtensorMap &map_q, const CUtensorMap &map_kv, const PagedArgs &args, cudaStream_t stream) {
+    return 2 * args.p.max_fresh <= args.caps.tile.rows_per ? tile<E4M3, true>(map_q, map_kv, args, stream) : tile<E4M3, false>(map_q, map_kv, args, stream);
 }
 
 /* The queries as [rows][heads][128] in boxes of 64 columns, the heads of a group and the rows of a tile. */

@@ -5,6 +5,9 @@
  * under this page's softmax, and one tile's MMAs under the other's.
  *   - one block per SM with both tiles, which share the pages in its ring: what brings a page there (TMA, or widening it) is done once for 256 slots. Each tile
  *     has softmax warps and two that issue its MMAs, which go at their own pace; a page's place is free when both tiles have used it;
+ *   - TWICE, where no request has more slots than one tile: both have the same, and every second page each. A page's chain of scores, softmax and products is long, and two
+ *     of them run side by side (33 requests of 5 rows, 16 heads over 4, window 1,024: e4m3 42.3 -> 38.9 us, bf16 31.7 -> 29.3; decided per piece instead, a prompt of 8,190
+ *     rows takes 254 us in place of 243, for the registers);
  *   - the block walks over the pieces of its part of the line (paged.cuh), the next piece's pages and queries coming under the end of this one;
  *   - the slots of a tile are packed by row and head, so that a chunk of few rows still fills the MMAs and a page is read
  *     once for all heads of its group; queries come as 3-d boxes (64 columns, the group's heads, a tile's rows);
@@ -42,8 +45,8 @@ template <bool E4M3> struct Shape {
     static constexpr int Q_BYTES = 2 * ROWS * 128, K_BYTES = 2 * KEYS * 128, V_BYTES = K_BYTES; /* Q: of a tile */
     static constexpr int STAGES = E4M3 ? 2 : 4, RAW_STAGES = E4M3 ? 4 : 0; /* raw: a page's bytes */
     static constexpr int AT_K = 2 * Q_BYTES, AT_V = AT_K + STAGES * K_BYTES, AT_RAW = AT_V + STAGES * V_BYTES, AT_SCALE = AT_RAW + RAW_STAGES * PAGE_BYTES;
-    static constexpr int SCALE_FLOATS = 3 * KEYS, AT_BARS = AT_SCALE + (E4M3 ? STAGES * SCALE_FLOATS * 4 : 0);
-    static constexpr int SMEM = 1024 + AT_BARS + 1024;
+    static constexpr int SCALE_FLOATS = 3 * KEYS, SCALES = 8, AT_BARS = AT_SCALE + (E4M3 ? SCALES * SCALE_FLOATS * 4 : 0);
+    static constexpr int AT_HALF = AT_BARS + 1024, SMEM = 1024 + AT_HALF + ROWS * 8; /* half: the second tile's maxima and sums where both have the same slots */
     static_assert(SMEM <= 227 * 1024, "one block per SM");
 };
 
@@ -132,7 +135,7 @@ __device__ __forceinline__ float query_row_to_f16(uint8_t *q, int row) {
     return __uint_as_float((uint32_t)(127 + down) << 23);
 }
 
-template <bool E4M3> __global__ void __launch_bounds__(THREADS, 1) k_paged_tiles(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_kv,
+template <bool E4M3, bool TWICE> __global__ void __launch_bounds__(THREADS, 1) k_paged_tiles(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_kv,
                                                                                             const PagedArgs args) {
     using S = Shape<E4M3>;
     constexpr int STAGES = S::STAGES, RAW = E4M3 ? S::RAW_STAGES : 1;
@@ -150,6 +153,7 @@ template <bool E4M3> __global__ void __launch_bounds__(THREADS, 1) k_paged_tiles
     auto v_free = [&](int k) { return bars + 96u + 8u * (k % STAGES); };
     auto raw_full = [&](int k) { return bars + 128u + 8u * (k % RAW); };
     auto raw_free = [&](int k) { return bars + 320u + 8u * (k % RAW); };
+    const uint32_t half_ready = bars + 352u; /* TWICE: the second tile's state */
     auto of_tile = [&](int x, int i) { return bars + 160u + 80u * x + 8u * i; };
     auto s_full = [&](int x, int c) { return of_tile(x, c & 1); };
     auto p_ready = [&](int x, int c) { return of_tile(x, 2 + (c & 1)); };
@@ -179,6 +183,7 @@ template <bool E4M3> __global__ void __launch_bounds__(THREADS, 1) k_paged_tiles
             mbar_init(q_full(x), 1);
             mbar_init(q_ready(x), TILE_WARPS);
         }
+        mbar_init(half_ready, TILE_WARPS);
         *failed = 0;
         for (int i = 0; i < 2 * MOST_ODD; i++) odd_of[i] = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -226,18 +231,22 @@ template <bool E4M3> __global__ void __launch_bounds__(THREADS, 1) k_paged_tiles
     auto load_piece = [&] { return piece_at(piece); };
     auto begin_of = [&](int pos) { return a.window > 0 ? max(0, pos + 1 - a.window) : 0; };
     /* What tile x has of a piece: its rows and its first row's position; the pages that some row of it sees, from the piece's first; the border of some row's range
-     * lies in the pages before lo and in those from hi on. */
+     * lies in the pages before lo and in those from hi on. TWICE: both tiles have the rows, and every second page each. `count` pages are the tile's. */
+    constexpr int STEP = TWICE ? 2 : 1;
     struct Tile {
-        int rows, pos, pages, lo, hi;
+        int rows, pos, pages, count, lo, hi;
     };
     auto tile_of = [&](const Piece &e, int x) {
         Tile t;
-        t.rows = max(0, min(rows_per, e.rows - x * rows_per)), t.pos = e.pos + x * rows_per;
+        const int row0 = TWICE && e.pages > 0 ? 0 : x * rows_per;
+        t.rows = max(0, min(rows_per, e.rows - row0)), t.pos = e.pos + row0;
         const int last = t.pos + t.rows - 1;
         t.pages = t.rows > 0 ? max(0, min(e.pages, last / KEYS + 1 - e.page0)) : 0;
+        t.count = TWICE ? (t.pages + 1 - x) >> 1 : t.pages;
         t.lo = (begin_of(last) - e.page0 * KEYS + KEYS - 1) / KEYS, t.hi = (t.pos + 1) / KEYS - e.page0;
         return t;
     };
+    auto takes = [&](const Tile &t, int x, int i) { return i < t.pages && (!TWICE || (i & 1) == x); };
     bool ok = true;
 
     if (warp >= PAGE_WARP) {
@@ -255,6 +264,9 @@ template <bool E4M3> __global__ void __launch_bounds__(THREADS, 1) k_paged_tiles
                         if (!in) flag(a.status, NCB_DEV_BAD_PAGE);
                         /* outside the pool: a box behind its end, zeros */
                         const int row = in ? (page * a.Hkv + e.head) * 2 * KEYS : a.n_pages * a.Hkv * 2 * KEYS, st = k % STAGES;
+                        /* TWICE: values four pages back first, since a softmax warp that has this page's scores may then wait for its values' barrier, whatever it waited for
+                         * before */
+                        if (TWICE && k >= STAGES && !(ok = wait(v_full(k), k / STAGES - 1))) break;
                         if (k >= STAGES && !(ok = wait(k_free(k), k / STAGES - 1))) break;
                         mbar_expect_tx(k_full(k), S::K_BYTES);
                         for (int j = 0; j < 2; j++) tma_load(base + S::AT_K + st * S::K_BYTES + j * KEYS * 128, &map_kv, 64 * j, row, k_full(k), keep);
@@ -312,6 +324,15 @@ template <bool E4M3> __global__ void __launch_bounds__(THREADS, 1) k_paged_tiles
                     if (!ok) break;
                     uint8_t *keys = raw + S::AT_K + k % STAGES * S::K_BYTES;
                     uint4 in4[4];
+                    float *scales = reinterpret_cast<float *>(raw + S::AT_SCALE) + k % S::SCALES * S::SCALE_FLOATS;
+                    if (lane < 16) { /* score factor, log2 of the value's scale, its scale; with the keys, so that the softmax need not wait for the values' place. Page k - 8's have been read: the
+                                    * scores of page k - 2 are there, and so the tile's buffers of two pages before that one were free */
+                        const int j = 16 * y + lane;
+                        const float vs = in ? reinterpret_cast<const float *>(page + PAGE_VS)[j] : 0.f;
+                        scales[j] = in ? reinterpret_cast<const float *>(page + PAGE_KS)[j] : 0.f;
+                        scales[KEYS + j] = fmaxf(log2_of(vs), MIN_LOG2_VSCALE);
+                        scales[2 * KEYS + j] = vs * P_SCALE;
+                    }
 #pragma unroll
                     for (int n = 0; n < 4; n++) in4[n] = *reinterpret_cast<const uint4 *>(page + page_k_chunk(16 * y + 4 * n + (lane >> 3), lane & 7)); /* 16 codes of a key */
 #pragma unroll
@@ -332,14 +353,6 @@ template <bool E4M3> __global__ void __launch_bounds__(THREADS, 1) k_paged_tiles
                     for (int n = 0; n < 4; n++) in4[n] = *reinterpret_cast<const uint4 *>(page + PAGE_V + y * 2048 + (n * 32 + lane) * 16); /* 16 positions of a dimension */
                     if (k >= STAGES && !(ok = wait_all(v_free(k), k / STAGES - 1))) break;
                     uint8_t *values = raw + S::AT_V + k % STAGES * S::V_BYTES;
-                    float *scales = reinterpret_cast<float *>(raw + S::AT_SCALE) + k % STAGES * S::SCALE_FLOATS;
-                    if (lane < 16) { /* score factor, log2 of the value's scale, its scale */
-                        const int j = 16 * y + lane;
-                        const float vs = in ? reinterpret_cast<const float *>(page + PAGE_VS)[j] : 0.f;
-                        scales[j] = in ? reinterpret_cast<const float *>(page + PAGE_KS)[j] : 0.f;
-                        scales[KEYS + j] = fmaxf(log2_of(vs), MIN_LOG2_VSCALE);
-                        scales[2 * KEYS + j] = vs * P_SCALE;
-                    }
                     const int used = (in ? e.pos + e.rows - (e.page0 + i) * KEYS : 0) - 16 * y; /* positions past the last row may hold anything: zeros */
                     if (used < 16) {
 #pragma unroll
@@ -381,12 +394,12 @@ template <bool E4M3> __global__ void __launch_bounds__(THREADS, 1) k_paged_tiles
             if (e.pages == 0) continue;
             const Tile tile = tile_of(e, x);
             if (warp < VALUE_WARP) {
-                if (tile.pages > 0) { /* its queries, when the products of the piece before have read theirs */
+                if (tile.count > 0) { /* its queries, when the products of the piece before have read theirs */
                     if (used > 0 && !(ok = wait_all(s_full(x, c - 1), (c - 1) >> 1))) break;
                     if (elect_one()) {
                         const int group = a.Hq / a.Hkv;
                         mbar_expect_tx(q_full(x), 2 * rows_per * group * 128); /* a box is whole, whatever the tile uses of it */
-                        for (int j = 0; j < 2; j++) tma_load_3d(b + x * S::Q_BYTES + j * ROWS * 128, &map_q, 64 * j, e.head * group, e.row + x * rows_per, q_full(x));
+                        for (int j = 0; j < 2; j++) tma_load_3d(b + x * S::Q_BYTES + j * ROWS * 128, &map_q, 64 * j, e.head * group, e.row + (TWICE ? 0 : x * rows_per), q_full(x));
                     }
                     __syncwarp();
                     if (!(ok = wait_all(E4M3 ? q_ready(x) : q_full(x), used))) break;
@@ -394,11 +407,11 @@ template <bool E4M3> __global__ void __launch_bounds__(THREADS, 1) k_paged_tiles
                 for (int i = 0; ok && i < e.pages; i++, k++) {
                     ok = wait_all(k_full(k), k / STAGES);
                     if (!ok) break;
-                    if (i >= tile.pages) { /* the tile has no part in the page, which only passes */
+                    if (!takes(tile, x, i)) { /* the tile has no part in the page, which only passes */
                         if (lane == 0) arrive(k_free(k));
                         continue;
                     }
-                    const int ci = c + i;
+                    const int ci = c + i / STEP;
                     ok = ci < 2 || wait_all(pv_done(x, ci), (ci - 2) >> 1); /* the buffer's probabilities have been used */
                     if (!ok) break;
                     att::fence_after();
@@ -418,12 +431,12 @@ template <bool E4M3> __global__ void __launch_bounds__(THREADS, 1) k_paged_tiles
                 for (int i = 0; ok && i < e.pages; i++, k++) {
                     ok = wait_all(v_full(k), k / STAGES);
                     if (!ok) break;
-                    if (i >= tile.pages) {
+                    if (!takes(tile, x, i)) {
                         if (lane == 0) arrive(v_free(k));
                         continue;
                     }
-                    const int ci = c + i;
-                    ok = (i > 0 || used == 0 || wait_all(o_free(x), used - 1)) && wait_all(p_ready(x, ci), ci >> 1);
+                    const int ci = c + i / STEP;
+                    ok = (i >= STEP || used == 0 || wait_all(o_free(x), used - 1)) && wait_all(p_ready(x, ci), ci >> 1);
                     if (!ok) break;
                     att::fence_after();
                     const uint32_t vs = b + S::AT_V + k % STAGES * S::V_BYTES, p = t + (ci & 1) * KEYS;
@@ -433,7 +446,7 @@ template <bool E4M3> __global__ void __launch_bounds__(THREADS, 1) k_paged_tiles
                         if (by_mma) {
 #pragma unroll
                             for (int h = 0; h < KEYS / 16; h++) /* 16 keys: 8 columns of packed probabilities */
-                                att::umma_from_tmem(t + AT_O, p + h * 8, E4M3 ? umma_desc(vs + h * 32) : att::desc_by_rows(vs + h * 2048, KEYS * 128), value, (i | h) != 0);
+                                att::umma_from_tmem(t + AT_O, p + h * 8, E4M3 ? umma_desc(vs + h * 32) : att::desc_by_rows(vs + h * 2048, KEYS * 128), value, (i / STEP | h) != 0);
                         }
                         umma_commit(pv_done(x, ci));
                         umma_commit(v_free(k));
@@ -441,27 +454,27 @@ template <bool E4M3> __global__ void __launch_bounds__(THREADS, 1) k_paged_tiles
                     __syncwarp();
                 }
             }
-            c += tile.pages, used += tile.pages > 0;
+            c += tile.count, used += tile.count > 0;
         }
         if (warp < VALUE_WARP && *failed && used > 0) mbar_wait(q_full(x), (used - 1) & 1); /* the block must not leave under a copy still in flight */
     } else { /* softmax: a thread has a slot of its tile */
         const int x = warp / TILE_WARPS, slot = tid % (32 * TILE_WARPS), first = slot & ~31;
         const uint32_t t_mine = tmem + x * TILE_COLUMNS + ((uint32_t)first << 16), o_mine = t_mine + AT_O;
-        int k = 0, c = 0, used = 0, borders = 0;
+        int k = 0, c = 0, used = 0, borders = 0, joined = 0; /* joined: pieces of which both tiles had pages */
         for (; ok && piece < pieces; piece++) {
             const Piece e = load_piece();
             const Tile tile = tile_of(e, x);
             const int G = a.Hq / a.Hkv, slots = tile.rows * G, mine = min(slot, slots - 1) / G; /* the thread's row of the tile */
             const bool on = slot < slots;
-            bf16 *out = (bf16 *)a.out + (size_t)(e.row + x * rows_per + (on ? mine : 0)) * a.ldo + (size_t)(e.head * G + (on ? slot % G : 0)) * HEAD_DIM;
+            bf16 *out = (bf16 *)a.out + (size_t)(e.row + (TWICE && e.pages > 0 ? 0 : x * rows_per) + (on ? mine : 0)) * a.ldo + (size_t)(e.head * G + (on ? slot % G : 0)) * HEAD_DIM;
             if (e.pages == 0) { /* rows that are not served */
                 if (on)
                     for (int d = 0; d < HEAD_DIM; d += 8) *reinterpret_cast<uint4 *>(out + d) = make_uint4(0u, 0u, 0u, 0u);
                 continue;
             }
-            float *part = (float *)a.workspace + parts_at(args.caps, 1) + ((size_t)max(e.part, 0) * args.caps.tile.slots + x * rows_per * G + slot) * PART;
-            if (tile.pages == 0) { /* the tile has no part in this piece: an empty state */
-                if (on && e.part >= 0) part[0] = -INFINITY, part[1] = 0.f;
+            float *part = (float *)a.workspace + parts_at(args.caps, 1) + ((size_t)max(e.part, 0) * args.caps.tile.slots + (TWICE ? 0 : x * rows_per * G) + slot) * PART;
+            if (tile.count == 0) { /* the tile has no part in this piece: an empty state */
+                if (!TWICE && on && e.part >= 0) part[0] = -INFINITY, part[1] = 0.f;
                 k += e.pages;
                 continue;
             }
@@ -482,17 +495,16 @@ template <bool E4M3> __global__ void __launch_bounds__(THREADS, 1) k_paged_tiles
             const uint64_t factor2 = att::pair_of(factor, factor);
             float m = -INFINITY;
             uint64_t sums[2] = {0, 0};
-            int page = table[0];
-            for (int i = 0; i < tile.pages; i++) {
+            int page = table[TWICE ? x : 0];
+            for (int i = TWICE ? x : 0; i < tile.pages; i += STEP) {
                 const bool in = (unsigned)page < (unsigned)a.n_pages;
-                page = i + 1 < tile.pages ? table[i + 1] : 0;
-                const int ci = c + i, ki = k + i;
+                page = i + STEP < tile.pages ? table[i + STEP] : 0;
+                const int ci = c + i / STEP, ki = k + i;
                 ok = wait_all(s_full(x, ci), ci >> 1);
-                if (ok && E4M3) ok = wait_all(v_full(ki), ki / STAGES); /* the scales come with the values, whose place is free only once P V has read this warp's probabilities */
                 if (!ok) break;
                 att::fence_after();
                 const uint32_t s_mine = t_mine + (ci & 1) * KEYS;
-                const float *scales = reinterpret_cast<const float *>(raw + S::AT_SCALE) + ki % STAGES * S::SCALE_FLOATS;
+                const float *scales = reinterpret_cast<const float *>(raw + S::AT_SCALE) + ki % S::SCALES * S::SCALE_FLOATS;
                 auto scales_at = [&](int j, int which) { return *reinterpret_cast<const ulonglong2 *>(scales + which * KEYS + j); }; /* of four keys from j */
                 const bool border = i < tile.lo || i >= tile.hi;
                 const bool plain = i >= my_lo && i < my_hi && in; /* every row of the warp sees the whole page */
@@ -581,7 +593,7 @@ template <bool E4M3> __global__ void __launch_bounds__(THREADS, 1) k_paged_tiles
                         float top = fmaxf(best[0], best[1]);
                         if (!E4M3) top *= factor;
                         const bool grown = raise && top > m;
-                        if (i > 0 && __any_sync(0xffffffffu, grown)) {
+                        if (i >= STEP && __any_sync(0xffffffffu, grown)) {
                             ok = wait_all(pv_done(x, ci - 1), (ci - 1) >> 1); /* O is complete up to the page before */
                             if (!ok) break;
                             att::fence_after();
@@ -630,10 +642,11 @@ template <bool E4M3> __global__ void __launch_bounds__(THREADS, 1) k_paged_tiles
                     ok = wait_all(looked(x), borders);
                     if (!ok) break;
                     if (odd_of[x * MOST_ODD + borders % MOST_ODD] == borders + 1) {
-                        ok = i == 0 || wait_all(pv_done(x, ci - 1), (ci - 1) >> 1); /* O is complete up to the page before */
+                        /* O is complete up to the page before, or has been read (TWICE: by the other tile's warps, it may be) */
+                        ok = i >= STEP ? wait_all(pv_done(x, ci - 1), (ci - 1) >> 1) : !TWICE || used < 2 || wait_all(o_free(x), used - 2);
                         if (!ok) break;
                         att::fence_after();
-                        multiply_seen<E4M3>(raw + S::AT_V + ki % STAGES * S::V_BYTES, s_mine, o_mine, begin - i * KEYS, last - i * KEYS + 1, i == 0);
+                        multiply_seen<E4M3>(raw + S::AT_V + ki % STAGES * S::V_BYTES, s_mine, o_mine, begin - i * KEYS, last - i * KEYS + 1, i < STEP);
                         att::fence_before();
                         __syncwarp();
                     }
@@ -641,17 +654,49 @@ template <bool E4M3> __global__ void __launch_bounds__(THREADS, 1) k_paged_tiles
                 }
                 if (lane == 0) arrive(p_ready(x, ci));
             }
-            ok = ok && wait_all(pv_done(x, c + tile.pages - 1), (c + tile.pages - 1) >> 1);
+            ok = ok && wait_all(pv_done(x, c + tile.count - 1), (c + tile.count - 1) >> 1);
             if (!ok) break;
             att::fence_after();
             const uint64_t two = att::add2(sums[0], sums[1]);
-            const float l = __uint_as_float((uint32_t)two) + __uint_as_float((uint32_t)(two >> 32));
+            float l = __uint_as_float((uint32_t)two) + __uint_as_float((uint32_t)(two >> 32)), f = 1.f, f_other = 0.f;
+            const bool join = TWICE && tile.pages > 1;
+            if (join) { /* the first tile takes the second one's state, whose O it reads in tensor memory */
+                float2 *half = reinterpret_cast<float2 *>(raw + S::AT_HALF);
+                if (x == 1) {
+                    half[slot] = make_float2(m, l);
+                    att::fence_before();
+                    __syncwarp();
+                    if (lane == 0) arrive(half_ready);
+                    k += e.pages, c += tile.count, joined++;
+                    continue;
+                }
+                ok = wait_all(half_ready, joined++);
+                if (!ok) break;
+                att::fence_after();
+                const float2 other = half[slot];
+                auto scale_of = [](float m, float l, float top) { return m == -INFINITY && l == l ? 0.f : ex2(m - top); }; /* nothing where the state holds nothing */
+                const float top = fmaxf(m, other.x);
+                f = scale_of(m, l, top), f_other = scale_of(other.x, other.y, top);
+                l = l * f + other.y * f_other, m = top;
+            }
             const float inv = l > 0.f || l != l ? __fdiv_rn(1.f, E4M3 ? l * P_SCALE : l) : 0.f;
             if (on && e.part >= 0) part[0] = m, part[1] = l;
 #pragma unroll 1
             for (int d = 0; d < HEAD_DIM; d += 32) {
                 float y[32];
                 tmem_load32(o_mine + d, y);
+                if (join) {
+#pragma unroll
+                    for (int h = 0; h < 32; h += 16) {
+                        float z[16];
+                        att::tmem_load16(o_mine + TILE_COLUMNS + d + h, z);
+#pragma unroll
+                        for (int j = 0; j < 16; j++) {
+                            const float own = f != 0.f ? y[h + j] * f : 0.f;
+                            y[h + j] = f_other != 0.f ? fmaf(z[j], f_other, own) : own;
+                        }
+                    }
+                }
                 if (!on) continue;
                 if (e.part < 0) {
                     att::store32(out + d, y, [&](int) { return inv; });
@@ -662,8 +707,11 @@ template <bool E4M3> __global__ void __launch_bounds__(THREADS, 1) k_paged_tiles
             }
             att::fence_before();
             __syncwarp();
-            if (lane == 0) arrive(o_free(x));
-            k += e.pages, c += tile.pages;
+            if (lane == 0) {
+                arrive(o_free(x));
+                if (join) arrive(o_free(1));
+            }
+            k += e.pages, c += tile.count;
         }
     }
     att::fence_before();
