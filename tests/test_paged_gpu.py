@@ -328,6 +328,17 @@ def test_attention_long_contexts_are_split(dtype, lens, new):
     run_attention(dtype, 8, 2, lens, new, seed=9)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("window", [0, 64, 700])
+@pytest.mark.parametrize("heads, lens, new", [
+    ((8, 2), [9000, 64, 700, 20, 65, 129], [20, 20, 7, 18, 17, 1]),   # 16 < slots <= 128: both tiles have them
+    ((8, 2), [3000, 40, 1500], [32, 32, 31]), ((16, 1), [900, 128, 5000, 66], [8, 3, 5, 2]), ((2, 2), [4000, 127, 128, 129], [128, 127, 60, 65])])
+def test_attention_of_few_rows(dtype, window, heads, lens, new):
+    pool, plan, q, out = run_attention(dtype, *heads, lens, new, window=window, seed=15)
+    for _ in range(3):
+        assert torch.equal(ncb.paged_attention(q, pool.cache, plan, window=window)[:sum(new)], out[:sum(new)])
+
+
 @pytest.mark.parametrize("width", [1, 40])
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_attention_of_many_small_requests(dtype, width):
