@@ -638,9 +638,10 @@ int delta_step(const ncb_delta *args, int f32, void *stream);
  *                 `rows` (NCB_DEV_BAD_LENGTH). out: table's new entries; served [requests] = fresh where served, else 0; lens
  *                 [requests] = positions held after the step; per row position, place (page * 64 + position % 64) and request;
  *                 -1, -1 for rows of requests not served and -1 in all three behind the last request.
- *                 work: for each of n_windows windows the schedule of that layer kind's paged_attn calls, page_plan_words() words,
- *                 in units that fill `blocks` blocks; a schedule holds for `group` query heads per key/value head.
- *                 ticket: one word, zero before the first call and after each. At most NCB_PLAN_REQUESTS requests, 64 heads a group.
+ *                 work (16-byte aligned): for each of n_windows windows the schedule of that layer kind's paged_attn calls, page_plan_words() words,
+ *                 for a GPU of `blocks` SMs (paged_attn_blocks()) and `group` query heads for each of kv_heads.
+ *                 ticket: one word, zero before the first call and after each. Calls on one table follow one another. At most NCB_PLAN_REQUESTS
+ *                 requests, 64 heads a group.
  *   page_release  requests with release[b] != 0 give back the pages of their lens[b] positions: their entries become -1, lens 0, the
  *                 pages go to the end of the free list. A request whose entries are not in the pool gives back none of those.
  */
@@ -670,8 +671,9 @@ int paged_append(const void *qkv, const void *q_gain, const void *k_gain, const 
 /* ---- library paged_attn ------------------------------------------------------------------------------------------------
  * Causal attention of every request's new rows over its pages, after page_plan and paged_append: the row at position p of a request
  * attends its positions (p - window, p]. q bf16 [rows][ldq], out bf16 [rows][ldo]: Hq heads of 128. `work` is
- * page_plan's schedule for this window, made with the same requests, rows, max_fresh, group and kv_heads; `blocks` of page_plan is
- * paged_attn_blocks(). Rows of requests that were not served become zeros; rows behind the last request are left as they were.
+ * page_plan's schedule for this window, made with the same requests, rows, width, max_fresh, group, kv_heads and blocks (any number of calls may read
+ * it at once). Requests of at most 16 query slots (new rows x group) and longer ones are different launches; which of them there are follows from
+ * max_fresh, so a step that only decodes should say 1. out must not overlap what is read. Rows of requests that were not served become zeros; rows behind the last request are left as they were.
  * workspace: paged_attn_workspace_bytes(), 16-byte aligned, for calls on one stream at a time. */
 typedef struct {
     const void *q, *pool;

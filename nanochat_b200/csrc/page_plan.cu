@@ -5,8 +5,8 @@
  *
  * Every block repeats the same two prefix sums over the requests (rows, then new pages) in shared memory, 16 KB for a thousand requests,
  * instead of waiting for a launch that makes them once; then the row blocks write rows and table entries, each finding its
- * request by a binary search in the sums, and one block per window cuts the attention's work into entries (paged.cuh). A step's bytes
- * are a few per row, so the launch is bound by latency: the chain of sums and searches.
+ * request by a binary search in the sums, and one block per window and class makes a schedule of the attention's work (paged.cuh). A step's bytes
+ * are a few per row, so the launch is bound by latency: the chain of sums and searches. 64 requests 8 to 10 us, 1,025 requests 12 to 15.
  */
 #include "paged.cuh"
 

@@ -6,8 +6,8 @@
  *   - one block per SM with both tiles, which share the pages in its ring: what brings a page there (TMA, or widening it) is done once for 256 slots. Each tile
  *     has softmax warps and two that issue its MMAs, which go at their own pace; a page's place is free when both tiles have used it;
  *   - TWICE, where no request has more slots than one tile: both have the same, and every second page each. A page's chain of scores, softmax and products is long, and two
- *     of them run side by side (33 requests of 5 rows, 16 heads over 4, window 1,024: e4m3 42.3 -> 38.9 us, bf16 31.7 -> 29.3; decided per piece instead, a prompt of 8,190
- *     rows takes 254 us in place of 243, for the registers);
+ *     of them run side by side (33 requests of 5 rows, 16 heads over 4, window 1,024: e4m3 42.3 -> 37.6 us, bf16 31.5 -> 28.8; behind whole contexts of up to 6,000
+ *     positions 64.3 -> 66.5 and 43.9 -> 45.8; decided per piece instead, a prompt of 8,190 rows takes 254 us in place of 243, for the registers);
  *   - the block walks over the pieces of its part of the line (paged.cuh), the next piece's pages and queries coming under the end of this one;
  *   - the slots of a tile are packed by row and head, so that a chunk of few rows still fills the MMAs and a page is read
  *     once for all heads of its group; queries come as 3-d boxes (64 columns, the group's heads, a tile's rows);
@@ -17,8 +17,12 @@
  *     probability turns out above 2^7, or a row has seen nothing yet; then the reference is raised, O rescaled and the page done again;
  *   - bf16 pages: a probability enters P V as one bf16 term, at most 2^-9 of it away: the tensor cores would need 512 cycles a page and tile in place of
  *     256 for two terms;
- *   - e4m3 pages: four warps widen a quarter of every page each to f16 in shared memory (keys in the form of a TMA box, values transposed as they lie), in place
+ *   - e4m3 pages: four warps widen a quarter of every page each (a page each: drafts 55 us for 44) to f16 in shared memory (keys in the form of a TMA box, values transposed as they lie), in place
  *     of a launch that widens a request's pages into a workspace of twice the pool's size. Queries are made f16 once per piece, each row times a power of two.
+ * Bound by the softmax warps' chain: a page of both tiles takes 2,000 cycles for bf16 pages, 1,300 of them on 64 exponentials a thread (the tensor cores need 1,000, and are 43 %
+ * busy), the rest on tensor memory and barriers; 3,000 for e4m3, where 48 scale vectors a thread, the widened pages and the MMAs' operands share the shared memory's bandwidth.
+ * 8,190 rows of a prompt, 16 heads over 4, bf16: 243 us, 1,130 TFLOP/s (280 us where such calls fill seconds, and the card's power is bounded); 512 rows behind 16,384 positions,
+ * 32 over 8: bf16 138 us, e4m3 200.
  * A position that a row does not see must not reach it: scores are masked, values are looked at in the pages that the border of some row crosses (three
  * at either end at most), and a page that holds one that is not finite there is multiplied row by row over the positions seen.
  */

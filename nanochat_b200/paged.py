@@ -59,7 +59,7 @@ def _layout(requests: int, rows: int, max_new: int, Hq: int, Hkv: int, windows: 
 class PageTable:
     """Which pages the requests hold, for the pools of every layer, on the device: `table` int32 (requests, width), -1 where there is
     none; `lens` int32 (requests,), positions held; `free` int32 (n_pages,) and `free_count` int32 (1,), the pages nobody holds.
-    A page belongs to one request. At most 8,192 requests."""
+    A page belongs to one request. At most 8,192 requests. What changes a table (page_plan, release) is one call after the other."""
 
     def __init__(self, n_pages: int, requests: int, max_len: int, device: "torch.device | str" = "cuda", table: Tensor | None = None,
                  lens: Tensor | None = None, free: Tensor | None = None, free_count: Tensor | None = None):
@@ -123,7 +123,7 @@ def page_plan(pages: PageTable, cached: Tensor, new: Tensor, rows: int, *, max_n
     """One step's bookkeeping in one launch: request b holds cached[b] positions and adds new[b] (int32 (requests,) on the device, 0 for
     a request that idles), whose rows follow the rows of request b - 1 in the step's `rows` rows. Takes the new pages off pages.free
     into pages.table, and returns the step's PagePlan (`plan`: one of the same sizes to fill again, as a captured step does).
-    max_new: an upper bound of new known to the host. lens: where the new lengths go (default: the plan's own; pages.lens, or
+    max_new: an upper bound of new known to the host (a step that only decodes says 1: longer requests cost attention a launch). lens: where the new lengths go (default: the plan's own; pages.lens, or
     `cached` itself, to advance them in place); free_left: where the count of free pages goes (default: pages.free_count).
     Requests are served in order. One that would need more pages than are left (NCB_DEV_NO_PAGES), or that passes the table's
     width, max_new or `rows` or has a negative length (NCB_DEV_BAD_LENGTH), is not served: it keeps its length, and its rows are idle in the operators below."""
@@ -178,7 +178,7 @@ def paged_attention(q: Tensor, cache: PagedKVCache, plan: PagePlan, window: int 
     row at position p attends (p - window, p], or [0, p] with window 0. q (rows, Hq, 128) bf16, heads contiguous, row stride free;
     `window` is one that the plan was made with. Rows of requests that the plan did not serve become zeros; rows behind the last
     request are left as they were in `out`. workspace: uint8, plan.workspace_bytes long, for calls that no other stream overlaps
-    (default: a new one). Returns out (rows, Hq, 128) bf16."""
+    (default: a new one). `out` overlaps nothing that is read. Returns out (rows, Hq, 128) bf16."""
     rows, Hq, pages = plan.rows, plan.Hq, plan.pages
     shape = (rows, Hq, HEAD_DIM)
     ldq, head, step = q.stride()
