@@ -108,8 +108,8 @@ class PagePlan:
         flat = pages.table.new_empty(sum(parts))
         self.work, self.row_start, self.fresh, self.lens, self.pos, self.place, self.request = flat.split_with_sizes(parts)
         self.own_lens = self.lens
+        self.filled = False  # by page_plan: before, the schedules are whatever was in memory
         self._args = args = Plan.from_buffer_copy(sizes)
-        args.table, args.free_pages, args.free_count, args.ticket = pages.table.data_ptr(), pages.free.data_ptr(), pages.free_count.data_ptr(), pages.ticket.data_ptr()
         args.width, args.n_pages = pages.width, pages.n_pages
         args.work = work = flat.data_ptr()
         args.row_start = at = work + 4 * parts[0]
@@ -138,11 +138,13 @@ def page_plan(pages: PageTable, cached: Tensor, new: Tensor, rows: int, *, max_n
             raise ValueError("the plan was made for other sizes or another table")
         plan.lens = plan.own_lens if lens is None else lens
         args = Plan.from_buffer_copy(plan._args)  # a call's own
+        args.table, args.free_pages, args.free_count, args.ticket = pages.table.data_ptr(), pages.free.data_ptr(), pages.free_count.data_ptr(), pages.ticket.data_ptr()
         args.cached, args.fresh, args.lens = cached.data_ptr(), new.data_ptr(), plan.lens.data_ptr()
         args.free_left = (pages.free_count if free_left is None else free_left).data_ptr()
         if status is not None:
             args.status = status.data_ptr()
         check(cuda_library("page_plan").page_plan(ctypes.byref(args), stream()), "page_plan")
+        plan.filled = True
     return plan
 
 
@@ -189,6 +191,8 @@ def paged_attention(q: Tensor, cache: PagedKVCache, plan: PagePlan, window: int 
     work = plan._schedules.get(window)
     if work is None:
         raise ValueError(f"the plan has schedules for windows {plan.windows}, not {window}")
+    if not plan.filled:
+        raise ValueError("page_plan has not filled this plan")
     if cache.n_pages != pages.n_pages:
         raise ValueError(f"a pool of {cache.n_pages} pages, a table over {pages.n_pages}")
     if out is None:

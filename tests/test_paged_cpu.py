@@ -110,8 +110,13 @@ def test_python_faces_refuse():
     cache, q = ncb.PagedKVCache(16, 2, device="cpu"), torch.zeros(8, 8, 128, dtype=torch.bfloat16)
     with pytest.raises(ValueError):
         ncb.paged_attention(q, cache, plan, window=64)
-    with pytest.raises(ValueError):
+    with pytest.raises(ValueError, match="not filled"):
+        ncb.paged_attention(q, cache, plan)
+    plan.filled = True
+    with pytest.raises(ValueError, match="15 pages"):
         ncb.paged_attention(q, ncb.PagedKVCache(15, 2, device="cpu"), plan)
+    with pytest.raises(AssertionError):  # not on a GPU
+        ncb.paged_attention(q, cache, plan)
     with pytest.raises(AssertionError):
         ncb.paged_attention(q[:7], cache, plan)
     with pytest.raises(AssertionError):

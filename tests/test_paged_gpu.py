@@ -437,6 +437,27 @@ def test_pages_outside_the_pool_are_flagged_and_left_out(dtype):
         assert status.item() == 16 and torch.equal(out[1], want[1]) and out[0].isfinite().all()
 
 
+@pytest.mark.parametrize("dtype, many", [(torch.float8_e4m3fn, 300_000), (torch.bfloat16, 150_000)])
+def test_pages_behind_4_gib(dtype, many):
+    """The same step in the last pages of a pool of 5 GB and in a small one: the same bits."""
+    gen = torch.Generator().manual_seed(31)
+    new, rows, Hq, Hkv = words([1, 300, 20]), 321, 4, 1
+    qkv = torch.randn(rows, (Hq + 2 * Hkv) * 128, generator=gen).bfloat16().cuda()
+    gain = torch.ones(128, device="cuda")
+    cos, sin = ncb.rotary_table(512, 1e4, "cuda")
+    found = []
+    for n_pages in (12, many):
+        pages = ncb.PageTable(n_pages, 3, 512)
+        pages.free.copy_(torch.arange(n_pages, dtype=torch.int32))  # the last ones first
+        cache = ncb.PagedKVCache(n_pages, Hkv, dtype)
+        plan = ncb.page_plan(pages, pages.lens, new, rows, max_new=300, Hq=Hq, Hkv=Hkv, lens=pages.lens)
+        q = ncb.paged_append(qkv, gain, gain, cos, sin, plan.pos, plan.place, cache, Hq)
+        found.append(ncb.paged_attention(q, cache, plan))
+        assert pages.table[0, 0].item() == n_pages - 1
+        del cache
+    assert torch.equal(*found) and found[0].isfinite().all()
+
+
 def test_operands_of_another_device_are_refused():
     pages = ncb.PageTable(4, 2, 2 * PAGE)
     new, other = words([1, 1]), torch.tensor([1, 1], dtype=torch.int32)
