@@ -74,9 +74,11 @@ static __host__ __device__ __forceinline__ Caps caps_of(int requests, long long 
     const int few = SMALL_SLOTS / group; /* 0: even one row has too many slots */
     c.smalls = few > 0 && rows > 0, c.tiles = max_fresh > few && rows > few;
     if (c.smalls) {
-        c.small.rows_per = few;
-        c.small.slots = (max_fresh < few ? max_fresh : few) * group;
-        c.small.owners = one_each + (c.tiles ? 0 : rows / few);
+        /* Without tiles, rows of requests that are not served, however many, are in owners of no more slots than the others', which the kernel is chosen for. */
+        const int per = max_fresh < few ? max_fresh : few;
+        c.small.rows_per = per;
+        c.small.slots = per * group;
+        c.small.owners = c.tiles ? one_each : (rows + one_each * (per - 1)) / per;
         c.small.blocks = 3 * blocks, c.small.overhead = 2, c.small.least = 6, c.small.slack = SMALL_SLACK;
     }
     if (c.tiles) {

@@ -592,7 +592,7 @@ template <bool E4M3, bool TWICE> cudaError_t tile(const CUtensorMap &map_q, cons
 }
 
 template <bool E4M3> cudaError_t tile(const CUtensorMap &map_q, const CUtensorMap &map_kv, const PagedArgs &args, cudaStream_t stream) {
-    return 2 * args.p.max_fresh <= args.caps.tile.rows_per ? tile<E4M3, true>(map_q, map_kv, args, stream) : tile<E4M3, false>(map_q, map_kv, args, stream);
+    return args.p.max_fresh <= args.caps.tile.rows_per / 2 ? tile<E4M3, true>(map_q, map_kv, args, stream) : tile<E4M3, false>(map_q, map_kv, args, stream);
 }
 
 /* The queries as [rows][heads][128] in boxes of 64 columns, the heads of a group and the rows of a tile. */

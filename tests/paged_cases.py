@@ -61,7 +61,8 @@ def schedule(words, requests, rows, max_new, group, sms):
     classes = []
     tiles = max_new > few and rows > few
     if few and rows:
-        classes.append((few, each + (0 if tiles else rows // few), 3 * sms, 2, 6, 0))
+        per = min(few, max_new)
+        classes.append((per, each if tiles else (rows + each * (per - 1)) // per, 3 * sms, 2, 6, 0))
     if tiles:
         per = 128 // group * 2
         classes.append((per, rows // per + min(rows // (few + 1), each), sms, 4, 8, 4 * sms))

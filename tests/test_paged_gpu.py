@@ -63,7 +63,7 @@ def check_schedule(plan, want, cached, new, rows, group, Hkv, max_new):
                 row0 = row - want["row_start"][b]
                 assert 0 < count <= per and row0 % per == 0
                 if group <= 16 and max_new > 16 // group:  # both classes
-                    assert (want["row_start"][b + 1] - want["row_start"][b] > 16 // group) == (per != 16 // group) or want["row_start"][b + 1] > rows
+                    assert (want["row_start"][b + 1] - want["row_start"][b] > 16 // group) == (overhead == 4) or want["row_start"][b + 1] > rows
                 cover += range(row, row + count)
                 if want["fresh"][b]:
                     first, last = cached[b] + row0, cached[b] + row0 + count - 1
@@ -73,7 +73,7 @@ def check_schedule(plan, want, cached, new, rows, group, Hkv, max_new):
                 assert at == before
                 before += max(pages, 1) + overhead
             assert total == before and share == max(-(-total * Hkv // blocks), least)
-            tile = per != 16 // group
+            tile = overhead == 4
             heaviest = max(owners[:, 5].clip(1), default=0) + overhead
             fit = len(owners) * Hkv <= blocks and heaviest <= share + (8 if tile else 6)
             assert whole == (fit or (len(owners) * Hkv >= 3 * blocks if tile else plan.pages.width <= 16))
@@ -240,13 +240,13 @@ class Pool:
     """A pool whose every byte that no request wrote is NaN (codes and scales too), with requests of lens positions, of which a plan
     (`plan`, with spare rows behind the last) has just added the last new."""
 
-    def __init__(self, dtype, Hq, Hkv, lens, new, window=0, seed=0, tail=3, free=None, width=1):
+    def __init__(self, dtype, Hq, Hkv, lens, new, window=0, seed=0, tail=3, free=None, width=1, bound=1):
         gen = torch.Generator().manual_seed(seed)
         held = [-(-n // PAGE) for n in lens]
         self.n_pages, self.rows = sum(held) + 3, sum(new)
         cached, status = [n - k for n, k in zip(lens, new)], words([0])
         self.pages, *_ = make_table(cached, self.n_pages, max(held + [1, width - 1]) + 1, free=free, seed=seed)
-        self.plan = ncb.page_plan(self.pages, words(cached), words(new), self.rows + tail, max_new=max(new + [1]), Hq=Hq, Hkv=Hkv, windows=(window,),
+        self.plan = ncb.page_plan(self.pages, words(cached), words(new), self.rows + tail, max_new=max(new + [bound]), Hq=Hq, Hkv=Hkv, windows=(window,),
                                   status=status)
         self.status = status.item()
         self.table = table = self.pages.table.tolist()
@@ -279,9 +279,9 @@ class Pool:
         self.cache.write(row, args[0][0], args[1][0], args[0][1], args[1][1], start=start)
 
 
-def run_attention(dtype, Hq, Hkv, lens, new, window=0, seed=0, tail=3, scale_q=1.0, width=1):
+def run_attention(dtype, Hq, Hkv, lens, new, window=0, seed=0, tail=3, scale_q=1.0, width=1, bound=1):
     """The last new[b] of request b's lens[b] positions attend. Checks every row against 64 bits; returns the pieces."""
-    pool = Pool(dtype, Hq, Hkv, lens, new, window, seed, tail, width=width)
+    pool = Pool(dtype, Hq, Hkv, lens, new, window, seed, tail, width=width, bound=bound)
     rows, plan, status = pool.rows, pool.plan, words([0])
     q = (pool.q.float() * scale_q).bfloat16()
     out = torch.full((rows + tail, Hq, 128), 7.0, dtype=torch.bfloat16, device="cuda")
@@ -337,6 +337,15 @@ def test_attention_of_few_rows(dtype, window, heads, lens, new):
     pool, plan, q, out = run_attention(dtype, *heads, lens, new, window=window, seed=15)
     for _ in range(3):
         assert torch.equal(ncb.paged_attention(q, pool.cache, plan, window=window)[:sum(new)], out[:sum(new)])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("bound", [32, 33, 1000, 2 ** 30, 2 ** 31 - 1])
+def test_attention_under_bounds_that_nobody_reaches(dtype, bound):
+    run_attention(dtype, 8, 2, [300, 64, 1000, 129], [1, 0, 30, 5], seed=17, bound=bound)
+    run_attention(dtype, 8, 2, [300, 64], [1, 1], seed=17, bound=bound)
+    if bound >= 1000:
+        run_attention(dtype, 8, 2, [300, 900], [1, 700], seed=17, bound=bound)
 
 
 @pytest.mark.parametrize("width", [1, 40])
@@ -435,6 +444,25 @@ def test_pages_outside_the_pool_are_flagged_and_left_out(dtype):
         status = words([0])
         out = ncb.paged_attention(q, pool.cache, plan, status=status)
         assert status.item() == 16 and torch.equal(out[1], want[1]) and out[0].isfinite().all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("bound", [1, 20, 100])
+def test_requests_past_the_bound_get_zeros(dtype, bound):
+    gen = torch.Generator().manual_seed(33)
+    wide, Hq, Hkv = torch.randn(301, 12 * 128, generator=gen).bfloat16().cuda(), 8, 2
+    gain, (cos, sin) = torch.ones(128, device="cuda"), ncb.rotary_table(512, 1e4, "cuda")
+    found = []
+    for new, take in (([bound, 200, 1], slice(0, bound + 201)), ([bound, 0, 1], [*range(bound), bound + 200])):
+        pages, status = ncb.PageTable(20, 3, 512), words([0])
+        cache, qkv = ncb.PagedKVCache(20, Hkv, dtype), wide[take].contiguous()
+        plan = ncb.page_plan(pages, pages.lens, words(new), len(qkv), max_new=bound, Hq=Hq, Hkv=Hkv, lens=pages.lens, status=status)
+        q = ncb.paged_append(qkv, gain, gain, cos, sin, plan.pos, plan.place, cache, Hq)
+        found.append(ncb.paged_attention(q, cache, plan, out=torch.full_like(q, 7.0)))
+        assert status.item() == (4 if new[1] else 0) and plan.fresh.tolist() == [bound, 0, 1]
+    assert not found[0][bound:bound + 200].any()
+    got = torch.cat([found[0][:bound], found[0][bound + 200:]]).float()
+    assert torch.allclose(got, found[1].float(), rtol=2 ** -7, atol=2 ** -10)
 
 
 @pytest.mark.parametrize("dtype, many", [(torch.float8_e4m3fn, 300_000), (torch.bfloat16, 150_000)])
