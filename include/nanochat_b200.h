@@ -685,7 +685,7 @@ typedef struct {
     float scale;
 } ncb_paged;
 int paged_attn_blocks(void);
-long long paged_attn_workspace_bytes(int requests, long long rows, int max_fresh, int Hq, int Hkv, int blocks);
+long long paged_attn_workspace_bytes(int requests, long long rows, int width, int max_fresh, int Hq, int Hkv, int blocks); /* 0: none is needed */
 int paged_attn(const ncb_paged *args, void *stream);
 
 /* ---- GEMMs around an fp32 residual stream (ncb_gemm_rs above) ------------------------------------------------

@@ -22,7 +22,7 @@ constexpr int HEADER_WORDS = 8;                   /* owners, total, share, whole
 constexpr int OWNER_WORDS = 8, START_WORDS = 4, PIECE_WORDS = 8, JOIN_WORDS = 8;
 constexpr int WHOLE_ROUNDS = 3; /* tiles are cut only where there are fewer than this many for every block */
 /* Small owners are cut only where a request may have more pages than this: the launch that joins states costs more than it saves (three users of up to 11 pages, 10 heads:
- * 12.6 us whole, 13.5 cut; the host needs a launch less). */
+ * 8.7 us whole, 12.4 cut; the host needs a launch and a workspace less). */
 constexpr int WHOLE_WIDTH = 16;
 /* What the cut of an owner costs, in pages: its overhead once more and the states (33 requests of 5 rows behind a window of 512, 16 heads over 4: 34.0 us cut, 31.7
  * whole; 100 of 2,000 positions: 43.4, 41.5; with no bound at all a mixed step went from 91 to 126). */

@@ -29,7 +29,7 @@ namespace {
 
 using namespace paged;
 
-constexpr int WARPS = 4, DEEP = 3;
+constexpr int FEW = 4, MANY = 12; /* warps of a block, of which three or one are on an SM */
 constexpr float LOG2_E = 1.4426950408889634f;
 constexpr float P_SCALE = 256.f; /* keeps small folded probabilities among f16's normal numbers; an exact power of two */
 constexpr float MIN_LOG2_VSCALE = -64.f;
@@ -37,13 +37,13 @@ constexpr int BOX_ROWS = 32, BOX_BYTES = BOX_ROWS * 128;
 
 /* What a warp fetches and consumes at a time: an e4m3 page, or half a bf16 page (four boxes of 32 rows x 64 columns, swizzled: keys' columns 0 .. 63
  * and 64 .. 127, then the values'). */
-template <bool E4M3, int DEPTH> struct Unit {
+template <bool E4M3, int WARPS> struct Unit {
     static constexpr int KEYS = E4M3 ? PAGE_TOKENS : PAGE_TOKENS / 2, PER_PAGE = PAGE_TOKENS / KEYS;
     static constexpr int BYTES = E4M3 ? PAGE_BYTES : 4 * BOX_BYTES;
-    static constexpr int PLACES = WARPS * DEPTH, BLOCKS = DEPTH == 1 ? 3 : 1; /* blocks per SM */
-    static constexpr int SMEM = 1024 + PLACES * BYTES; /* 1024: swizzled boxes are aligned by hand */
+    static constexpr int BLOCKS = MANY / WARPS;
+    static constexpr int SMEM = 1024 + WARPS * BYTES; /* 1024: swizzled boxes are aligned by hand */
     static_assert(BLOCKS * (SMEM + 2048) <= 228 * 1024, "blocks per SM");
-    static_assert(WARPS * SMALL_SLOTS * PART * 4 <= PLACES * BYTES, "the warps' states lie where their units were");
+    static_assert(SMALL_SLOTS * PART * 4 <= BYTES, "a warp's states lie where its unit was");
 };
 
 __device__ __forceinline__ float lg2(float x) {
@@ -131,21 +131,20 @@ template <bool E4M3> __device__ __forceinline__ bool strange_values(const uint8_
     return __any_sync(0xffffffffu, strange);
 }
 
-template <bool E4M3, int NT, int DEPTH> __global__ void __launch_bounds__(32 * WARPS, (Unit<E4M3, DEPTH>::BLOCKS)) k_paged_small(const __grid_constant__ CUtensorMap map, const PagedArgs args) {
-    using U = Unit<E4M3, DEPTH>;
+template <bool E4M3, int NT, int WARPS> __global__ void __launch_bounds__(32 * WARPS, MANY / WARPS) k_paged_small(const __grid_constant__ CUtensorMap map, const PagedArgs args) {
+    using U = Unit<E4M3, WARPS>;
     constexpr int TILES = U::KEYS / 16; /* of 16 keys */
     extern __shared__ __align__(128) uint8_t raw[];
-    __shared__ __align__(8) uint64_t bars[U::PLACES];
+    __shared__ __align__(8) uint64_t bars[WARPS];
     __shared__ int failed;
     __shared__ float state_m[WARPS][8 * NT], state_l[WARPS][8 * NT];
     const ncb_paged &a = args.p;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     uint8_t *smem = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
-    /* the warp's n-th unit has its place n % DEPTH */
-    auto place = [&](uint32_t n) { return smem + (warp * DEPTH + n % DEPTH) * U::BYTES; };
-    auto bar = [&](uint32_t n) { return smem_u32(bars + warp * DEPTH + n % DEPTH); };
+    const uint8_t *unit = smem + warp * U::BYTES;
+    const uint32_t unit_u = smem_u32(unit), bar = smem_u32(bars + warp);
     if (tid == 0) {
-        for (int w = 0; w < U::PLACES; w++) mbar_init(smem_u32(bars + w), 1);
+        for (int w = 0; w < WARPS; w++) mbar_init(smem_u32(bars + w), 1);
         failed = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -158,50 +157,46 @@ template <bool E4M3, int NT, int DEPTH> __global__ void __launch_bounds__(32 * W
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int G = a.Hq / a.Hkv;
     const uint64_t once = policy_evict_first();
-    uint32_t begun = 0, done = 0, there = 0; /* units of this warp; which places hold one that is in the pool */
+    uint32_t loads = 0; /* of this warp so far: the parity of its barrier */
+    bool there = false; /* the unit in its place is in the pool */
     const Line line(args, 0);
     Start start = {(int)blockIdx.x / a.Hkv, (int)blockIdx.x % a.Hkv, 0, 0};
     long long left;
-    if (line.whole) {
-        left = start.owner < line.n ? line.overhead + max(of_l2(line.owners + start.owner).pages, 1) : 0;
+    const bool whole = WARPS > FEW || line.whole; /* one owner, to its end */
+    if (whole) {
+        left = WARPS > FEW || start.owner < line.n ? 1 << 30 : 0;
     } else {
         start = of_l2(line.starts + blockIdx.x);
         left = max(0ll, min(line.all() - blockIdx.x * line.share, line.share));
     }
     Walk walk(line.owners, line.n, line.overhead, start, (int)left, blockIdx.x);
     while (walk.next()) {
+        if (WARPS > FEW && start.owner >= line.n) break; /* looked at only here: the owner's record comes beside the header */
         const Owner &e = walk.o;
         const int kvh = walk.head, page0 = e.page0 + walk.page0, part_at = walk.part;
         const int slots = e.rows * G, units = (walk.page1 - walk.page0) * U::PER_PAGE, first_pos = e.pos, last_pos = e.pos + e.rows - 1;
         const long long first_row = e.row;
         const int *table = a.table + (size_t)e.request * a.width + page0;
         auto begin_of = [&](int pos) { return a.window > 0 ? max(0, pos + 1 - a.window) : 0; }; /* the first position that the row at pos sees */
-        /* The piece's unit i, of this page, into the warp's next place; a page that is not in the pool is left out. */
+        /* The piece's unit i, of this page, into the warp's place; a page that is not in the pool is left out. */
         auto fetch = [&](int i, int page) {
-            const bool in = (unsigned)page < (unsigned)a.n_pages;
-            const uint32_t to = smem_u32(place(begun)), full = bar(begun), bit = 1u << begun % DEPTH;
-            there = in ? there | bit : there & ~bit;
-            begun++;
+            there = (unsigned)page < (unsigned)a.n_pages;
             if (lane != 0) return;
-            if (!in) {
+            if (!there) {
                 flag(a.status, NCB_DEV_BAD_PAGE);
-                att::arrive(full);
+                att::arrive(bar);
                 return;
             }
-            mbar_expect_tx(full, U::BYTES);
+            mbar_expect_tx(bar, U::BYTES);
             if (E4M3) {
-                bulk_load_once(to, (const uint8_t *)a.pool + ((size_t)page * a.Hkv + kvh) * PAGE_BYTES, PAGE_BYTES, full, once);
+                bulk_load_once(unit_u, (const uint8_t *)a.pool + ((size_t)page * a.Hkv + kvh) * PAGE_BYTES, PAGE_BYTES, bar, once);
             } else {
                 const int row = (page * a.Hkv + kvh) * 2 * PAGE_TOKENS + i % U::PER_PAGE * BOX_ROWS;
 #pragma unroll
-                for (int x = 0; x < 4; x++) tma_load(to + x * BOX_BYTES, &map, 64 * (x & 1), row + (x >> 1) * PAGE_TOKENS, full, once);
+                for (int x = 0; x < 4; x++) tma_load(unit_u + x * BOX_BYTES, &map, 64 * (x & 1), row + (x >> 1) * PAGE_TOKENS, bar, once);
             }
         };
-#pragma unroll
-        for (int d = 0; d < DEPTH; d++) {
-            const int i = warp + d * WARPS;
-            if (i < units) fetch(i, __ldcg(table + i / U::PER_PAGE));
-        }
+        if (warp < units) fetch(warp, __ldcg(table + warp / U::PER_PAGE));
         /* ---- queries: column n = lane / 4 of tile nt is slot 8 nt + n; k slots (2t, 2t+1), (2t+8, 2t+9) of step s are dims 16 s + 2 t .. and + 8, or (E4M3)
          * 16 s + 4 t .. + 3, as the cache bytes arrive ---- */
         uint32_t qb[NT][8][2];
@@ -254,17 +249,13 @@ template <bool E4M3, int NT, int DEPTH> __global__ void __launch_bounds__(32 * W
         }
         for (int i = warp; i < units; i += WARPS) {
             const int unit_pos = (page0 * U::PER_PAGE + i) * U::KEYS;
-            const int ahead = i + DEPTH * WARPS, next = ahead < units ? __ldcg(table + ahead / U::PER_PAGE) : 0;
-            const uint8_t *unit = place(done);
-            const uint32_t unit_u = smem_u32(unit);
-            if (!__all_sync(0xffffffffu, mbar_wait(bar(done), done / DEPTH & 1))) {
+            const int next = i + WARPS < units ? __ldcg(table + (i + WARPS) / U::PER_PAGE) : 0;
+            if (!__all_sync(0xffffffffu, mbar_wait(bar, loads++ & 1))) {
                 if (lane == 0) flag(a.status, NCB_DEV_WAIT_TIMEOUT), failed = 1;
-                for (uint32_t n = done; n < begun; n++) mbar_wait(bar(n), n / DEPTH & 1); /* nobody leaves under a copy */
+                mbar_wait(bar, loads - 1 & 1); /* nobody leaves under a copy */
                 break;
             }
-            const bool in = there >> done % DEPTH & 1;
-            done++;
-            if (in && unit_pos <= last_pos && unit_pos + U::KEYS > any_from) {
+            if (there && unit_pos <= last_pos && unit_pos + U::KEYS > any_from) {
                 /* ---- scores: tile k, element x: key row lane / 4 (x < 2) or 8 + lane / 4 of the tile, slots 2 t + x % 2. Rows are keys in order, or (E4M3) rows r and
                  * 8 + r keys 4 (r / 2) + r % 2 and 2 more, so that their transposes meet four consecutive bytes of V^T ---- */
                 const int row[2] = {E4M3 ? 4 * (g >> 1) + (g & 1) : g, E4M3 ? 4 * (g >> 1) + (g & 1) + 2 : g + 8};
@@ -431,7 +422,7 @@ template <bool E4M3, int NT, int DEPTH> __global__ void __launch_bounds__(32 * W
                 }
             }
             __syncwarp(); /* every lane has read the unit */
-            if (ahead < units) fetch(ahead, next);
+            if (i + WARPS < units) fetch(i + WARPS, next);
         }
         __syncthreads(); /* every warp has finished with its units: their states go there */
         float *mine = reinterpret_cast<float *>(smem) + warp * 8 * NT * PART;
@@ -469,7 +460,7 @@ template <bool E4M3, int NT, int DEPTH> __global__ void __launch_bounds__(32 * W
                 *reinterpret_cast<float4 *>(part + 4 + 4 * lane) = x;
             }
         }
-        if (failed) break; /* the same for all: written before the barriers */
+        if (failed || whole) break; /* failed: the same for all, written before the barriers */
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); /* the states were written where the next units will be copied */
         __syncthreads();
     }
@@ -568,19 +559,19 @@ template <typename Kernel> cudaError_t allow_smem(Kernel kernel, int bytes, std:
     return rc;
 }
 
-template <bool E4M3, int NT, int DEPTH> cudaError_t small(const CUtensorMap &map, const PagedArgs &args, long long blocks, cudaStream_t stream) {
-    constexpr int smem = Unit<E4M3, DEPTH>::SMEM;
+template <bool E4M3, int NT, int WARPS> cudaError_t small(const CUtensorMap &map, const PagedArgs &args, long long blocks, cudaStream_t stream) {
+    constexpr int smem = Unit<E4M3, WARPS>::SMEM;
     static std::atomic<unsigned long long> ready{0};
-    const cudaError_t rc = allow_smem(k_paged_small<E4M3, NT, DEPTH>, smem, ready);
+    const cudaError_t rc = allow_smem(k_paged_small<E4M3, NT, WARPS>, smem, ready);
     if (rc != cudaSuccess) return rc;
-    return launch(k_paged_small<E4M3, NT, DEPTH>, (unsigned)blocks, 32 * WARPS, smem, stream, map, args);
+    return launch(k_paged_small<E4M3, NT, WARPS>, (unsigned)blocks, 32 * WARPS, smem, stream, map, args);
 }
-/* Where owners are whole and there is at most one for every SM, a warp has three units in flight instead of one: the call is then as long as its longest owner, not as
- * its bytes (three users of up to 700 positions, 10 heads, bf16: 13.5 -> 12.6 us). */
+/* Where owners are whole and there is at most one for every SM, it has twelve warps in place of four: the call is then as long as its longest owner, not as
+ * its bytes (three users of up to 700 positions, 10 heads, bf16: 8.7 us; four warps 13.5, four with three units under way each 12.0). */
 template <bool E4M3, int NT> cudaError_t small(const CUtensorMap &map, const PagedArgs &args, cudaStream_t stream) {
     const bool whole = args.p.width <= WHOLE_WIDTH;
     const long long blocks = whole ? args.caps.small.owners * args.p.Hkv : args.caps.small.blocks;
-    return whole && blocks <= args.p.blocks ? small<E4M3, NT, DEEP>(map, args, blocks, stream) : small<E4M3, NT, 1>(map, args, blocks, stream);
+    return whole && blocks <= args.p.blocks ? small<E4M3, NT, MANY>(map, args, blocks, stream) : small<E4M3, NT, FEW>(map, args, blocks, stream);
 }
 template <bool E4M3, bool TWICE> cudaError_t tile(const CUtensorMap &map_q, const CUtensorMap &map_kv, const PagedArgs &args, cudaStream_t stream) {
     constexpr int smem = tiles::Shape<E4M3>::SMEM;
@@ -611,9 +602,10 @@ extern "C" {
 
 int paged_attn_blocks(void) { return 148; } /* SMs */
 
-long long paged_attn_workspace_bytes(int requests, long long rows, int max_fresh, int Hq, int Hkv, int blocks) {
-    if (Hq <= 0 || Hkv <= 0 || Hq % Hkv || !sizes_ok(requests, rows, max_fresh, Hq / Hkv, Hkv, blocks)) return -1;
-    return 4 * workspace_floats(caps_of(requests, rows, max_fresh, Hq / Hkv, blocks));
+long long paged_attn_workspace_bytes(int requests, long long rows, int width, int max_fresh, int Hq, int Hkv, int blocks) {
+    if (Hq <= 0 || Hkv <= 0 || Hq % Hkv || width <= 0 || !sizes_ok(requests, rows, max_fresh, Hq / Hkv, Hkv, blocks)) return -1;
+    const Caps caps = caps_of(requests, rows, max_fresh, Hq / Hkv, blocks);
+    return caps.tiles || width > WHOLE_WIDTH ? 4 * workspace_floats(caps) : 0;
 }
 
 int paged_attn(const ncb_paged *args, void *stream) {
@@ -623,10 +615,12 @@ int paged_attn(const ncb_paged *args, void *stream) {
     if (!sizes_ok(a.requests, a.rows, a.max_fresh, a.Hq / a.Hkv, a.Hkv, a.blocks)) return NCB_ERR_ARG;
     if (a.ldq < (long long)a.Hq * HEAD_DIM || a.ldo < (long long)a.Hq * HEAD_DIM) return NCB_ERR_ARG;
     if (a.rows == 0) return NCB_OK;
-    if (!a.q || !a.pool || !a.out || !a.workspace || !a.table || !a.work) return NCB_ERR_ARG;
+    if (!a.q || !a.pool || !a.out || !a.table || !a.work) return NCB_ERR_ARG;
     if (((uintptr_t)a.q | (uintptr_t)a.pool | (uintptr_t)a.out | (uintptr_t)a.workspace | (uintptr_t)a.work) % 16 || a.ldq % 8 || a.ldo % 8) return NCB_ERR_ALIGN;
     PagedArgs p = {a, caps_of(a.requests, a.rows, a.max_fresh, a.Hq / a.Hkv, a.blocks), a.scale * LOG2_E};
-    if (a.workspace_bytes < paged_attn_workspace_bytes(a.requests, a.rows, a.max_fresh, a.Hq, a.Hkv, a.blocks)) return NCB_ERR_WORKSPACE;
+    const long long needed = paged_attn_workspace_bytes(a.requests, a.rows, a.width, a.max_fresh, a.Hq, a.Hkv, a.blocks);
+    if (needed > 0 && !a.workspace) return NCB_ERR_ARG;
+    if (a.workspace_bytes < needed) return NCB_ERR_WORKSPACE;
     const long long key_rows = (long long)a.n_pages * a.Hkv * 2 * PAGE_TOKENS;
     if (key_rows > 0x7fffffffll || p.caps.tile.owners * a.Hkv > 0x7fffffffll || p.caps.small.owners * a.Hkv > 0x7fffffffll) return NCB_ERR_UNSUPPORTED;
     CUtensorMap map = {}, map_q = {};

@@ -120,7 +120,7 @@ SIGNATURES = {
     "paged_append": {"paged_append": ([c_ptr] * 9 + [c_ll, c_int, c_int, c_ll, c_int, c_int, c_int, c_ptr, c_ptr], c_int)},
     "paged_attn": {
         "paged_attn_blocks": ([], c_int),
-        "paged_attn_workspace_bytes": ([c_int, c_ll] + [c_int] * 4, c_ll),
+        "paged_attn_workspace_bytes": ([c_int, c_ll] + [c_int] * 5, c_ll),
         "paged_attn": ([c_ptr, c_ptr], c_int),
     },
     "kv_append": {

@@ -23,6 +23,7 @@ from .native import PLAN_WINDOWS, Paged, Plan, check, cuda_library, pointer, str
 
 _READY = contextlib.nullcontext()
 _INT, _BF16, _F32 = torch.int32, torch.bfloat16, torch.float32
+_SCALE = HEAD_DIM ** -0.5
 
 
 def on_device_of(*operands: "Tensor | None"):
@@ -42,14 +43,14 @@ def address(t: "Tensor | None") -> "int | None":
 
 
 @functools.lru_cache(maxsize=1024)
-def _layout(requests: int, rows: int, max_new: int, Hq: int, Hkv: int, windows: "tuple[int, ...]"):
+def _layout(requests: int, rows: int, width: int, max_new: int, Hq: int, Hkv: int, windows: "tuple[int, ...]"):
     """Of plans of this size: (blocks, words of a window's schedule, bytes of a workspace, words of the plan's parts, the native arguments that only
     sizes decide); words -1: none."""
     assert Hkv > 0 and Hq > 0 and Hq % Hkv == 0 and 0 < len(windows) <= PLAN_WINDOWS and len(set(windows)) == len(windows)
     attn = cuda_library("paged_attn")
     blocks = attn.paged_attn_blocks()
     words = cuda_library("page_plan").page_plan_words(requests, rows, max_new, Hq // Hkv, Hkv, blocks)
-    workspace = attn.paged_attn_workspace_bytes(requests, rows, max_new, Hq, Hkv, blocks)
+    workspace = attn.paged_attn_workspace_bytes(requests, rows, width, max_new, Hq, Hkv, blocks)
     parts = [words * len(windows), requests + 1, requests, requests, rows, rows, rows]
     sizes = Plan(rows=rows, requests=requests, max_fresh=max_new, group=Hq // Hkv, kv_heads=Hkv, blocks=blocks, n_windows=len(windows),
                  windows=(ctypes.c_int * PLAN_WINDOWS)(*windows))
@@ -102,7 +103,7 @@ class PagePlan:
     def __init__(self, pages: PageTable, rows: int, max_new: int, Hq: int, Hkv: int, windows: "tuple[int, ...]" = (0,)):
         self.pages, self.rows, self.max_new, self.Hq, self.Hkv, self.windows = pages, rows, max_new, Hq, Hkv, tuple(windows)
         n = pages.requests
-        self.blocks, words, self.workspace_bytes, parts, sizes = _layout(n, rows, max_new, Hq, Hkv, self.windows)
+        self.blocks, words, self.workspace_bytes, parts, sizes = _layout(n, rows, pages.width, max_new, Hq, Hkv, self.windows)
         if words < 0:
             raise ValueError(f"no plan for {n} requests, {rows} rows, at most {max_new} a request, {Hq} heads over {Hkv}")
         flat = pages.table.new_empty(sum(parts))
@@ -202,13 +203,14 @@ def paged_attention(q: Tensor, cache: PagedKVCache, plan: PagePlan, window: int 
         assert out.dtype is _BF16 and out.shape == shape and step == 1 and (head == HEAD_DIM or Hq == 1)
         if rows <= 1:
             ldo = Hq * HEAD_DIM
-    if workspace is None:
-        workspace, size = q.new_empty(plan.workspace_bytes, dtype=torch.uint8), plan.workspace_bytes
-    else:
+    size = plan.workspace_bytes
+    if workspace is not None:
         size = workspace.numel() * workspace.element_size()
-    args = Paged(q.data_ptr(), cache.pages.data_ptr(), out.data_ptr(), workspace.data_ptr(), pages.table.data_ptr(), work,
+    elif size:
+        workspace = q.new_empty(size, dtype=torch.uint8)
+    args = Paged(q.data_ptr(), cache.pages.data_ptr(), out.data_ptr(), address(workspace), pages.table.data_ptr(), work,
                  address(status), rows, ldq, ldo, size, pages.requests, pages.width, pages.n_pages,
-                 plan.max_new, Hq, plan.Hkv, cache.e4m3, window, plan.blocks, HEAD_DIM ** -0.5 if softmax_scale is None else softmax_scale)
+                 plan.max_new, Hq, plan.Hkv, cache.e4m3, window, plan.blocks, _SCALE if softmax_scale is None else softmax_scale)
     with on_device_of(q, cache.pages, pages.table, out, workspace, status):
         check(cuda_library("paged_attn").paged_attn(ctypes.byref(args), stream()), "paged_attn")
     return out

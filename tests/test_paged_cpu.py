@@ -79,8 +79,9 @@ def test_schedules_have_a_size_for_every_head_group():
     words, size = native.cuda_library("page_plan").page_plan_words, native.cuda_library("paged_attn").paged_attn_workspace_bytes
     for group in (1, 3, 4, 12, 64):
         assert words(64, 64, 1, group, 8, 296) > 64 * 8
-        assert size(64, 64, 1, group * 8, 8, 296) > 0
-    assert words(64, 64, 1, 65, 8, 296) == -1 and size(64, 64, 1, 9, 8, 296) == -1
+        assert size(64, 64, 40, 1, group * 8, 8, 296) > 0
+        assert (size(64, 64, 16, 1, group * 8, 8, 296) == 0) == (group <= 16)  # few pages, one row each: no owner is cut
+    assert words(64, 64, 1, 65, 8, 296) == -1 and size(64, 64, 40, 1, 9, 8, 296) == -1 and size(64, 64, 0, 1, 8, 8, 296) == -1
     assert words(8192, 1 << 26, 1 << 20, 64, 1, 296) > 0
 
 

@@ -501,7 +501,7 @@ def test_operands_of_another_device_are_refused():
         with pytest.raises(AssertionError):
             ncb.paged_append(*operands[:i], operands[i].cpu(), *operands[i + 1:], cache, 4)
     q = ncb.paged_append(*operands, cache, 4)
-    for bad in (dict(q=q.cpu()), dict(out=q.cpu()), dict(workspace=torch.empty(plan.workspace_bytes, dtype=torch.uint8)),
+    for bad in (dict(q=q.cpu()), dict(out=q.cpu()), dict(workspace=torch.empty(64, dtype=torch.uint8)),
                 dict(cache=ncb.PagedKVCache(4, 2, device="cpu"))):
         with pytest.raises(AssertionError):
             ncb.paged_attention(**(dict(q=q, cache=cache, plan=plan) | bad))
