@@ -59,6 +59,32 @@ struct Requests { /* shared memory, one value a request each */
     int *owner_end;          /* schedule blocks: inclusive sum of owners */
 };
 
+/* How long the last block has work if owners are whole and the heaviest go first: no less than the heaviest, nor than what some block has of the n heaviest, ceil(n
+ * heads / blocks) of them at least, for n down to each of sixteen weights; and hardly more. heaviest: of the thread's owners, which it has written itself. */
+__device__ long long longest_whole(const Owner *records, int owners, int heads, const Class &c, int heaviest) {
+    constexpr int STEPS = 16;
+    __shared__ int most, count[STEPS], least[STEPS];
+    const int tid = threadIdx.x;
+    if (tid == 0) most = 1;
+    if (tid < STEPS) count[tid] = 0, least[tid] = 0x7fffffff;
+    __syncthreads();
+    heaviest = __reduce_max_sync(0xffffffffu, heaviest);
+    if (tid % 32 == 0) atomicMax(&most, heaviest);
+    __syncthreads();
+    const int top = most;
+    for (int o = tid; o < owners; o += THREADS) {
+        const int weight = max(records[o].pages, 1) + c.overhead, step = ((long long)weight * STEPS - 1) / top;
+        atomicAdd(count + step, 1);
+        atomicMin(least + step, weight);
+    }
+    __syncthreads();
+    long long last = top, n = 0;
+#pragma unroll 1
+    for (int i = STEPS - 1; i >= 0; i--)
+        if (count[i]) n += count[i], last = max(last, (n * heads + c.blocks - 1) / c.blocks * least[i]);
+    return last;
+}
+
 /* The schedule of one window's attention, of one class of requests (paged.cuh). */
 __device__ void schedule(const ncb_page_plan &a, const Requests &r, int window, int tile, int *work, long long *sums) {
     const Caps caps = caps_of(a.requests, a.rows, a.max_fresh, a.group, a.blocks);
@@ -104,10 +130,12 @@ __device__ void schedule(const ncb_page_plan &a, const Requests &r, int window, 
         weight += total;
     }
     const long long all = weight * a.kv_heads, share = min(max((all + c.blocks - 1) / c.blocks, (long long)c.least), 0x7fffffffll);
-    /* Enough tiles for every block: the GPU's own order balances them, and states of cut ones (128 slots each) would cost more than that leaves. */
     const long long each = (long long)owners * a.kv_heads;
     bool whole = tile ? each >= (long long)WHOLE_ROUNDS * c.blocks : a.width <= WHOLE_WIDTH;
-    if (each <= c.blocks && !whole) whole = !__syncthreads_or(heaviest > share + c.slack);
+    if (!whole && (tile || each <= c.blocks)) { /* small owners have a block each, or are cut */
+        const long long last = longest_whole(records, owners, a.kv_heads, c, heaviest);
+        whole = last <= share + c.slack;
+    }
     if (tid == 0) *reinterpret_cast<int4 *>(work) = make_int4(owners, (int)weight, (int)share, whole);
     Join *joins = reinterpret_cast<Join *>(work + joins_at(c));
     if (whole || owners == 0) {

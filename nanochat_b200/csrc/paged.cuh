@@ -6,8 +6,9 @@
  * An owner weighs its pages and OVERHEAD (what a block spends on it besides); `before` are the exclusive sums of the weights, `total` their sum. The work of all
  * key/value heads, one after the other, is a line of length total * heads, and block b has the piece [b * share, (b + 1) * share) of it, wherever owners
  * begin and end: every block has the same to do, whatever the lengths are. A block leaves at most two owners unfinished, the one that it goes on with
- * from the block before it and the one that the next block goes on with: their states go to parts 2 b and 2 b + 1, and the schedule lists which parts are joined. Where tiles are so many that they fill the GPU several times over, where small owners have few pages at most, or where there is a
- * block for every owner and the longest is little longer than a block's share, none is cut: each is a block's, tiles the longest first, and no state is written or read.
+ * from the block before it and the one that the next block goes on with: their states go to parts 2 b and 2 b + 1, and the schedule lists which
+ * parts are joined. Where the blocks would not be done much later with whole owners, the longest first, or where small owners have few pages at most, none is cut:
+ * each is a block's, and no state is written or read.
  */
 #pragma once
 
@@ -20,13 +21,14 @@ constexpr int SMALL_SLOTS = 16, TILE_SLOTS = 256; /* query slots of a block of t
 constexpr int MAX_GROUP = 64;                     /* query heads per key/value head */
 constexpr int HEADER_WORDS = 8;                   /* owners, total, share, whole: of a class */
 constexpr int OWNER_WORDS = 8, START_WORDS = 4, PIECE_WORDS = 8, JOIN_WORDS = 8;
-constexpr int WHOLE_ROUNDS = 3; /* tiles are cut only where there are fewer than this many for every block */
+constexpr int WHOLE_ROUNDS = 8; /* tiles are cut only where there are fewer than this many for every block */
 /* Small owners are cut only where a request may have more pages than this: the launch that joins states costs more than it saves (three users of up to 11 pages, 10 heads:
  * 8.7 us whole, 12.4 cut; the host needs a launch and a workspace less). */
 constexpr int WHOLE_WIDTH = 16;
-/* What the cut of an owner costs, in pages: its overhead once more and the states (33 requests of 5 rows behind a window of 512, 16 heads over 4: 34.0 us cut, 31.7
- * whole; 100 of 2,000 positions: 43.4, 41.5; with no bound at all a mixed step went from 91 to 126). */
-constexpr int SMALL_SLACK = 6, TILE_SLACK = 8;
+/* What cutting owners costs a block, in pages: an overhead more, and the states. Small owners and few rows (33 requests of 5 behind a window of 512, 16 heads over 4: 34.0 us cut,
+ * 31.7 whole; of 2,048: 55.5, 62; 100 of one row, 2,000 positions: 43.4, 41.5); full tiles (bf16, 16 heads over 4: prompts of 2,500, 4,096 and 6,000 rows 54.8, 101 and 179 us cut, 50.8, 78
+ * and 154 whole; eight of 512 behind 4,000 positions, 32 over 8, e4m3, whose last round would be half empty: 398, 426; a mixed step 91, 126). */
+constexpr int SMALL_SLACK = 6, FEW_SLACK = 8, TILE_SLACK = 20;
 
 struct alignas(16) Owner {
     int request, row, rows; /* absolute first row */
@@ -86,7 +88,7 @@ static __host__ __device__ __forceinline__ Caps caps_of(int requests, long long 
         c.tile.rows_per = TILE_SLOTS / 2 / group * 2;
         c.tile.slots = (max_fresh < c.tile.rows_per ? max_fresh : c.tile.rows_per) * group;
         c.tile.owners = rows / c.tile.rows_per + (longer < one_each ? longer : one_each);
-        c.tile.blocks = blocks, c.tile.overhead = 4, c.tile.least = 8, c.tile.slack = TILE_SLACK;
+        c.tile.blocks = blocks, c.tile.overhead = 4, c.tile.least = 8, c.tile.slack = max_fresh <= c.tile.rows_per / 2 ? FEW_SLACK : TILE_SLACK;
     }
     return c;
 }

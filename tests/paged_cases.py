@@ -65,7 +65,7 @@ def schedule(words, requests, rows, max_new, group, sms):
         classes.append((per, each if tiles else (rows + each * (per - 1)) // per, 3 * sms, 2, 6, 0))
     if tiles:
         per = 128 // group * 2
-        classes.append((per, rows // per + min(rows // (few + 1), each), sms, 4, 8, 4 * sms))
+        classes.append((per, rows // per + min(rows // (few + 1), each), sms, 4, 8, 9 * sms))
     found, at = [], 0
     for per, most, blocks, overhead, least, room in classes:
         n = int(w[at])
@@ -79,6 +79,18 @@ def schedule(words, requests, rows, max_new, group, sms):
         at = pieces + 8 * room
     assert at == len(w)
     return found
+
+
+def last_whole(weights, heads, blocks):
+    """A bound of the last block's work if owners are whole: the heaviest, and what some block has of all owners of at least a weight."""
+    top, last, n = int(weights.max()), int(weights.max()), 0
+    steps = (weights.astype(np.int64) * 16 - 1) // top
+    for i in range(15, -1, -1):
+        here = weights[steps == i]
+        n += len(here)
+        if len(here):
+            last = max(last, -(-n * heads // blocks) * int(here.min()))
+    return last
 
 
 def pieces(owners, heads, blocks, overhead, total, share):

@@ -74,9 +74,9 @@ def check_schedule(plan, want, cached, new, rows, group, Hkv, max_new):
                 before += max(pages, 1) + overhead
             assert total == before and share == max(-(-total * Hkv // blocks), least)
             tile = overhead == 4
-            heaviest = max(owners[:, 5].clip(1), default=0) + overhead
-            fit = len(owners) * Hkv <= blocks and heaviest <= share + (8 if tile else 6)
-            assert whole == (fit or (len(owners) * Hkv >= 3 * blocks if tile else plan.pages.width <= 16))
+            slack = 6 if not tile else 8 if max_new <= per // 2 else 20
+            fit = len(owners) == 0 or (tile or len(owners) * Hkv <= blocks) and plain.last_whole(owners[:, 5].clip(1) + overhead, Hkv, blocks) <= share + slack
+            assert whole == (fit or (len(owners) * Hkv >= 8 * blocks if tile else plan.pages.width <= 16))
             if whole or len(owners) == 0:
                 assert not joins[:, 1].any()
             if whole or len(owners) == 0 or len(owners) * Hkv > 100000:
