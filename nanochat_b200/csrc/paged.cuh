@@ -7,7 +7,7 @@
  * key/value heads, one after the other, is a line of length total * heads, and block b has the piece [b * share, (b + 1) * share) of it, wherever owners
  * begin and end: every block has the same to do, whatever the lengths are. A block leaves at most two owners unfinished, the one that it goes on with
  * from the block before it and the one that the next block goes on with: their states go to parts 2 b and 2 b + 1, and the schedule lists which
- * parts are joined. Where the blocks would not be done much later with whole owners, the longest first, or where small owners have few pages at most, none is cut:
+ * parts are joined. Where the blocks would not be done much later with whole owners, from the last (a request's longest) on, or where small owners have few pages at most, none is cut:
  * each is a block's, and no state is written or read.
  */
 #pragma once
