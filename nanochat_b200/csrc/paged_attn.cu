@@ -98,6 +98,19 @@ __device__ __forceinline__ void bulk_load_once(uint32_t dst, const void *src, ui
                  ::"r"(dst), "l"(src), "r"(bytes), "r"(bar), "l"(policy) : "memory");
 }
 
+/* Past L1, of what nobody writes while the kernel runs: free to move, unlike __ldcg, which cost the stream of pages 1 us of 60. (Not before the wait for the launches before:
+ * the addresses come from the schedule, which is read behind it.) */
+__device__ __forceinline__ uint2 two_words_of_l2(const bf16 *at) {
+    uint2 x;
+    asm("ld.global.cg.v2.u32 {%0, %1}, [%2];" : "=r"(x.x), "=r"(x.y) : "l"(at));
+    return x;
+}
+template <typename Word> __device__ __forceinline__ uint32_t word_of_l2(const Word *at) {
+    uint32_t x;
+    asm("ld.global.cg.u32 %0, [%1];" : "=r"(x) : "l"(at));
+    return x;
+}
+
 /* What a state (m, l) counts relative to 2^top: nothing where it holds nothing. */
 __device__ __forceinline__ float scale_of(float m, float l, float top) { return m == -INFINITY && l == l ? 0.f : ex2(m - top); }
 
@@ -196,7 +209,7 @@ template <bool E4M3, int NT, int WARPS> __global__ void __launch_bounds__(32 * W
                 for (int x = 0; x < 4; x++) tma_load(unit_u + x * BOX_BYTES, &map, 64 * (x & 1), row + (x >> 1) * PAGE_TOKENS, bar, once);
             }
         };
-        if (warp < units) fetch(warp, __ldcg(table + warp / U::PER_PAGE));
+        if (warp < units) fetch(warp, (int)word_of_l2(table + warp / U::PER_PAGE));
         /* ---- queries: column n = lane / 4 of tile nt is slot 8 nt + n; k slots (2t, 2t+1), (2t+8, 2t+9) of step s are dims 16 s + 2 t .. and + 8, or (E4M3)
          * 16 s + 4 t .. + 3, as the cache bytes arrive ---- */
         uint32_t qb[NT][8][2];
@@ -212,7 +225,7 @@ template <bool E4M3, int NT, int WARPS> __global__ void __launch_bounds__(32 * W
                 uint2 u[8];
 #pragma unroll
                 for (int s = 0; s < 8; s++) {
-                    u[s] = on ? __ldcg(reinterpret_cast<const uint2 *>(src + 16 * s + 4 * t)) : make_uint2(0u, 0u);
+                    u[s] = on ? two_words_of_l2(src + 16 * s + 4 * t) : make_uint2(0u, 0u);
                     most = fmaxf(most, fmaxf(fmaxf(fabsf(__uint_as_float(u[s].x << 16)), fabsf(__uint_as_float(u[s].x & 0xffff0000u))),
                                              fmaxf(fabsf(__uint_as_float(u[s].y << 16)), fabsf(__uint_as_float(u[s].y & 0xffff0000u)))));
                 }
@@ -229,8 +242,8 @@ template <bool E4M3, int NT, int WARPS> __global__ void __launch_bounds__(32 * W
             } else {
 #pragma unroll
                 for (int s = 0; s < 8; s++) {
-                    qb[nt][s][0] = on ? __ldcg(reinterpret_cast<const unsigned *>(src + 16 * s + 2 * t)) : 0u;
-                    qb[nt][s][1] = on ? __ldcg(reinterpret_cast<const unsigned *>(src + 16 * s + 8 + 2 * t)) : 0u;
+                    qb[nt][s][0] = on ? word_of_l2(src + 16 * s + 2 * t) : 0u;
+                    qb[nt][s][1] = on ? word_of_l2(src + 16 * s + 8 + 2 * t) : 0u;
                 }
             }
 #pragma unroll
@@ -249,7 +262,7 @@ template <bool E4M3, int NT, int WARPS> __global__ void __launch_bounds__(32 * W
         }
         for (int i = warp; i < units; i += WARPS) {
             const int unit_pos = (page0 * U::PER_PAGE + i) * U::KEYS;
-            const int next = i + WARPS < units ? __ldcg(table + (i + WARPS) / U::PER_PAGE) : 0;
+            const int next = i + WARPS < units ? (int)word_of_l2(table + (i + WARPS) / U::PER_PAGE) : 0;
             if (!__all_sync(0xffffffffu, mbar_wait(bar, loads++ & 1))) {
                 if (lane == 0) flag(a.status, NCB_DEV_WAIT_TIMEOUT), failed = 1;
                 mbar_wait(bar, loads - 1 & 1); /* nobody leaves under a copy */
