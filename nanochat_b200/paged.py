@@ -160,9 +160,10 @@ def paged_append(qkv: Tensor, q_gain: Tensor, k_gain: Tensor, cos: Tensor, sin: 
     if rows <= 1:
         stride = width  # of a single row it says nothing
     assert _words(pos, rows) and _words(place, rows)
-    assert cos.shape == sin.shape and cos.shape[1] == HEAD_DIM // 2 and cos.is_contiguous() and sin.is_contiguous()
+    length, half = table = cos.shape
+    assert half == HEAD_DIM // 2 and sin.shape == table and cos.is_contiguous() and sin.is_contiguous()
     assert q_gain.dtype is k_gain.dtype is cos.dtype is sin.dtype is _F32
-    assert q_gain.shape == k_gain.shape == (HEAD_DIM,) and q_gain.is_contiguous() and k_gain.is_contiguous()
+    assert q_gain.numel() == k_gain.numel() == HEAD_DIM and q_gain.is_contiguous() and k_gain.is_contiguous()
     if q_out is None:
         q_out = qkv.new_empty((rows, Hq, HEAD_DIM))
     else:
@@ -170,7 +171,7 @@ def paged_append(qkv: Tensor, q_gain: Tensor, k_gain: Tensor, cos: Tensor, sin: 
     with on_device_of(qkv, q_gain, k_gain, cos, sin, pos, place, pages, q_out, status):
         check(cuda_library("paged_append").paged_append(
             qkv.data_ptr(), q_gain.data_ptr(), k_gain.data_ptr(), cos.data_ptr(), sin.data_ptr(), pos.data_ptr(), place.data_ptr(),
-            q_out.data_ptr(), pages.data_ptr(), rows, Hq, Hkv, stride, cos.shape[0], cache.n_pages, cache.e4m3, address(status), stream()),
+            q_out.data_ptr(), pages.data_ptr(), rows, Hq, Hkv, stride, length, cache.n_pages, cache.e4m3, address(status), stream()),
             "paged_append")
     return q_out
 
