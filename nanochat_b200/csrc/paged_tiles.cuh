@@ -268,9 +268,9 @@ template <bool E4M3, bool TWICE> __global__ void __launch_bounds__(THREADS, 1) k
                         if (!in) flag(a.status, NCB_DEV_BAD_PAGE);
                         /* outside the pool: a box behind its end, zeros */
                         const int row = in ? (page * a.Hkv + e.head) * 2 * KEYS : a.n_pages * a.Hkv * 2 * KEYS, st = k % STAGES;
-                        /* TWICE: values four pages back first, since a softmax warp that has this page's scores may then wait for its values' barrier, whatever it waited for
-                         * before */
-                        if (TWICE && k >= STAGES && !(ok = wait(v_full(k), k / STAGES - 1))) break;
+                        /* The values of the page before in this place first: a softmax warp that has this page's scores may wait for its values' barrier next, by parity, and need not
+                         * have waited for that page's (the other tile's, it may be, whose owner has no rows for this one) */
+                        if (k >= STAGES && !(ok = wait(v_full(k), k / STAGES - 1))) break;
                         if (k >= STAGES && !(ok = wait(k_free(k), k / STAGES - 1))) break;
                         mbar_expect_tx(k_full(k), S::K_BYTES);
                         for (int j = 0; j < 2; j++) tma_load(base + S::AT_K + st * S::K_BYTES + j * KEYS * 128, &map_kv, 64 * j, row, k_full(k), keep);
