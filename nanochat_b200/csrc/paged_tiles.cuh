@@ -393,6 +393,7 @@ template <bool E4M3, bool TWICE> __global__ void __launch_bounds__(THREADS, 1) k
         const int x = __shfl_sync(0xffffffffu, (warp - SCORE_WARP) & 1, 0);
         const uint32_t t = __shfl_sync(0xffffffffu, tmem, 0) + x * TILE_COLUMNS, b = __shfl_sync(0xffffffffu, base, 0);
         int k = 0, c = 0, used = 0, borders = 0; /* pages, pages of the tile, pieces that the tile had pages of, pages that its border crossed */
+        int asked = 0, issued = 0;               /* copies of queries, pages whose MMAs this warp has begun */
         for (; ok && piece < pieces; piece++) {
             const Piece e = load_piece();
             if (e.pages == 0) continue;
@@ -405,6 +406,7 @@ template <bool E4M3, bool TWICE> __global__ void __launch_bounds__(THREADS, 1) k
                         mbar_expect_tx(q_full(x), 2 * rows_per * group * 128); /* a box is whole, whatever the tile uses of it */
                         for (int j = 0; j < 2; j++) tma_load_3d(b + x * S::Q_BYTES + j * ROWS * 128, &map_q, 64 * j, e.head * group, e.row + (TWICE ? 0 : x * rows_per), q_full(x));
                     }
+                    asked = used + 1;
                     __syncwarp();
                     if (!(ok = wait_all(E4M3 ? q_ready(x) : q_full(x), used))) break;
                 }
@@ -429,6 +431,7 @@ template <bool E4M3, bool TWICE> __global__ void __launch_bounds__(THREADS, 1) k
                         umma_commit(s_full(x, ci));
                         umma_commit(k_free(k));
                     }
+                    issued = ci + 1;
                     __syncwarp();
                 }
             } else {
@@ -455,12 +458,15 @@ template <bool E4M3, bool TWICE> __global__ void __launch_bounds__(THREADS, 1) k
                         umma_commit(pv_done(x, ci));
                         umma_commit(v_free(k));
                     }
+                    issued = ci + 1;
                     __syncwarp();
                 }
             }
             c += tile.count, used += tile.count > 0;
         }
-        if (warp < VALUE_WARP && *failed && used > 0) mbar_wait(q_full(x), (used - 1) & 1); /* the block must not leave under a copy still in flight */
+        /* the block must not leave under a copy or MMAs still in flight: after a failed wait they may be, else they have long ended */
+        if (asked > 0) mbar_wait(q_full(x), (asked - 1) & 1);
+        if (issued > 0) mbar_wait(warp < VALUE_WARP ? s_full(x, issued - 1) : pv_done(x, issued - 1), ((issued - 1) >> 1) & 1);
     } else { /* softmax: a thread has a slot of its tile */
         const int x = warp / TILE_WARPS, slot = tid % (32 * TILE_WARPS), first = slot & ~31;
         const uint32_t t_mine = tmem + x * TILE_COLUMNS + ((uint32_t)first << 16), o_mine = t_mine + AT_O;
