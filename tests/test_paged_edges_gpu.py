@@ -1,4 +1,4 @@
-"""Edges of the paged operators on the GPU: owners of one tile between owners of two.
+"""Edges of the paged operators on the GPU: owners of one tile between owners of two, keys that are not finite.
 Tolerances as in test_paged_gpu.py."""
 
 import pytest
@@ -6,7 +6,7 @@ import torch
 
 import nanochat_b200 as ncb
 from tests import paged_cases as plain
-from tests.test_paged_gpu import DTYPES, run_attention
+from tests.test_paged_gpu import DTYPES, PAGE, Pool, run_attention, words
 
 pytestmark = pytest.mark.gpu
 
@@ -26,3 +26,33 @@ def test_owners_of_one_tile_between_owners_of_two(dtype, window, seed):
         assert not whole and plan.max_new > 32  # cut, and two different tiles
     for _ in range(20):
         assert torch.equal(ncb.paged_attention(q, pool.cache, plan, window=window)[:sum(new)], out[:sum(new)])
+
+
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("new", [3, 20, 150])  # the small kernel; both tiles with the rows; rows of their own
+def test_keys_that_are_not_finite_reach_their_rows(dtype, new, value):
+    """A key in one of two inner pages with such a value in one dimension, at each position of eight: rows whose score is NaN or infinite are NaN, as
+    in 64 bits, others leave the key out (a score of minus infinity) or have another head."""
+    if dtype != torch.bfloat16 and value == float("inf"):
+        pytest.skip("a code of e4m3 is never infinite")
+    n, dim = 400 + new, 5
+    pool = Pool(dtype, 8, 2, [n], [new], seed=new)
+    page, kept = pool.pages.table[0].tolist(), pool.cache.pages.clone()
+    for at in [128 + j for j in range(8)] + [192 + 16 + j for j in range(8)]:
+        if dtype == torch.bfloat16:
+            pool.cache.pages[page[at // PAGE], 1, 0, at % PAGE, dim] = value
+        else:
+            j = at % PAGE
+            pool.cache.pages[page[at // PAGE], 1, j * 128 + (((dim >> 4) ^ ((j >> 2) & 7)) << 4) + (dim & 15)] = 0x7f
+        k = pool.cache.read(words(page), n)[0].double()
+        assert k[1, at, dim].isnan() if value != value else k[1, at, dim].isinf()
+        out = ncb.paged_attention(pool.q, pool.cache, pool.plan)[:new]
+        want, size = plain.attention(pool.q[:new].double(), k, pool.v[0], n - new, 0)
+        bad = want.isnan()
+        same = torch.equal(out.isnan(), bad)
+        assert same and bad[:, 4:].any() and not bad[:, :4].any(), at
+        rounding = 2.0 ** -11 if pool.cache.e4m3 else 2.0 ** -8
+        off = (out.double() - want).abs() - 2.0 ** -8 * want.abs() - (rounding + 2.0 ** -14) * size
+        assert off[~bad].max().item() <= 0, at
+        pool.cache.pages.copy_(kept)
