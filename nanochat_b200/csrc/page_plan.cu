@@ -8,6 +8,8 @@
  * request by a binary search in the sums, and one block per window and class makes a schedule of the attention's work (paged.cuh). A step's bytes
  * are a few per row, so the launch is bound by latency: the chain of sums and searches. 64 requests 8 to 10 us, 1,025 requests 12 to 15.
  */
+#include <atomic>
+
 #include "paged.cuh"
 
 namespace {
@@ -58,6 +60,7 @@ struct Requests { /* shared memory, one value a request each */
     int *cached, *served;    /* served: rows, 0 for a request that is not */
     int *owner_end;          /* schedule blocks: inclusive sum of owners */
 };
+constexpr int REQUEST_BYTES = 5 * 4;
 
 /* How long the last block has work if owners are whole: no less than the heaviest, nor than what some block has of the n heaviest, ceil(n * heads / blocks) of them
  * at least, for n down to each of sixteen weights; and hardly more, a request's heaviest going first. (All sorted by weight is slower, eight prompts of 600 rows 48 us
@@ -349,6 +352,20 @@ __global__ void __launch_bounds__(THREADS) k_page_release(const ReleaseArgs a) {
     if (tid == 0) *a.free_count = (int)min(count, (long long)a.n_pages);
 }
 
+/* Opts k_page_plan in to the arrays of the most requests, once per device and whatever the call's size: what a launch may have without is 48 KB for
+ * these and the kernel's own shared memory together. */
+cudaError_t allow_requests() {
+    static std::atomic<unsigned long long> ready{0};
+    int device;
+    cudaError_t rc = cudaGetDevice(&device);
+    if (rc != cudaSuccess) return rc;
+    const unsigned long long bit = device < 64 ? 1ull << device : 0;
+    if (ready.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+    rc = cudaFuncSetAttribute(k_page_plan, cudaFuncAttributeMaxDynamicSharedMemorySize, REQUEST_BYTES * NCB_PLAN_REQUESTS);
+    if (rc == cudaSuccess) ready.fetch_or(bit, std::memory_order_relaxed);
+    return rc;
+}
+
 cudaError_t launch(void (*kernel)(const PlanArgs), int grid, int smem, cudaStream_t stream, const PlanArgs &args) {
     cudaLaunchConfig_t config = {};
     config.gridDim = dim3(grid);
@@ -388,9 +405,8 @@ int page_plan(const ncb_page_plan *args, void *stream) {
     /* a block writes 2,048 rows in about the time that its sums take; more blocks than SMs would repeat them */
     p.row_blocks = (int)((a.rows + 2047) / 2048);
     p.row_blocks = p.row_blocks < 1 ? 1 : p.row_blocks > 64 ? 64 : p.row_blocks;
-    const int smem = 4 * 5 * a.requests;
-    if (smem > 48 * 1024 && cudaFuncSetAttribute(k_page_plan, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return NCB_ERR_LAUNCH;
-    return launch(k_page_plan, p.row_blocks + a.n_windows * (caps.smalls + caps.tiles), smem, (cudaStream_t)stream, p) == cudaSuccess ? NCB_OK : NCB_ERR_LAUNCH;
+    if (allow_requests() != cudaSuccess) return NCB_ERR_LAUNCH;
+    return launch(k_page_plan, p.row_blocks + a.n_windows * (caps.smalls + caps.tiles), REQUEST_BYTES * a.requests, (cudaStream_t)stream, p) == cudaSuccess ? NCB_OK : NCB_ERR_LAUNCH;
 }
 
 int page_release(int *table, int *lens, const int *release, int *free_pages, int *free_count, int requests, int width, int n_pages, int *status,

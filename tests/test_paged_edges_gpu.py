@@ -1,5 +1,9 @@
-"""Edges of the paged operators on the GPU: owners of one tile between owners of two, keys that are not finite.
+"""Edges of the paged operators on the GPU: owners of one tile between owners of two, keys that are not finite, sizes of plans.
 Tolerances as in test_paged_gpu.py."""
+
+import subprocess
+import sys
+from pathlib import Path
 
 import pytest
 import torch
@@ -56,3 +60,15 @@ def test_keys_that_are_not_finite_reach_their_rows(dtype, new, value):
         off = (out.double() - want).abs() - 2.0 ** -8 * want.abs() - (rounding + 2.0 ** -14) * size
         assert off[~bad].max().item() <= 0, at
         pool.cache.pages.copy_(kept)
+
+
+def test_plans_of_every_number_of_requests():
+    """Around the number whose shared memory passes 48 KB with and without what the kernel has besides, in a process that has made no larger plan."""
+    done = subprocess.run([sys.executable, "-c", """
+import torch, nanochat_b200 as ncb
+for n in (2437, 2438, 2450, 2457, 2458, 2459):
+    pages = ncb.PageTable(n, n, 64)
+    plan = ncb.page_plan(pages, pages.lens, torch.ones(n, dtype=torch.int32, device="cuda"), n, max_new=1, Hq=4, Hkv=4)
+    assert plan.pos.eq(0).all() and plan.place.tolist() == [64 * b for b in range(n)], n
+"""], cwd=Path(__file__).parent.parent, capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stderr[-2000:]
