@@ -644,6 +644,9 @@ int delta_step(const ncb_delta *args, int f32, void *stream);
  *                 requests, 64 heads a group.
  *   page_release  requests with release[b] != 0 give back the pages of their lens[b] positions: their entries become -1, lens 0, the
  *                 pages go to the end of the free list. A request whose entries are not in the pool gives back none of those.
+ *   page_trim     request b keeps its first min(keep[b], lens[b]) positions, its new lens[b], and gives back the pages behind them in the same way (a negative
+ *                 keep: NCB_DEV_BAD_LENGTH, it keeps all). A request holds the pages of its lens positions and no others: lengths that go back by
+ *                 any other way leave pages that neither a request nor the list has.
  */
 #define NCB_PLAN_REQUESTS 8192
 #define NCB_PLAN_WINDOWS 8
@@ -659,6 +662,8 @@ long long page_plan_words(int requests, long long rows, int max_fresh, int group
 int page_plan(const ncb_page_plan *args, void *stream);
 int page_release(int *table, int *lens, const int *release, int *free_pages, int *free_count, int requests, int width, int n_pages, int *status,
                  void *stream);
+int page_trim(int *table, int *lens, const int *keep, int *free_pages, int *free_count, int requests, int width, int n_pages, int *status,
+              void *stream);
 
 /* ---- library paged_append ----------------------------------------------------------------------------------------------
  * kv_append_fp8 (same arithmetic, same bits) with a row's k and v stored at place[row] = page * 64 + position % 64 of the pool; bf16 pools

@@ -1,6 +1,7 @@
 /*
  * page_plan: block tables, positions and places of one step from the requests' lengths, on the GPU, so that a captured step serves
- * lengths that change; page_release: finished requests give their pages back. No counterpart in the reference, whose slots are of
+ * lengths that change; page_release: finished requests give their pages back; page_trim: requests whose lengths go back (rejected drafts) give back the
+ * pages behind them. No counterpart in the reference, whose slots are of
  * one size (inference/decoder.py:112-121).
  *
  * Every block repeats the same two prefix sums over the requests (rows, then new pages) in shared memory, 16 KB for a thousand requests,
@@ -306,7 +307,7 @@ __global__ void __launch_bounds__(THREADS) k_page_plan(const PlanArgs args) {
 
 struct ReleaseArgs {
     int *table, *lens;
-    const int *release;
+    const int *release, *keep; /* one of them: requests that keep nothing; positions that each keeps */
     int *free_pages, *free_count;
     int requests, width, n_pages;
     int *status;
@@ -322,11 +323,13 @@ __global__ void __launch_bounds__(THREADS) k_page_release(const ReleaseArgs a) {
     auto valid = [&](int page) { return (unsigned)page < (unsigned)a.n_pages; };
     for (int from = 0; from < a.requests; from += WARPS) { /* a warp per request: its entries are counted, then moved */
         const int b = from + warp;
-        const bool on = b < a.requests && a.release[b] != 0;
-        const int held = on ? min(pages_for(max(a.lens[b], 0)), a.width) : 0;
+        const bool on = b < a.requests && (a.keep || a.release[b] != 0);
+        const int had = on ? max(a.lens[b], 0) : 0, keep = on && a.keep ? a.keep[b] : 0, stay = keep < 0 ? had : min(keep, had);
+        if (keep < 0 && lane == 0) flag(a.status, NCB_DEV_BAD_LENGTH);
+        const int held = min(pages_for(had), a.width), first = min(pages_for(stay), held);
         int *entries = a.table + (size_t)(on ? b : 0) * a.width;
         int good = 0;
-        for (int i = 0; i < held; i += 32) {
+        for (int i = first; i < held; i += 32) {
             const bool in = i + lane < held, ok = in && valid(entries[i + lane]);
             good += __popc(__ballot_sync(0xffffffffu, ok));
             if (in && !ok) flag(a.status, NCB_DEV_BAD_PAGE);
@@ -334,7 +337,7 @@ __global__ void __launch_bounds__(THREADS) k_page_release(const ReleaseArgs a) {
         long long total;
         long long at = count + block_sum_before(lane == 0 ? good : 0, sums, &total);
         at = __shfl_sync(0xffffffffu, at, 0) + good; /* the end of this request's pages in the list */
-        for (int i = 0; i < held; i += 32) {
+        for (int i = first; i < held; i += 32) {
             const int page = i + lane < held ? entries[i + lane] : -1;
             const uint32_t ok = __ballot_sync(0xffffffffu, valid(page));
             if (valid(page)) {
@@ -345,7 +348,7 @@ __global__ void __launch_bounds__(THREADS) k_page_release(const ReleaseArgs a) {
             at -= __popc(ok);
             if (i + lane < held) entries[i + lane] = -1;
         }
-        if (on && lane == 0) a.lens[b] = 0;
+        if (on && lane == 0) a.lens[b] = stay;
         count += total;
     }
     __syncthreads();
@@ -380,6 +383,13 @@ cudaError_t launch(void (*kernel)(const PlanArgs), int grid, int smem, cudaStrea
     return cudaLaunchKernelEx(&config, kernel, args);
 }
 
+int give_back(const ReleaseArgs &a, void *stream) {
+    if (a.requests <= 0 || a.requests > NCB_PLAN_REQUESTS || a.width <= 0 || a.n_pages <= 0) return NCB_ERR_ARG;
+    if (!a.table || !a.lens || (!a.release && !a.keep) || !a.free_pages || !a.free_count) return NCB_ERR_ARG;
+    k_page_release<<<1, THREADS, 0, (cudaStream_t)stream>>>(a);
+    return cudaGetLastError() == cudaSuccess ? NCB_OK : NCB_ERR_LAUNCH;
+}
+
 } /* namespace */
 
 extern "C" {
@@ -411,11 +421,11 @@ int page_plan(const ncb_page_plan *args, void *stream) {
 
 int page_release(int *table, int *lens, const int *release, int *free_pages, int *free_count, int requests, int width, int n_pages, int *status,
                  void *stream) {
-    if (requests <= 0 || requests > NCB_PLAN_REQUESTS || width <= 0 || n_pages <= 0) return NCB_ERR_ARG;
-    if (!table || !lens || !release || !free_pages || !free_count) return NCB_ERR_ARG;
-    const ReleaseArgs a = {table, lens, release, free_pages, free_count, requests, width, n_pages, status};
-    k_page_release<<<1, THREADS, 0, (cudaStream_t)stream>>>(a);
-    return cudaGetLastError() == cudaSuccess ? NCB_OK : NCB_ERR_LAUNCH;
+    return give_back({table, lens, release, nullptr, free_pages, free_count, requests, width, n_pages, status}, stream);
+}
+
+int page_trim(int *table, int *lens, const int *keep, int *free_pages, int *free_count, int requests, int width, int n_pages, int *status, void *stream) {
+    return give_back({table, lens, nullptr, keep, free_pages, free_count, requests, width, n_pages, status}, stream);
 }
 
 } /* extern "C" */

@@ -116,6 +116,7 @@ SIGNATURES = {
         "page_plan_words": ([c_int, c_ll] + [c_int] * 4, c_ll),
         "page_plan": ([c_ptr, c_ptr], c_int),
         "page_release": ([c_ptr] * 5 + [c_int] * 3 + [c_ptr, c_ptr], c_int),
+        "page_trim": ([c_ptr] * 5 + [c_int] * 3 + [c_ptr, c_ptr], c_int),
     },
     "paged_append": {"paged_append": ([c_ptr] * 9 + [c_ll, c_int, c_int, c_ll, c_int, c_int, c_int, c_ptr, c_ptr], c_int)},
     "paged_attn": {

@@ -7,7 +7,7 @@ slots of one size (as the reference does, inference/decoder.py:112-121). One ste
         out = paged_attention(q, cache, plan, window=...)
 
 with any mixture of decoding requests (one fresh token), drafted tokens (a few) and chunks of prompts (hundreds); a finished request's
-pages go back with pages.release(). Lengths stay on the device, so a captured step serves lengths that change. Like attention.py's
+pages go back with pages.release(), those behind rejected drafts with pages.trim(). Lengths stay on the device, so a captured step serves lengths that change. Like attention.py's
 operators, each launches on the current stream and returns without synchronising; a non-zero native status raises
 NativeError, what only the device can see is ORed into `status` (NCB_DEV_* bits)."""
 
@@ -60,7 +60,9 @@ def _layout(requests: int, rows: int, width: int, max_new: int, Hq: int, Hkv: in
 class PageTable:
     """Which pages the requests hold, for the pools of every layer, on the device: `table` int32 (requests, width), -1 where there is
     none; `lens` int32 (requests,), positions held; `free` int32 (n_pages,) and `free_count` int32 (1,), the pages nobody holds.
-    A page belongs to one request. At most 8,192 requests. What changes a table (page_plan, release) is one call after the other."""
+    A page belongs to one request, which holds the pages of its `lens` positions: lengths go up by page_plan and back by trim and release only, since an
+    entry behind a request's length counts as empty and its page would be lost. At most 8,192 requests. What changes a table (page_plan, release, trim) is
+    one call after the other."""
 
     def __init__(self, n_pages: int, requests: int, max_len: int, device: "torch.device | str" = "cuda", table: Tensor | None = None,
                  lens: Tensor | None = None, free: Tensor | None = None, free_count: Tensor | None = None):
@@ -86,11 +88,19 @@ class PageTable:
 
     def release(self, which: Tensor, status: Tensor | None = None) -> None:
         """Requests with which[b] != 0 (int32 (requests,)) give back the pages of their lens[b] positions and hold none."""
-        assert _words(which, self.requests)
-        with on_device_of(self.table, which, status):
-            check(cuda_library("page_plan").page_release(
-                pointer(self.table), pointer(self.lens), pointer(which), pointer(self.free), pointer(self.free_count), self.requests, self.width,
-                self.n_pages, pointer(status), stream()), "page_release")
+        self._give_back("page_release", which, status)
+
+    def trim(self, keep: Tensor, status: Tensor | None = None) -> None:
+        """Request b keeps its first keep[b] positions (int32 (requests,); all that it has where that is more, or negative: NCB_DEV_BAD_LENGTH), its new
+        lens[b], and gives back the pages behind them: after a step of drafts, pages.trim(pages.lens - rejected)."""
+        self._give_back("page_trim", keep, status)
+
+    def _give_back(self, call: str, words: Tensor, status: Tensor | None) -> None:
+        assert _words(words, self.requests)
+        with on_device_of(self.table, words, status):
+            check(getattr(cuda_library("page_plan"), call)(
+                pointer(self.table), pointer(self.lens), pointer(words), pointer(self.free), pointer(self.free_count), self.requests, self.width,
+                self.n_pages, pointer(status), stream()), call)
 
 
 class PagePlan:
@@ -124,8 +134,9 @@ def page_plan(pages: PageTable, cached: Tensor, new: Tensor, rows: int, *, max_n
     """One step's bookkeeping in one launch: request b holds cached[b] positions and adds new[b] (int32 (requests,) on the device, 0 for
     a request that idles), whose rows follow the rows of request b - 1 in the step's `rows` rows. Takes the new pages off pages.free
     into pages.table, and returns the step's PagePlan (`plan`: one of the same sizes to fill again, as a captured step does).
-    max_new: an upper bound of new known to the host (a step that only decodes says 1: longer requests cost attention a launch). lens: where the new lengths go (default: the plan's own; pages.lens, or
-    `cached` itself, to advance them in place); free_left: where the count of free pages goes (default: pages.free_count).
+    max_new: an upper bound of new known to the host (a step that only decodes says 1: longer requests cost attention a launch). lens: where the new lengths go (may be
+    `cached`); free_left: where the count of free pages goes. By default pages.lens and pages.free_count, so that the table is the step's; with free_left elsewhere
+    lens is the plan's own by default, and neither moves: the new pages are in pages.table and still on the list, for a caller who keeps both apart.
     Requests are served in order. One that would need more pages than are left (NCB_DEV_NO_PAGES), or that passes the table's
     width, max_new or `rows` or has a negative length (NCB_DEV_BAD_LENGTH), is not served: it keeps its length, and its rows are idle in the operators below."""
     n = pages.requests
@@ -137,7 +148,7 @@ def page_plan(pages: PageTable, cached: Tensor, new: Tensor, rows: int, *, max_n
             plan = PagePlan(pages, rows, max_new, Hq, Hkv, windows)
         elif plan.pages is not pages or (plan.rows, plan.max_new, plan.Hq, plan.Hkv, plan.windows) != (rows, max_new, Hq, Hkv, tuple(windows)):
             raise ValueError("the plan was made for other sizes or another table")
-        plan.lens = plan.own_lens if lens is None else lens
+        plan.lens = lens if lens is not None else pages.lens if free_left is None else plan.own_lens
         args = Plan.from_buffer_copy(plan._args)  # a call's own
         args.table, args.free_pages, args.free_count, args.ticket = pages.table.data_ptr(), pages.free.data_ptr(), pages.free_count.data_ptr(), pages.ticket.data_ptr()
         args.cached, args.fresh, args.lens = cached.data_ptr(), new.data_ptr(), plan.lens.data_ptr()

@@ -1,0 +1,21 @@
+"""Refusals of the paged operators that need no GPU, beside test_paged_cpu.py."""
+
+import pytest
+import torch
+
+import nanochat_b200 as ncb
+from nanochat_b200 import native
+
+P, NUL = 4096, None  # a non-NULL, aligned stand-in: validation fails before any use
+
+
+def test_page_trim_refuses():
+    trim = native.cuda_library("page_plan").page_trim
+    assert trim(P, P, P, P, P, 0, 8, 32, NUL, NUL) == 1 and trim(P, P, P, P, P, 8193, 8, 32, NUL, NUL) == 1
+    assert trim(P, P, P, P, P, 4, 0, 32, NUL, NUL) == 1 and trim(P, P, P, P, P, 4, 8, 0, NUL, NUL) == 1
+    for i in range(5):
+        assert trim(*[NUL if j == i else P for j in range(5)], 4, 8, 32, NUL, NUL) == 1
+    pages = ncb.PageTable(16, 4, 200, device="cpu")
+    for keep in (torch.zeros(4), torch.zeros(3, dtype=torch.int32), torch.zeros(8, dtype=torch.int32)[::2], torch.zeros(4, dtype=torch.int32)):
+        with pytest.raises(AssertionError):  # the last: not on a GPU
+            pages.trim(keep)

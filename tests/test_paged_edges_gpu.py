@@ -1,10 +1,11 @@
-"""Edges of the paged operators on the GPU: owners of one tile between owners of two, keys that are not finite, sizes of plans.
+"""Edges of the paged operators on the GPU: owners of one tile between owners of two, keys that are not finite, sizes of plans, lengths that go back.
 Tolerances as in test_paged_gpu.py."""
 
 import subprocess
 import sys
 from pathlib import Path
 
+import numpy as np
 import pytest
 import torch
 
@@ -72,3 +73,114 @@ for n in (2437, 2438, 2450, 2457, 2458, 2459):
     assert plan.pos.eq(0).all() and plan.place.tolist() == [64 * b for b in range(n)], n
 """], cwd=Path(__file__).parent.parent, capture_output=True, text=True, timeout=300)
     assert done.returncode == 0, done.stderr[-2000:]
+
+
+def give_back(table, free, held, keep):
+    """trim (release: keep 0) on lists: the entries behind min(keep, held) positions, a request's last page first."""
+    for row, n, k in zip(table, held, keep):
+        first, end = -(-min(k, n) // PAGE), min(-(-n // PAGE), len(row))
+        free += reversed(row[first:end])
+        row[first:end] = [-1] * (end - first)
+
+
+def check_pages(pages, table, free, lens):
+    """The device's table is the lists', and every page is a request's or free, once."""
+    assert pages.table.tolist() == table and pages.lens.tolist() == lens
+    count = pages.free_count.item()
+    assert pages.free[:count].tolist() == free
+    held = [p for row in table for p in row if p >= 0]
+    assert sorted(held + free) == list(range(pages.n_pages)) and len(held) == sum(-(-n // PAGE) for n in lens)
+
+
+@pytest.mark.parametrize("in_place", [True, False])
+def test_rejected_drafts_lose_no_page(in_place):
+    """Steps of up to 70 drafts of which some stay, across borders of pages, with requests that come and go: by default the plan advances the table."""
+    n, n_pages, width = 40, 120, 6
+    rng = np.random.default_rng(7)
+    pages, status = ncb.PageTable(n_pages, n, width * PAGE), words([0])
+    table, free, lens = [[-1] * width for _ in range(n)], list(range(n_pages - 1, -1, -1)), [0] * n
+    for step in range(60):
+        drafts = np.where(rng.random(n) < 0.2, rng.integers(0, 70, n), rng.integers(0, 6, n))
+        new = np.minimum(drafts, [width * PAGE - x for x in lens]).tolist()
+        want, bits = plain.plan(table, lens, new, free, sum(new), 70)
+        plan = ncb.page_plan(pages, pages.lens, words(new), sum(new), max_new=70, Hq=4, Hkv=2, lens=pages.lens if in_place else None, status=status)
+        assert status.item() == bits and plan.lens.tolist() == want["lens"] and plan.place.tolist() == want["place"]
+        status.zero_()
+        table, free, now = want["table"], free[:want["left"]], want["lens"]
+        check_pages(pages, table, free, now)
+        keep = [int(rng.integers(a, b + 1)) for a, b in zip(lens, now)]
+        pages.trim(words(keep), status=status)
+        give_back(table, free, now, keep)
+        lens = keep
+        check_pages(pages, table, free, lens)
+        done = [int(rng.random() < 0.1) for _ in range(n)]
+        pages.release(words(done), status=status)
+        give_back(table, free, lens, [0 if d else x for d, x in zip(done, lens)])
+        lens = [0 if d else x for d, x in zip(done, lens)]
+        check_pages(pages, table, free, lens)
+        assert status.item() == 0
+    pages.trim(words([0] * n))
+    assert pages.free_count.item() == n_pages and not pages.lens.any() and (pages.table == -1).all()
+
+
+def test_trim_keeps_no_more_than_there_is():
+    pages, status = ncb.PageTable(30, 5, 5 * PAGE), words([0])
+    ncb.page_plan(pages, pages.lens, words([300, 64, 65, 0, 128]), 557, max_new=300, Hq=4, Hkv=4)
+    before = pages.table.tolist()
+    pages.trim(words([301, 2 ** 31 - 1, 300, 9, 128]), status=status)  # nothing goes back
+    assert pages.lens.tolist() == [300, 64, 65, 0, 128] and pages.table.tolist() == before and pages.free_count.item() == 30 - 10 and status.item() == 0
+    pages.trim(words([-1, 63, 64, 0, -2 ** 31]), status=status)  # negative ones are flagged and keep all
+    assert pages.lens.tolist() == [300, 63, 64, 0, 128] and status.item() == 4 and pages.free_count.item() == 30 - 9
+    assert pages.table.tolist() == [before[0], before[1], [before[2][0], -1, -1, -1, -1], before[3], before[4]]
+    pages.trim(pages.lens)
+    assert pages.lens.tolist() == [300, 63, 64, 0, 128] and pages.free_count.item() == 30 - 9
+    pages.table[0, 4] = 30  # outside the pool
+    status.zero_()
+    pages.trim(words([256, 0, 64, 0, 0]), status=status)
+    assert status.item() == 16 and pages.lens.tolist() == [256, 0, 64, 0, 0] and pages.free_count.item() == 30 - 5 - 1
+    assert sorted(pages.free[:24].tolist()) == sorted(set(range(30)) - set(before[0][:4]) - {before[2][0]} - {before[0][4]})
+
+
+def test_a_captured_step_of_drafts():
+    """Plan, append, attention and trim in one graph, replayed, against the same eager steps."""
+    Hq, Hkv, gen = 4, 2, torch.Generator().manual_seed(29)
+    cos, sin = ncb.rotary_table(6 * PAGE, 1e4, "cuda")
+    gain = torch.ones(128, device="cuda")
+
+    class Side:
+        def __init__(self):
+            self.pages, self.cache, self.status = ncb.PageTable(30, 4, 6 * PAGE), ncb.PagedKVCache(30, Hkv, torch.bfloat16), words([0])
+            self.new, self.rejected = words([0] * 4), words([0] * 4)
+            self.qkv, self.plan, self.out = torch.zeros(80, (Hq + 2 * Hkv) * 128, dtype=torch.bfloat16, device="cuda"), None, None
+
+        def step(self):
+            self.plan = ncb.page_plan(self.pages, self.pages.lens, self.new, 80, max_new=20, Hq=Hq, Hkv=Hkv, plan=self.plan, status=self.status)
+            q = ncb.paged_append(self.qkv, gain, gain, cos, sin, self.plan.pos, self.plan.place, self.cache, Hq, status=self.status)
+            self.out = ncb.paged_attention(q, self.cache, self.plan, status=self.status)
+            self.pages.trim(self.pages.lens - self.rejected, status=self.status)
+
+    eager, captured = Side(), Side()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        captured.step()  # first-use set-up, all requests idle
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            captured.step()
+    torch.cuda.current_stream().wait_stream(side)
+    rng = np.random.default_rng(3)
+    for i in range(40):
+        new = rng.integers(0, 21, 4)
+        back = np.minimum(new, rng.integers(0, 21, 4))
+        x = torch.randn(80, (Hq + 2 * Hkv) * 128, generator=gen).bfloat16().cuda()
+        for s in (eager, captured):
+            s.new.copy_(words(new.tolist()))
+            s.rejected.copy_(words(back.tolist()))
+            s.qkv.copy_(x)
+        eager.step()
+        graph.replay()
+        assert torch.equal(eager.out[:new.sum()], captured.out[:new.sum()])
+        assert torch.equal(eager.pages.table, captured.pages.table) and torch.equal(eager.pages.lens, captured.pages.lens)
+        held = sum(-(-n // PAGE) for n in eager.pages.lens.tolist())
+        assert eager.pages.free_count.item() == captured.pages.free_count.item() == 30 - held
+    assert eager.status.item() == captured.status.item() == 0
