@@ -75,7 +75,8 @@ class PageTable:
         self.free_count = torch.full((1,), n_pages, **new) if free_count is None else free_count
         assert _words(self.table, requests, self.width) and _words(self.lens, requests)
         assert _words(self.free, n_pages) and _words(self.free_count, 1)
-        self.ticket = torch.zeros(1, **new)
+        assert self.table.device == self.lens.device == self.free.device == self.free_count.device, "a table lives on one device"
+        self.ticket = torch.zeros(1, dtype=torch.int32, device=self.device)
 
     @property
     def device(self) -> torch.device:

@@ -19,3 +19,11 @@ def test_page_trim_refuses():
     for keep in (torch.zeros(4), torch.zeros(3, dtype=torch.int32), torch.zeros(8, dtype=torch.int32)[::2], torch.zeros(4, dtype=torch.int32)):
         with pytest.raises(AssertionError):  # the last: not on a GPU
             pages.trim(keep)
+
+
+@pytest.mark.parametrize("part", ["table", "lens", "free", "free_count"])
+def test_a_table_lives_on_one_device(part):
+    """Kernels take its parts' addresses; a part elsewhere would be an address of another memory."""
+    shape = {"table": (4, 4), "lens": (4,), "free": (16,), "free_count": (1,)}[part]
+    with pytest.raises(AssertionError, match="one device"):
+        ncb.PageTable(16, 4, 200, device="cpu", **{part: torch.zeros(shape, dtype=torch.int32, device="meta")})
