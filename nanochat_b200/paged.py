@@ -218,6 +218,7 @@ def paged_attention(q: Tensor, cache: PagedKVCache, plan: PagePlan, window: int 
             ldo = Hq * HEAD_DIM
     size = plan.workspace_bytes
     if workspace is not None:
+        assert workspace.is_contiguous(), "a workspace is contiguous: its size says what may be written"
         size = workspace.numel() * workspace.element_size()
     elif size:
         workspace = q.new_empty(size, dtype=torch.uint8)

@@ -27,3 +27,15 @@ def test_a_table_lives_on_one_device(part):
     shape = {"table": (4, 4), "lens": (4,), "free": (16,), "free_count": (1,)}[part]
     with pytest.raises(AssertionError, match="one device"):
         ncb.PageTable(16, 4, 200, device="cpu", **{part: torch.zeros(shape, dtype=torch.int32, device="meta")})
+
+
+def test_a_workspace_is_as_large_as_it_says():
+    """An expanded tensor has more elements than memory behind it."""
+    pages = ncb.PageTable(16, 4, 64 * 64, device="cpu")
+    plan = ncb.PagePlan(pages, 8, 8, 8, 2)
+    plan.filled = True
+    cache, q = ncb.PagedKVCache(16, 2, device="cpu"), torch.zeros(8, 8, 128, dtype=torch.bfloat16)
+    assert plan.workspace_bytes > 0
+    for workspace in (torch.zeros(1, dtype=torch.uint8).expand(plan.workspace_bytes), torch.zeros(2 * plan.workspace_bytes, dtype=torch.uint8)[::2]):
+        with pytest.raises(AssertionError, match="contiguous"):
+            ncb.paged_attention(q, cache, plan, workspace=workspace)
