@@ -54,6 +54,12 @@ def attention(q, k, v, first_pos, window):
     return out, size
 
 
+def few_slots_bound(want, size):
+    """What requests of at most 16 query slots may be off over bf16 pages: a result's rounding 2^-8, a probability's two bf16 terms 2^-16 (2^-8 of
+    the first one's 2^-8), scores, sums and exponentials in 32 bits 2^-14."""
+    return 2.0 ** -8 * want.abs() + (2.0 ** -16 + 2.0 ** -14) * size
+
+
 def schedule(words, requests, rows, max_new, group, sms):
     """[(rows an owner has at most, blocks, overhead, least share, [total, share, whole], owners, starts, joins, pieces)] of a schedule's classes."""
     w = np.asarray(words)

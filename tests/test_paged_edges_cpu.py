@@ -5,6 +5,7 @@ import torch
 
 import nanochat_b200 as ncb
 from nanochat_b200 import native
+from tests import paged_cases as plain
 
 P, NUL = 4096, None  # a non-NULL, aligned stand-in: validation fails before any use
 
@@ -39,3 +40,22 @@ def test_a_workspace_is_as_large_as_it_says():
     for workspace in (torch.zeros(1, dtype=torch.uint8).expand(plan.workspace_bytes), torch.zeros(2 * plan.workspace_bytes, dtype=torch.uint8)[::2]):
         with pytest.raises(AssertionError, match="contiguous"):
             ncb.paged_attention(q, cache, plan, workspace=workspace)
+
+
+@pytest.mark.parametrize("terms", [1, 2])
+def test_the_bound_for_few_slots_tells_one_term_from_two(terms):
+    """Attention of few query slots over bf16 pages, restated: probabilities that enter the products as two bf16 terms keep the bound that the
+    GPU's test has for them, one term does not."""
+    gen = torch.Generator().manual_seed(41)
+    q, k, v = (torch.randn(*shape, generator=gen).bfloat16().double() for shape in ((2, 8, 128), (2, 200, 128), (2, 200, 128)))
+    want, size = plain.attention(q, k, v, 198, 0)
+    out = torch.empty_like(want)
+    for i in range(2):
+        kk, vv = (x[:, :199 + i].repeat_interleave(4, 0) for x in (k, v))
+        p = torch.einsum("hd,hkd->hk", q[i], kk) * 128 ** -0.5
+        p = torch.exp(p - p.amax(-1, keepdim=True)).float()
+        hi = p.bfloat16()
+        rounded = hi.double() + ((p - hi.float()).bfloat16().double() if terms == 2 else 0)
+        out[i] = (torch.einsum("hk,hkd->hd", rounded, vv) / p.double().sum(-1, keepdim=True)).bfloat16().double()
+    off = (out - want).abs() - plain.few_slots_bound(want, size)
+    assert (off.max() <= 0) == (terms == 2)

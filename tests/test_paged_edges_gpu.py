@@ -1,4 +1,4 @@
-"""Edges of the paged operators on the GPU: owners of one tile between owners of two, keys that are not finite, sizes of plans, lengths that go back.
+"""Edges of the paged operators on the GPU: owners of one tile between owners of two, keys that are not finite, sizes of plans, lengths that go back, closer bounds.
 Tolerances as in test_paged_gpu.py."""
 
 import subprocess
@@ -184,3 +184,39 @@ def test_a_captured_step_of_drafts():
         held = sum(-(-n // PAGE) for n in eager.pages.lens.tolist())
         assert eager.pages.free_count.item() == captured.pages.free_count.item() == 30 - held
     assert eager.status.item() == captured.status.item() == 0
+
+
+@pytest.mark.parametrize("width", [1, 40])
+@pytest.mark.parametrize("heads", [(4, 4), (8, 2), (12, 1), (16, 1)])
+def test_few_slots_keep_both_terms_of_their_probabilities(heads, width):
+    lens, new = [200, 131, 64, 1, 900], [1, 1, 1, 1, 1] if heads[1] == 1 else [1, 2, 4, 1, 3]
+    pool, plan, q, out = run_attention(torch.bfloat16, *heads, lens, new, seed=19, width=width)
+    at = 0
+    for b, (n, k) in enumerate(zip(lens, new)):
+        want, size = plain.attention(q[at:at + k].double(), pool.k[b], pool.v[b], n - k, 0)
+        assert ((out[at:at + k].double() - want).abs() <= plain.few_slots_bound(want, size)).all()
+        at += k
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("heads", [(8, 2), (2, 2), (16, 1)])
+@pytest.mark.parametrize("new", [1, 4, 20, 33, 150])
+def test_rows_beside_what_they_do_not_see(dtype, heads, new):
+    """A key and a value that are not finite, behind some rows or left behind by their window: the other rows are right, within the bounds of clean calls."""
+    Hq, Hkv = heads
+    n = 200 + new
+    for window, at, clean in ((0, n - 2, range(0, new - 2)), (50, n - new - 49, range(1, new)), (0, n - 1, range(0, new - 1)), (50, 100, range(0, new)), (64, 3, range(0, new))):
+        pool = Pool(dtype, Hq, Hkv, [n], [new], window=window, seed=13)
+        if pool.cache.e4m3:
+            nan, inf = torch.full((Hkv, 1, 128), 0x7f, dtype=torch.uint8), torch.full((Hkv, 1), float("inf"))
+            pool.cache.write(words(pool.table[0]), nan, nan, inf, inf, start=at)
+        else:
+            v = torch.full((Hkv, 1, 128), float("nan"), dtype=torch.bfloat16)
+            v[..., ::2] = float("inf")
+            pool.cache.write(words(pool.table[0]), torch.full_like(v, float("inf")), v, start=at)
+        out = ncb.paged_attention(pool.q, pool.cache, pool.plan, window=window)
+        rounding = 2.0 ** -11 if pool.cache.e4m3 else 2.0 ** -8
+        for i in clean:
+            want, size = plain.attention(pool.q[i:i + 1].double(), pool.k[0], pool.v[0], n - new + i, window)
+            off = (out[i:i + 1].double() - want).abs() - 2.0 ** -8 * want.abs() - (rounding + 2.0 ** -14) * size
+            assert off.max().item() <= 0, (window, at, i)
