@@ -59,3 +59,10 @@ def test_the_bound_for_few_slots_tells_one_term_from_two(terms):
         out[i] = (torch.einsum("hk,hkd->hd", rounded, vv) / p.double().sum(-1, keepdim=True)).bfloat16().double()
     off = (out - want).abs() - plain.few_slots_bound(want, size)
     assert (off.max() <= 0) == (terms == 2)
+
+
+def test_a_pool_says_its_size():
+    """As the slot caches do: pages of a length, bytes of the pool."""
+    assert [ncb.PagedKVCache.pages_for(n) for n in (0, 1, 64, 65, 8191)] == [ncb.Fp8KVCache.pages_for(n) for n in (0, 1, 64, 65, 8191)] == [0, 1, 1, 2, 128]
+    assert ncb.PagedKVCache(5, 3, device="cpu").nbytes() == 5 * 3 * 64 * 264
+    assert ncb.PagedKVCache(5, 3, torch.bfloat16, device="cpu").nbytes() == 5 * 3 * 64 * 512
