@@ -50,11 +50,11 @@ enum {
 
 /* Bits a kernel ORs into the caller's optional device status word (int32, may be NULL). */
 enum {
-    NCB_DEV_BAD_POSITION = 1, /* kv_append_fp8: a row's position or slot is outside the cache; the row was skipped */
-    NCB_DEV_WAIT_TIMEOUT = 2, /* decode_attn_fp8: a bounded wait on a copy barrier ran out; outputs are invalid */
-    NCB_DEV_BAD_LENGTH = 4,   /* decode_attn_fp8: a length or slot is outside the cache; the sequence was skipped */
+    NCB_DEV_BAD_POSITION = 1, /* kv_append_fp8, paged_append: a row's position, slot or place is outside the cache; the row was skipped */
+    NCB_DEV_WAIT_TIMEOUT = 2, /* decode_attn_fp8, paged_attn: a bounded wait ran out; outputs are invalid */
+    NCB_DEV_BAD_LENGTH = 4,   /* decode_attn_fp8: a length or slot is outside the cache; the sequence was skipped. page_plan, page_trim: a length that cannot be */
     NCB_DEV_NO_PAGES = 8,     /* page_plan: the free pages do not last for every request; those behind were not served */
-    NCB_DEV_BAD_PAGE = 16     /* page_plan, paged_*: a page outside the pool in a block table, a free list or a place; it was left out */
+    NCB_DEV_BAD_PAGE = 16     /* page_plan, page_release, page_trim, paged_attn: a page outside the pool in a block table or a free list; it was left out */
 };
 
 const char *ncb_status_string(int status);
@@ -666,7 +666,7 @@ int page_trim(int *table, int *lens, const int *keep, int *free_pages, int *free
               void *stream);
 
 /* ---- library paged_append ----------------------------------------------------------------------------------------------
- * kv_append_fp8 (same arithmetic, same bits) with a row's k and v stored at place[row] = page * 64 + position % 64 of the pool; bf16 pools
+ * kv_append_fp8 (same arithmetic, same bits; no form with value embeddings) with a row's k and v stored at place[row] = page * 64 + position % 64 of the pool; bf16 pools
  * take the rotated keys and the values as they are. A row with a negative position or place is idle: nothing is written for it, q_out
  * included. A position outside the tables or a place outside the pool is flagged and skipped the same way. */
 int paged_append(const void *qkv, const void *q_gain, const void *k_gain, const void *cos, const void *sin, const void *pos, const void *place,
@@ -679,6 +679,9 @@ int paged_append(const void *qkv, const void *q_gain, const void *k_gain, const 
  * page_plan's schedule for this window, made with the same requests, rows, width, max_fresh, group, kv_heads and blocks (any number of calls may read
  * it at once). Requests of at most 16 query slots (new rows x group) and longer ones are different launches; which of them there are follows from
  * max_fresh, so a step that only decodes should say 1. out must not overlap what is read. Rows of requests that were not served become zeros; rows behind the last request are left as they were.
+ * Scores, sums and outputs are fp32 until the one rounding of out. A probability enters its product with the values as f16 (11 bits) over e4m3 pages; over bf16
+ * pages as two bf16 terms (16 bits) where the request has at most 16 query slots and as one (8 bits) where it has more, so that the same row may differ there in
+ * the last bits of bf16; a quarter of the latter come from a cubic within 7.5e-5. A key that is not finite counts by the formula in the rows that see it and reaches no other.
  * workspace: paged_attn_workspace_bytes(), 16-byte aligned, for calls on one stream at a time. */
 typedef struct {
     const void *q, *pool;

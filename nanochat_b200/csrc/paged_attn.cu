@@ -6,7 +6,7 @@
  * k_paged_small, for requests of at most 16 query slots (new rows x the heads of a key/value head's group): bound by the stream of pages. A block of
  * four warps (twelve: see the launch) walks over the pieces of its part of the line (paged.cuh); each warp fetches every fourth unit (an e4m3 page, half a bf16 page) into a place of its
  * own, consumes it and fetches its next: three blocks per SM keep twelve units of 16 KB in flight or in use, and no warp waits for another until the piece ends.
- * 64 requests of 8,191 positions, 32 heads over 8, e4m3: 167 us with the join, 6.6 TB/s; 45 of 130 to 16,384, 16 over 4, bf16: 60 us, 5.6 TB/s. Requests of 17 to 32 slots
+ * 64 requests of 8,191 positions, 32 heads over 8, e4m3: 167 us with the join, 6.6 TB/s; 45 of 130 to 16,384, 16 over 4, bf16: 58.5 us, 5.7 TB/s (device alone; 170 and 61 as calls). Requests of 17 to 32 slots
  * as two owners here in place of tiles: e4m3 41 us for 44, bf16 43 for 40; of 64 slots 75 for 59.
  * The CACHE is the A operand of both products (m16n8k16: 16 keys, or 16 dims of V^T), the slots its 8 columns (two tiles of them for more than 8), so
  * that few slots waste little; score accumulators become the B operand of V^T P by 8 x 8 transposes.

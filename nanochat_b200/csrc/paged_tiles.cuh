@@ -21,8 +21,8 @@
  *     of a launch that widens a request's pages into a workspace of twice the pool's size. Queries are made f16 once per piece, each row times a power of two.
  * Bound by the softmax warps' chain: a page of both tiles takes 2,000 cycles for bf16 pages, 1,300 of them on 64 exponentials a thread (the tensor cores need 1,000, and are 43 %
  * busy), the rest on tensor memory and barriers; 3,000 for e4m3, where 48 scale vectors a thread, the widened pages and the MMAs' operands share the shared memory's bandwidth.
- * 8,190 rows of a prompt, 16 heads over 4, bf16: 243 us, 1,130 TFLOP/s (280 us where such calls fill seconds, and the card's power is bounded); 512 rows behind 16,384 positions,
- * 32 over 8: bf16 138 us, e4m3 200.
+ * 8,190 rows of a prompt, 16 heads over 4, bf16: 240 us, 1,145 TFLOP/s in short runs at 1,965 MHz (280 us where such calls fill seconds, and the card's power is bounded); 512 rows behind 16,384 positions,
+ * 32 over 8: bf16 134 us (154), e4m3 193.
  * A position that a row does not see must not reach it: scores are masked, values are looked at in the pages that the border of some row crosses (three
  * at either end at most), and a page that holds one that is not finite there is multiplied row by row over the positions seen.
  */
@@ -575,7 +575,7 @@ template <bool E4M3, bool TWICE> __global__ void __launch_bounds__(THREADS, 1) k
                                 }
                             }
                             if (cubic) { /* to saturate makes NaN zero: where one of these scores is not finite the sum becomes NaN, and the page is done again without the cubic
-                                          * (here, off the loop's chains: prompt of 8,190 rows 253.6 -> 254.6 us; beside each pair 259.2) */
+                                          * (here, off the loop's chains: prompts of 8,190 rows back to back 253.6 -> 254.6 us; beside each pair 259.2) */
                                 const uint64_t some = att::add2(att::add2(att::pair_of(s[6], s[7]), att::pair_of(s[14], s[15])), att::add2(att::pair_of(s[22], s[23]), att::pair_of(s[30], s[31])));
                                 sum[0] = att::add2(sum[0], att::mul2(some, 0));
                             }

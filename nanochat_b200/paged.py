@@ -165,7 +165,8 @@ def paged_append(qkv: Tensor, q_gain: Tensor, k_gain: Tensor, cos: Tensor, sin: 
                  Hq: int, q_out: Tensor | None = None, status: Tensor | None = None) -> Tensor:
     """kv_append into a pool of pages: norm + rotate q and k, and store k and v at place[row] = page * 64 + position % 64 (a plan's
     pos and place; int32 (rows,), no place twice), quantised to e4m3 with a scale per row and head, or in bf16, as the pool is.
-    Same bits as kv_append. Rows with a negative position or place are idle: nothing is written for them. Returns q_out (rows, Hq, 128) bf16."""
+    Same bits as kv_append without value embeddings, which this has not. Rows with a negative position or place are idle: nothing is written for them. q_out overlaps nothing
+    that is read. Returns q_out (rows, Hq, 128) bf16."""
     (rows, width), Hkv, pages = qkv.shape, cache.kv_heads, cache.pages
     stride, step = qkv.stride()
     assert qkv.dtype is _BF16 and step == 1 and width == (Hq + 2 * Hkv) * HEAD_DIM
@@ -194,7 +195,8 @@ def paged_attention(q: Tensor, cache: PagedKVCache, plan: PagePlan, window: int 
     row at position p attends (p - window, p], or [0, p] with window 0. q (rows, Hq, 128) bf16, heads contiguous, row stride free;
     `window` is one that the plan was made with. Rows of requests that the plan did not serve become zeros; rows behind the last
     request are left as they were in `out`. workspace: uint8, plan.workspace_bytes long, for calls that no other stream overlaps
-    (default: a new one). `out` overlaps nothing that is read. Returns out (rows, Hq, 128) bf16."""
+    (default: a new one). `out` overlaps nothing that is read. Scores and sums are fp32; a probability meets the values as f16 (e4m3 pages), as two bf16 terms (bf16 pages, requests of
+    at most 16 rows times heads a group) or as one (longer ones), so that a row's last bits may depend on how many rows its request has. Returns out (rows, Hq, 128) bf16."""
     rows, Hq, pages = plan.rows, plan.Hq, plan.pages
     shape = (rows, Hq, HEAD_DIM)
     ldq, head, step = q.stride()
